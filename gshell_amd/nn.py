@@ -1,0 +1,162 @@
+"""Layers for networks that the fused SDF network (geometry/mlp.py) and the hash table (render/mlptexture.py) do not cover, on hand-written HIP kernels:
+
+  linear(x, weight, bias, residual, activation)   y = act(x W^T + b) + r with its backward pass   (csrc/linear.hip)
+  Linear                                          torch.nn.Linear with that epilogue; same parameter names, same initialisation
+
+bf16, fp16 and fp32; every sum is 32-bit; a call's sums are taken in a fixed order, so the same inputs give the same bits.  All operands live in HBM: there is no CPU
+fallback.  A call launches on the current stream of its operands' device and keeps nothing between calls.  Gradients can be taken once
+(a second differentiation raises).  Under torch.autocast the operators run in their operands' own type.
+
+A backward pass that is captured into a graph must be the only live graph of its leaves: drop the outputs of eager passes over the same parameters first."""
+import torch
+
+from . import _lib
+from ._lib import GShellHipError, c_float, c_int, c_int64, c_void_p, check
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "softplus": 2, "silu": 3, "gelu": 4}
+
+
+def _p(t):
+    return c_void_p(0 if t is None else t.data_ptr())
+
+
+class _on:
+    """The operands' device as the current one, without the context manager's cost where it is already."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return c_void_p(torch.cuda.current_stream(self.index).cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
+def _rows(t):
+    """`t` [rows, n] with contiguous rows, and the stride between them (a copy only where a row's elements are apart)."""
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _workspace(nbytes, device):
+    if nbytes < 0:
+        raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
+    M, K = x.shape
+    N = weight.shape[0]
+    x, ldx = _rows(x)
+    w, ldw = _rows(weight)
+    b = None if bias is None else bias.contiguous()
+    r, ldr = (None, 0) if residual is None else _rows(residual)
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    dact = torch.empty((M, N), dtype=torch.float16 if x.dtype == torch.bfloat16 else torch.float32, device=x.device) if want_dact and act else None
+    L = _lib.lib()
+    with _on(x.device) as stream:
+        code = _DTYPES[x.dtype]
+        need = L.gs_linear_fwd_workspace_bytes(c_int64(M), c_int64(N), c_int64(K), c_int(code))
+        ws = _workspace(need, x.device)
+        check(L.gs_linear_fwd(_p(x), c_int64(ldx), _p(w), c_int64(ldw), _p(b), _p(r), c_int64(ldr), c_int64(M), c_int64(N), c_int64(K), c_int(code), c_int(act),
+                              c_float(beta), _p(y), c_int64(N), _p(dact), _p(ws), c_int64(need), stream), "gs_linear_fwd")
+    return y, dact
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, beta):
+        need = ctx.needs_input_grad
+        y, dact = _linear_forward(x, weight, bias, residual, act, beta, need[0] or need[1] or need[2])
+        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, dact)
+        ctx.sizes = (x.shape[0], weight.shape[0], x.shape[1])
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, dact = ctx.saved_tensors
+        M, N, K = ctx.sizes
+        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if want_x or want_w or want_b:
+            gr, ldg = _rows(g)
+            x, ldx = _rows(x) if x is not None else (None, 0)
+            weight, ldw = _rows(weight) if weight is not None else (None, 0)
+            new = lambda *shape: torch.empty(shape, dtype=g.dtype, device=g.device)      # noqa: E731
+            dx, dw, db = new(M, K) if want_x else None, new(N, K) if want_w else None, new(N) if want_b else None
+            L = _lib.lib()
+            with _on(g.device) as stream:
+                code = _DTYPES[g.dtype]
+                need = L.gs_linear_bwd_workspace_bytes(c_int64(M), c_int64(N), c_int64(K), c_int(code), c_int(dact is not None), c_int(want_x), c_int(want_w), c_int(want_b))
+                ws = _workspace(need, g.device)
+                check(L.gs_linear_bwd(_p(gr), c_int64(ldg), _p(dact), _p(x), c_int64(ldx), _p(weight), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K), c_int(code),
+                                      _p(dx), _p(dw), _p(db), _p(ws), c_int64(need), stream), "gs_linear_bwd")
+        return dx, dw, db, g if want_r else None, None, None
+
+
+def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
+    """act(x W^T + b) + r: x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N].
+
+    activation: None, "relu", "softplus" (log(1 + exp(beta z)) / beta), "silu" or "gelu" (erf form).  The residual is added behind the activation and has the
+    output's shape (an expanded view may stand for it).  All operands have one type (float32, bfloat16, float16) and one device; x, weight and residual may be views whose rows are
+    any stride apart.  fp32 operands keep fp32's accuracy.  Where the gradient is taken of an activation, act'(z) is kept for the backward pass: 2 bytes an output
+    for bf16, 4 for the others."""
+    if activation not in ACTIVATIONS:
+        raise GShellHipError(f"linear: activation {activation!r} is not one of {sorted(k for k in ACTIVATIONS if k)} or None")
+    act = ACTIVATIONS[activation]
+    beta = float(beta)
+    if act == 2 and not 0.0 < beta < 1e30:
+        raise GShellHipError(f"linear: softplus needs a positive finite beta, got {beta}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise GShellHipError(f"linear: x [..., K] and weight [N, K] are wanted, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N, K = weight.shape
+    shape = x.shape[:-1] + (N,)
+    if bias is not None and bias.shape != (N,):
+        raise GShellHipError(f"linear: bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise GShellHipError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)}")
+    if x.dtype not in _DTYPES:
+        raise GShellHipError(f"linear: float32, bfloat16 or float16 operands are wanted, got {x.dtype}")
+    operands = (("x", x), ("weight", weight), ("bias", bias), ("residual", residual))
+    for name, t in operands:
+        if t is not None and t.dtype != x.dtype:
+            raise GShellHipError(f"linear: {name} is {t.dtype}, x is {x.dtype}")
+    for name, t in operands:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise GShellHipError(f"linear: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
+        if t.device != x.device:
+            raise GShellHipError(f"linear: {name} is on {t.device}, x on {x.device}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0)
+    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(x2.shape[0], N)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for _, t in operands):
+        y = _LinearFn.apply(x2, weight, bias, r2, act, beta)
+    else:
+        y, _ = _linear_forward(x2, weight, bias, r2, act, beta, False)
+    return y if x.dim() == 2 else y.reshape(shape)
+
+
+class Linear(torch.nn.Linear):
+    """torch.nn.Linear (same parameters, initialisation and state_dict) with an activation, and a residual that a call may hand over."""
+
+    def __init__(self, in_features, out_features, bias=True, activation=None, beta=1.0, device=None, dtype=None):
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        if activation not in ACTIVATIONS:
+            raise GShellHipError(f"Linear: activation {activation!r} is not one of {sorted(k for k in ACTIVATIONS if k)} or None")
+        self.activation, self.beta = activation, beta
+
+    def forward(self, x, residual=None):
+        return linear(x, self.weight, self.bias, residual, self.activation, self.beta)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", activation={self.activation}"

@@ -855,6 +855,25 @@ int gs_flexi_cut_bwd(const int64_t* pa, const int64_t* pb, int64_t n, const floa
                      const float* nu_d_sv, const float* g_bverts, const float* g_bnu, float* g_vd, float* g_nu_d,
                      float* g_nu_d_sv, gs_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Dense layer with its epilogue   (torch.nn.Linear + activation + residual as the reference's networks stack them, geometry/mlp.py:7-40)
+ *   z = x W^T + b,  y = act(z) + r:  x [M,K], W [N,K], b [N], r, y [M,N]; rows may be any stride apart (ld*, in elements), a row's
+ *   elements are contiguous.  dtype: 0 fp32, 1 bf16, 2 fp16, of every operand; sums are 32-bit.  act: 0 none, 1 relu, 2 softplus
+ *   log(1 + exp(beta z)) / beta, 3 silu, 4 gelu (erf form).  bias, residual may be null.
+ *   dact [M,N] (contiguous; fp16 for bf16 layers, fp32 otherwise; null = not wanted) receives act'(z) for gs_linear_bwd.
+ *   gs_linear_bwd: gz = g act'(z) -> dx = gz W [M,K], dW = gz^T x [N,K], db = column sums of gz; any of the three may be null.
+ *   dact null = no activation.  Sums are taken in a fixed order: the same bits every time.
+ *   The workspaces are the caller's and hold nothing between calls.
+ * ---------------------------------------------------------------------------------- */
+int64_t gs_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
+                  int64_t M, int64_t N, int64_t K, int dtype, int act, float beta, void* y, int64_t ldy, void* dact,
+                  void* workspace, int64_t workspace_bytes, gs_stream_t stream);
+int64_t gs_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int has_dact, int want_x, int want_w, int want_b);
+int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                  int64_t M, int64_t N, int64_t K, int dtype, void* dx, void* dw, void* db, void* workspace,
+                  int64_t workspace_bytes, gs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
