@@ -1,0 +1,461 @@
+// GS_CXXFLAGS: -Xclang -target-feature -Xclang -packed-fp32-ops
+// Table lookup with scaling, and its gradient by sorted row numbers (gfx950).
+//
+//     y_t = s W[id_t]                      dW_v = s sum_{t: id_t = v} g_t   (rows that no id names: zero)
+//
+// The gradient's sums run over the tokens of a row in their order, in 32 bits, and do not depend on how the launch is scheduled: the tokens are sorted by row
+// (a stable radix sort of our own), then every CHUNK neighbours of the sorted list are summed by one group of lanes.  A run of equal rows inside a chunk is written at once;
+// one that crosses chunks leaves a part in each and is joined in a second launch, so that a row that holds most of the tokens is spread over the chip as well.
+// No atomics, no pass over the table but the one that writes it.
+// An id outside of [0, V) (which the host cannot see without waiting for the GPU) reads nothing: its output row is NaN and it has no gradient.
+#include <hip/hip_runtime.h>
+
+#include "../../include/gshell_hip.h"
+#include "common.hpp"
+
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr int MAX_BITS = 9, MAX_BINS = 1 << MAX_BITS;
+constexpr int SORT_BLOCKS = 64;              // tiles of the sort: few enough that every tile adds up all tiles' counts by itself
+constexpr int SMALL_T = 2048, SMALL_BITS = 8;          // tokens that one workgroup sorts in LDS, in one launch
+constexpr int CHUNK = 32;
+
+template <typename I> __device__ __forceinline__ uint32_t key_of(I id, int64_t V, int64_t padding) {
+    const int64_t v = (int64_t)id;
+    return v < 0 || v >= V || v == padding ? (uint32_t)V : (uint32_t)v;          // V: sorted behind every row, summed into none
+}
+
+// Exclusive prefix sums of one value a thread, and their total.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* tmp, uint32_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+    }
+    if (lane == 63) tmp[wave] = s;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+    for (int w = 0; w < SORT_WAVES; ++w) {
+        if (w < wave) before += tmp[w];
+        total += tmp[w];
+    }
+    __syncthreads();
+    return before + s - v;
+}
+
+// Lanes of this wave that hold the same digit (among the active ones)
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool active) {
+    uint64_t m = __ballot(active);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t one = __ballot((digit >> b) & 1);
+        m &= (digit >> b) & 1 ? one : ~one;
+    }
+    return m;
+}
+
+// Each wave counts the digits of its own stretch [w0, w1) of the list; counts[wave][bin]
+template <typename F> __device__ __forceinline__ void wave_counts(F key, int64_t w0, int64_t w1, int shift, int bits, uint32_t* counts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << bits;
+    for (int b = threadIdx.x; b < SORT_WAVES * bins; b += SORT_THREADS) counts[b] = 0;
+    __syncthreads();
+    for (int64_t i = w0; i < w1; i += 64) {
+        const bool ok = i + lane < w1;
+        if (ok) atomicAdd(&counts[wave * bins + ((key(i + lane) >> shift) & (bins - 1))], 1u);
+    }
+    __syncthreads();
+}
+
+// Stable scatter of the wave's stretch; counts[wave][bin] holds the first free place of (wave, bin) and moves on
+template <typename F, typename G> __device__ __forceinline__ void wave_scatter(F key, G put, int64_t w0, int64_t w1, int shift, int bits, uint32_t* counts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, bins = 1 << bits;
+    for (int64_t i = w0; i < w1; i += 64) {
+        const bool ok = i + lane < w1;
+        const uint32_t k = ok ? key(i + lane) : 0, digit = (k >> shift) & (bins - 1);
+        const uint64_t same = same_digit(digit, bits, ok);
+        if (ok) {
+            uint32_t* c = &counts[wave * bins + digit];
+            const uint32_t at = *c + __popcll(same & ((1ull << lane) - 1));
+            put(i + lane, k, at);
+            // every lane of a digit has read its counter before the last of them moves it: they run in step, and the wave is the counter's only user
+            __builtin_amdgcn_wave_barrier();
+            if ((same >> lane) == 1) *c = at + 1;
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+template <typename I>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const I* ids, const uint32_t* keys, int64_t T, int64_t V, int64_t padding, int64_t tile, int shift, int bits, uint32_t* hist) {
+    __shared__ uint32_t counts[MAX_BINS];
+    const int bins = 1 << bits;
+    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) counts[b] = 0;
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * tile, t1 = t0 + tile < T ? t0 + tile : T;
+    for (int64_t i = t0 + threadIdx.x; i < t1; i += SORT_THREADS) {
+        const uint32_t k = ids ? key_of(ids[i], V, padding) : keys[i];
+        atomicAdd(&counts[(k >> shift) & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) hist[b * SORT_BLOCKS + blockIdx.x] = counts[b];
+}
+
+template <typename I>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(const I* ids, const uint32_t* keys, const uint32_t* pos, int64_t T, int64_t V, int64_t padding, int64_t tile,
+                                                              int shift, int bits, const uint32_t* hist, uint32_t* keys_out, uint32_t* pos_out) {
+    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], tmp[SORT_WAVES];
+    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t t0 = (int64_t)blockIdx.x * tile, t1 = t0 + tile < T ? t0 + tile : T;
+    const int64_t stretch = (tile / SORT_WAVES + 63) / 64 * 64;
+    const int64_t w0 = t0 + wave * stretch < t1 ? t0 + wave * stretch : t1, w1 = w0 + stretch < t1 ? w0 + stretch : t1;
+    const auto key = [&](int64_t i) { return ids ? key_of(ids[i], V, padding) : keys[i]; };
+    wave_counts(key, w0, w1, shift, bits, counts);
+    uint32_t before = 0, all = 0;          // of this thread's bin: tokens in earlier tiles, in all tiles
+    if ((int)threadIdx.x < bins) {
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+            const uint32_t c = hist[threadIdx.x * SORT_BLOCKS + b];
+            before += b < (int)blockIdx.x ? c : 0;
+            all += c;
+        }
+    }
+    uint32_t total;
+    uint32_t at = block_scan(all, tmp, total) + before;
+    if ((int)threadIdx.x < bins)
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            const uint32_t c = counts[w * bins + threadIdx.x];
+            counts[w * bins + threadIdx.x] = at;
+            at += c;
+        }
+    __syncthreads();
+    wave_scatter(key, [&](int64_t i, uint32_t k, uint32_t to) { keys_out[to] = k; pos_out[to] = ids ? (uint32_t)i : pos[i]; }, w0, w1, shift, bits, counts);
+}
+
+// the whole sort of a short list by one workgroup
+template <typename I>
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_small(const I* ids, int T, int64_t V, int64_t padding, int total_bits, uint32_t* keys_out, uint32_t* pos_out) {
+    __shared__ uint32_t keys[2][SMALL_T], counts[SORT_WAVES << SMALL_BITS], tmp[SORT_WAVES];
+    __shared__ uint16_t pos[2][SMALL_T];
+    for (int i = threadIdx.x; i < T; i += SORT_THREADS) keys[0][i] = key_of(ids[i], V, padding), pos[0][i] = (uint16_t)i;
+    __syncthreads();
+    const int wave = threadIdx.x >> 6;
+    const int stretch = ((T + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;
+    const int w0 = wave * stretch < T ? wave * stretch : T, w1 = w0 + stretch < T ? w0 + stretch : T;
+    int from = 0;
+    for (int shift = 0; shift < total_bits; shift += SMALL_BITS) {
+        const int bits = total_bits - shift < SMALL_BITS ? total_bits - shift : SMALL_BITS, bins = 1 << bits;
+        const uint32_t* kin = keys[from];
+        const uint16_t* pin = pos[from];
+        uint32_t* kout = keys[from ^ 1];
+        uint16_t* pout = pos[from ^ 1];
+        const auto key = [&](int64_t i) { return kin[i]; };
+        wave_counts(key, w0, w1, shift, bits, counts);
+        uint32_t all = 0, total;
+        if ((int)threadIdx.x < bins)
+            for (int w = 0; w < SORT_WAVES; ++w) all += counts[w * bins + threadIdx.x];
+        uint32_t at = block_scan(all, tmp, total);
+        if ((int)threadIdx.x < bins)
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const uint32_t c = counts[w * bins + threadIdx.x];
+                counts[w * bins + threadIdx.x] = at;
+                at += c;
+            }
+        __syncthreads();
+        wave_scatter(key, [&](int64_t i, uint32_t k, uint32_t to) { kout[to] = k; pout[to] = pin[i]; }, w0, w1, shift, bits, counts);
+        __syncthreads();
+        from ^= 1;
+    }
+    for (int i = threadIdx.x; i < T; i += SORT_THREADS) keys_out[i] = keys[from][i], pos_out[i] = pos[from][i];
+}
+
+// VEC neighbouring values of a row (rows may start at any element; the hardware loads unaligned vectors)
+template <typename T, int VEC> struct __attribute__((packed)) Pack { T v[VEC]; };
+
+template <typename T, int VEC, typename U> __device__ __forceinline__ void load_row(const T* p, int64_t left, U (&out)[VEC]) {
+    if (left >= VEC) {
+        const Pack<T, VEC> q = *(const Pack<T, VEC>*)p;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out[k] = (U)q.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out[k] = k < left ? (U)p[k] : (U)0.f;
+    }
+}
+template <typename T, int VEC, typename U> __device__ __forceinline__ void store_row(T* p, int64_t left, const U (&in)[VEC]) {
+    if (left >= VEC) {
+        Pack<T, VEC> q;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) q.v[k] = (T)in[k];
+        *(Pack<T, VEC>*)p = q;
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            if (k < left) p[k] = (T)in[k];
+    }
+}
+
+// Forward: a group of 2^group_log lanes takes one (token, stretch of columns).
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) k_lookup(const I* ids, const T* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, float scale, T* y) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
+    if (unit >= tokens * stretches) return;
+    const int64_t t = unit / stretches, c = ((unit % stretches) << group_log) * VEC + (threadIdx.x & ((1 << group_log) - 1)) * VEC;
+    if (c >= D) return;
+    const int64_t id = (int64_t)ids[t];
+    float v[VEC];
+    if (id < 0 || id >= V) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = __builtin_nanf("");
+    } else {
+        load_row<T, VEC>(w + id * ldw + c, D - c, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] *= scale;
+    }
+    store_row<T, VEC>(y + t * D + c, D - c, v);
+}
+
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+    int64_t lo = 0, hi = n;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (keys[mid] < key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+constexpr int BVEC = 4;          // columns of a lane in the gradient's sums
+
+// Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
+template <typename T>
+__global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int group_log,
+                                                    int64_t stretches, int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
+    if ((int64_t)blockIdx.x >= sum_blocks) {
+        const int lane = threadIdx.x & 63;
+        const int64_t v0 = (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, v = v0 + lane;
+        if (v0 >= V) return;
+        bool empty = false;
+        if (v < V) {
+            const int64_t at = lower_bound(keys, tokens, (uint32_t)v);
+            empty = at >= tokens || keys[at] != (uint32_t)v;
+        }
+        const float zero[BVEC] = {};
+        for (uint64_t m = __ballot(empty); m; m &= m - 1) {
+            T* row = dw + (v0 + (__ffsll((unsigned long long)m) - 1)) * D;
+            for (int64_t c = lane * BVEC; c < D; c += 64 * BVEC) store_row<T, BVEC>(row + c, D - c, zero);
+        }
+        return;
+    }
+    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
+    if (unit >= chunks * stretches) return;
+    const int64_t chunk = unit / stretches, c = ((unit % stretches) << group_log) * BVEC + (threadIdx.x & ((1 << group_log) - 1)) * BVEC;
+    if (c >= D) return;
+    const int64_t e0 = chunk * CHUNK, e1 = e0 + CHUNK < tokens ? e0 + CHUNK : tokens;
+    const uint32_t none = (uint32_t)V;
+    const uint32_t before = e0 > 0 ? keys[e0 - 1] : none, after = e1 < tokens ? keys[e1] : none;
+    uint32_t run = keys[e0];
+    bool head = true;          // the run began with the chunk
+    float acc[BVEC] = {};
+    const auto flush = [&](bool end) {
+        if (run == none) return;
+        if (head && run == before) store_row<float, BVEC>(first + chunk * D + c, D - c, acc);
+        else if (end && run == after) store_row<float, BVEC>(last + chunk * D + c, D - c, acc);
+        else {
+            float out[BVEC];
+#pragma unroll
+            for (int k = 0; k < BVEC; ++k) out[k] = acc[k] * scale;
+            store_row<T, BVEC>(dw + (int64_t)run * D + c, D - c, out);
+        }
+    };
+    for (int64_t e = e0; e < e1; e += 8) {
+        uint32_t key[8];
+        float v[8][BVEC];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) key[k] = e + k < e1 ? keys[e + k] : none;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (key[k] != none) load_row<T, BVEC>(g + (int64_t)pos[e + k] * ldg + c, D - c, v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (e + k >= e1) break;
+            if (key[k] != run) {
+                flush(false);
+                run = key[k], head = false;
+#pragma unroll
+                for (int q = 0; q < BVEC; ++q) acc[q] = 0.f;
+            }
+            if (key[k] != none)
+#pragma unroll
+                for (int q = 0; q < BVEC; ++q) acc[q] += v[k][q];
+        }
+    }
+    flush(true);
+}
+
+// Runs that cross chunks, in the order of their chunks: the chunk where a run begins joins it.  A workgroup takes one (chunk, stretch); its groups of lanes share
+// the run's chunks out in equal stretches.
+template <typename T>
+__global__ void __launch_bounds__(256) k_join_chunks(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, float scale, const float* first,
+                                                     const float* last, T* dw) {
+    __shared__ float part[256 * BVEC];
+    const int64_t chunk = blockIdx.x / stretches, e1 = (chunk + 1) * CHUNK;
+    if (e1 >= tokens) return;
+    const uint32_t run = keys[e1 - 1];
+    if (run == (uint32_t)V || keys[e1] != run) return;
+    if (keys[chunk * CHUNK] == run && chunk > 0 && keys[chunk * CHUNK - 1] == run) return;          // it began earlier
+    const int64_t end = lower_bound(keys, tokens, run + 1), more = (end - 1) / CHUNK - chunk;          // chunks behind this one that hold a part
+    const int groups = 256 >> group_log, group = threadIdx.x >> group_log;
+    const int64_t c = (((int64_t)(blockIdx.x % stretches) << group_log) + (threadIdx.x & ((1 << group_log) - 1))) * BVEC;
+    const int64_t share = (more + groups - 1) / groups, k0 = group * share, k1 = k0 + share < more ? k0 + share : more;
+    float acc[BVEC] = {};
+    if (c < D) {
+        for (int64_t k = k0; k < k1; k += 4) {
+            float v[4][BVEC];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + u < k1) load_row<float, BVEC>(first + (chunk + 1 + k + u) * D + c, D - c, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + u < k1)
+#pragma unroll
+                    for (int q = 0; q < BVEC; ++q) acc[q] += v[u][q];
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < BVEC; ++q) part[threadIdx.x * BVEC + q] = acc[q];
+    __syncthreads();
+    if (group != 0 || c >= D) return;
+    float sum[BVEC];
+    load_row<float, BVEC>(last + chunk * D + c, D - c, sum);
+    for (int s = 0; s < groups; ++s)
+#pragma unroll
+        for (int q = 0; q < BVEC; ++q) sum[q] += part[((s << group_log) + threadIdx.x) * BVEC + q];
+#pragma unroll
+    for (int q = 0; q < BVEC; ++q) sum[q] *= scale;
+    store_row<T, BVEC>(dw + (int64_t)run * D + c, D - c, sum);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
+static int group_log_of(int64_t vectors) {
+    int l = 0;
+    while (l < 6 && (1ll << l) < vectors) ++l;
+    return l;
+}
+
+struct SortPlan {
+    int64_t keys[2], pos[2], hist, first, last, total, chunks;
+};
+static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+static SortPlan sort_plan(int64_t T, int64_t D) {
+    SortPlan p;
+    int64_t at = 0;
+    for (int k = 0; k < 2; ++k) {
+        p.keys[k] = at, at += align256(T * 4);
+        p.pos[k] = at, at += align256(T * 4);
+    }
+    p.hist = at, at += MAX_BINS * SORT_BLOCKS * 4;
+    p.chunks = gs::cdiv(T, CHUNK);
+    p.first = at, at += align256(p.chunks * D * 4);
+    p.last = at, at += align256(p.chunks * D * 4);
+    p.total = at;
+    return p;
+}
+
+template <typename T, typename I>
+int lookup(const void* ids, const void* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, float scale, void* y, hipStream_t stream) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int64_t vectors = gs::cdiv(D, VEC);
+    const int gl = group_log_of(vectors);
+    const int64_t stretches = gs::cdiv(vectors, 1ll << gl), blocks = gs::cdiv((tokens * stretches) << gl, 256);
+    GS_REQUIRE(blocks < (1ll << 31), "gs_embedding_fwd: too large");
+    hipLaunchKernelGGL((k_lookup<T, I>), dim3((unsigned)blocks), dim3(256), 0, stream, (const I*)ids, (const T*)w, ldw, tokens, V, D, gl, stretches, scale, (T*)y);
+    GS_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename I> int sort_tokens(const void* ids, int64_t T, int64_t V, int64_t padding, const SortPlan& p, char* base, uint32_t*& keys, uint32_t*& pos, hipStream_t stream) {
+    int bits = 1;
+    while ((1ll << bits) <= V) ++bits;
+    keys = (uint32_t*)(base + p.keys[0]), pos = (uint32_t*)(base + p.pos[0]);
+    if (T <= SMALL_T) {
+        hipLaunchKernelGGL(k_sort_small<I>, dim3(1), dim3(SORT_THREADS), 0, stream, (const I*)ids, (int)T, V, padding, bits, keys, pos);
+        GS_LAUNCH_CHECK();
+        return 0;
+    }
+    uint32_t* hist = (uint32_t*)(base + p.hist);
+    const int passes = (bits + MAX_BITS - 1) / MAX_BITS, each = (bits + passes - 1) / passes;
+    int64_t tile = gs::cdiv(T, SORT_BLOCKS);
+    if (tile < SORT_THREADS) tile = SORT_THREADS;
+    tile = (tile + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;          // whole rounds of the workgroup: its waves' stretches cover the tile
+    const unsigned blocks = (unsigned)gs::cdiv(T, tile);
+    const I* in = (const I*)ids;
+    const uint32_t *kin = nullptr, *pin = nullptr;
+    for (int q = 0, shift = 0; q < passes; ++q, shift += each) {
+        const int b = bits - shift < each ? bits - shift : each;
+        keys = (uint32_t*)(base + p.keys[q & 1]), pos = (uint32_t*)(base + p.pos[q & 1]);
+        hipLaunchKernelGGL(k_sort_count<I>, dim3(blocks), dim3(SORT_THREADS), 0, stream, in, kin, T, V, padding, tile, shift, b, hist);
+        hipLaunchKernelGGL(k_sort_scatter<I>, dim3(blocks), dim3(SORT_THREADS), 0, stream, in, kin, pin, T, V, padding, tile, shift, b, (const uint32_t*)hist, keys, pos);
+        in = nullptr, kin = keys, pin = pos;
+    }
+    GS_LAUNCH_CHECK();
+    return 0;
+}
+
+template <typename T, typename I>
+int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t padding, float scale, void* dw, char* base, hipStream_t stream) {
+    const SortPlan p = sort_plan(tokens, D);
+    uint32_t *keys = nullptr, *pos = nullptr;
+    if (tokens > 0)
+        if (const int rc = sort_tokens<I>(ids, tokens, V, padding, p, base, keys, pos, stream)) return rc;
+    const int64_t vectors = gs::cdiv(D, BVEC);
+    const int gl = group_log_of(vectors);
+    const int64_t stretches = gs::cdiv(vectors, 1ll << gl), sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256), zero_blocks = gs::cdiv(V, 256);
+    GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31) && p.chunks * stretches < (1ll << 31), "gs_embedding_bwd: too large");
+    float *first = (float*)(base + p.first), *last = (float*)(base + p.last);
+    hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
+                       gl, stretches, p.chunks, sum_blocks, scale, (T*)dw, first, last);
+    if (p.chunks > 1)
+        hipLaunchKernelGGL(k_join_chunks<T>, dim3((unsigned)(p.chunks * stretches)), dim3(256), 0, stream, (const uint32_t*)keys, tokens, V, D, gl, stretches, scale,
+                           (const float*)first, (const float*)last, (T*)dw);
+    GS_LAUNCH_CHECK();
+    return 0;
+}
+
+static bool sizes_ok(int64_t T, int64_t V, int64_t D) {
+    const int64_t top = (1ll << 31) - 1;
+    return T >= 0 && V >= 0 && D >= 0 && T < top && V < top && D < top;
+}
+
+}  // namespace
+
+extern "C" int gs_embedding_fwd(const void* ids, int ids64, const void* weight, int64_t ldw, int64_t T, int64_t V, int64_t D, int dtype, float scale, void* y, gs_stream_t stream) {
+    GS_REQUIRE(sizes_ok(T, V, D), "gs_embedding_fwd: sizes are 0 .. 2^31 - 2");
+    GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_embedding_fwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (T == 0 || D == 0) return 0;
+    GS_REQUIRE(ids && y && (weight || V == 0) && ldw >= 0, "gs_embedding_fwd: null argument");
+    const auto run = dtype == 0 ? (ids64 ? lookup<float, int64_t> : lookup<float, int32_t>) : dtype == 1 ? (ids64 ? lookup<bf16, int64_t> : lookup<bf16, int32_t>)
+                                                                                            : (ids64 ? lookup<f16, int64_t> : lookup<f16, int32_t>);
+    return run(ids, weight, ldw, T, V, D, scale, y, (hipStream_t)stream);
+}
+
+extern "C" int64_t gs_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) { return sizes_ok(T, V, D) ? sort_plan(T, D).total : -1; }
+
+extern "C" int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64_t ldg, int64_t T, int64_t V, int64_t D, int64_t padding_idx, int dtype, float scale, void* dw,
+                                void* workspace, int64_t workspace_bytes, gs_stream_t stream) {
+    GS_REQUIRE(sizes_ok(T, V, D), "gs_embedding_bwd: sizes are 0 .. 2^31 - 2");
+    GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_embedding_bwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    if (V == 0 || D == 0) return 0;
+    GS_REQUIRE(dw && (T == 0 || (ids && g && ldg >= 0)), "gs_embedding_bwd: null argument");
+    GS_REQUIRE(workspace && workspace_bytes >= sort_plan(T, D).total, "gs_embedding_bwd: workspace too small");
+    const auto run = dtype == 0 ? (ids64 ? gradient<float, int64_t> : gradient<float, int32_t>) : dtype == 1 ? (ids64 ? gradient<bf16, int64_t> : gradient<bf16, int32_t>)
+                                                                                             : (ids64 ? gradient<f16, int64_t> : gradient<f16, int32_t>);
+    return run(ids, g, ldg, T, V, D, padding_idx, scale, dw, (char*)workspace, (hipStream_t)stream);
+}

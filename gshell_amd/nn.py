@@ -2,6 +2,8 @@
 
   linear(x, weight, bias, residual, activation)   y = act(x W^T + b) + r with its backward pass   (csrc/linear.hip)
   Linear                                          torch.nn.Linear with that epilogue; same parameter names, same initialisation
+  embedding(ids, weight, scale, padding_idx)      y_t = scale W[id_t], gradient by sorted ids             (csrc/embedding.hip)
+  Embedding                                       torch.nn.Embedding's parameters and initialisation, with the scale
 
 bf16, fp16 and fp32; every sum is 32-bit; a call's sums are taken in a fixed order, so the same inputs give the same bits.  All operands live in HBM: there is no CPU
 fallback.  A call launches on the current stream of its operands' device and keeps nothing between calls.  Gradients can be taken once
@@ -160,3 +162,80 @@ class Linear(torch.nn.Linear):
 
     def extra_repr(self):
         return super().extra_repr() + f", activation={self.activation}"
+
+
+_ID_TYPES = {torch.int64: 1, torch.int32: 0}
+
+
+def _lookup(ids, weight, scale):
+    w, ldw = _rows(weight)
+    V, D = w.shape
+    y = torch.empty((ids.numel(), D), dtype=w.dtype, device=w.device)
+    with _on(w.device) as stream:
+        check(_lib.lib().gs_embedding_fwd(_p(ids), c_int(_ID_TYPES[ids.dtype]), _p(w), c_int64(ldw), c_int64(ids.numel()), c_int64(V), c_int64(D), c_int(_DTYPES[w.dtype]),
+                                          c_float(scale), _p(y), stream), "gs_embedding_fwd")
+    return y
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.rest = (weight.shape, scale, padding_idx)
+        return _lookup(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        (V, D), scale, padding_idx = ctx.rest
+        g, ldg = _rows(g)
+        T = ids.numel()
+        dw = torch.empty((V, D), dtype=g.dtype, device=g.device)
+        L = _lib.lib()
+        with _on(g.device) as stream:
+            need = L.gs_embedding_bwd_workspace_bytes(c_int64(T), c_int64(V), c_int64(D))
+            ws = _workspace(need, g.device)
+            check(L.gs_embedding_bwd(_p(ids), c_int(_ID_TYPES[ids.dtype]), _p(g), c_int64(ldg), c_int64(T), c_int64(V), c_int64(D), c_int64(padding_idx), c_int(_DTYPES[g.dtype]),
+                                     c_float(scale), _p(dw), _p(ws), c_int64(need), stream), "gs_embedding_bwd")
+        return None, dw, None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """scale * weight[ids]: ids int64 or int32 of any shape, weight [V, D] (float32, bfloat16, float16) -> ids.shape + [D].
+
+    The gradient sums a row's tokens in their order in 32 bits: the same bits every time.  The row `padding_idx` gets none.  Ids are not looked at on the host: one outside
+    of [0, V) gives a row of NaN and has no gradient (negative ids do not count from the end)."""
+    if weight.dim() != 2 or weight.dtype not in _DTYPES:
+        raise GShellHipError(f"embedding: a weight [V, D] of float32, bfloat16 or float16 is wanted, got {tuple(weight.shape)} {weight.dtype}")
+    if ids.dtype not in _ID_TYPES:
+        raise GShellHipError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
+    if max(ids.numel(), *weight.shape) >= (1 << 31) - 1:
+        raise GShellHipError("embedding: sizes are 0 .. 2^31 - 2")
+    if padding_idx is None:
+        padding_idx = -1
+    elif not 0 <= padding_idx < weight.shape[0]:
+        raise GShellHipError(f"embedding: padding_idx {padding_idx} is not a row of the table of {weight.shape[0]}")
+    scale = float(scale)
+    for name, t in (("ids", ids), ("weight", weight)):
+        if not t.is_cuda:
+            raise GShellHipError(f"embedding: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
+    if ids.device != weight.device:
+        raise GShellHipError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
+    flat = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        y = _EmbeddingFn.apply(flat, weight, scale, int(padding_idx))
+    else:
+        y = _lookup(flat, weight, scale)
+    return y if ids.dim() == 1 else y.view(ids.shape + (weight.shape[1],))
+
+
+class Embedding(torch.nn.Embedding):
+    """torch.nn.Embedding (same parameter, initialisation and state_dict) whose rows come out scaled."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, device=None, dtype=None):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
+        self.scale = scale
+
+    def forward(self, ids):
+        return embedding(ids, self.weight, self.scale, self.padding_idx)

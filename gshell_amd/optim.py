@@ -2,9 +2,12 @@
 
 Same constructor, parameter groups, schedulers and state_dict as torch.optim.Adam(fused=True) -- the state is the fused optimiser's
 (`step` a float32 device scalar per parameter, `exp_avg`, `exp_avg_sq`), so checkpoints move freely between the two -- and the same
-arithmetic (ATen/native/cuda/fused_adam_utils.cuh).  The reference trains with torch.optim.Adam (train_gshelltet_deepfashion.py:372-383)."""
+arithmetic (ATen/native/cuda/fused_adam_utils.cuh).  The reference trains with torch.optim.Adam (train_gshelltet_deepfashion.py:372-383).
+
+And the gradient's global norm with clipping by it, two HIP launches over all tensors (csrc/gradnorm.hip: gs_grad_norm): grad_norm, clip_grads, clip_grad_norm_."""
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -80,3 +83,127 @@ class HipAdam(torch.optim.Adam):
         super().load_state_dict(state_dict)
         for st in self.state.values():
             st["_host_step"] = None
+
+
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_TYPES = {2.0: 0, 1.0: 1, float("inf"): 2}
+
+
+def _norm_code(norm_type, what):
+    code = _NORM_TYPES.get(float(norm_type))
+    if code is None:
+        raise _lib.GShellHipError(f"{what}: norm_type is 2, 1 or inf, got {norm_type}")
+    return code
+
+
+def _check_grads(tensors, what):
+    """One device for all, dense, of a known type -- on the host, before anything is launched."""
+    for t in tensors:
+        if t.layout is not torch.strided or t.dtype not in _GRAD_TYPES:
+            raise _lib.GShellHipError(f"{what}: dense float32, bfloat16 or float16 tensors are wanted, got {t.dtype} ({t.layout})")
+    for t in tensors:
+        if not t.is_cuda:
+            raise _lib.GShellHipError(f"{what}: tensors must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
+        if t.device != tensors[0].device:
+            raise _lib.GShellHipError(f"{what}: tensors are on {tensors[0].device} and on {t.device}")
+
+
+def _spans(tensors):
+    at = np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+    size = np.array([t.numel() * t.element_size() for t in tensors], dtype=np.int64)
+    return at, size
+
+
+def _check_apart(written, read, what):
+    """No two written tensors share memory, and none shares it with a tensor that is read, unless it is that tensor's own place."""
+    at, size = _spans(written)
+    order = np.argsort(at[size > 0], kind="stable")
+    a, z = at[size > 0][order], size[size > 0][order]
+    if (a[:-1] + z[:-1] > a[1:]).any():
+        raise _lib.GShellHipError(f"{what}: two of the tensors that are written share memory")
+    if read is None or len(a) == 0:
+        return
+    r_at, r_size = _spans(read)
+    own = r_at == at
+    r_at, r_size = r_at[(r_size > 0) & ~own], r_size[(r_size > 0) & ~own]
+    if len(r_at):
+        # the last written span that starts before a read one ends must end before it starts
+        k = np.searchsorted(a, r_at + r_size, side="left") - 1
+        if ((k >= 0) & (a[k] + z[k] > r_at)).any():
+            raise _lib.GShellHipError(f"{what}: an output shares memory with another gradient")
+
+
+def _launch_norm(tensors, out, max_norm, code, norm):
+    n = len(tensors)
+    vp = ctypes.c_void_p * n
+    L = _lib.lib()
+    dev = norm.device
+    with torch.cuda.device(dev):
+        need = L.gs_grad_norm_workspace_bytes(c_int(n))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(L.gs_grad_norm(c_int(n), vp(*[t.data_ptr() for t in tensors]), vp(*[t.data_ptr() for t in out]) if out is not None else None,
+                             (ctypes.c_int64 * n)(*[t.numel() for t in tensors]), (ctypes.c_int32 * n)(*[_GRAD_TYPES[t.dtype] for t in tensors]), c_int(code),
+                             ctypes.c_float(max_norm), _lib.ptr(norm), _lib.ptr(ws), ctypes.c_int64(need), stream()), "gs_grad_norm")
+
+
+@torch.no_grad()
+def grad_norm(tensors, norm_type=2.0):
+    """The norm (2, 1 or inf) of all elements of `tensors` together, one fp32 value on their device; summed in 64 bits."""
+    code = _norm_code(norm_type, "grad_norm")
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        return torch.zeros(())
+    _check_grads(tensors, "grad_norm")
+    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
+    norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+    _launch_norm(tensors, None, 0.0, code, norm)
+    return norm
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)) -> norm, one fp32 value on the device.  Without `out`, in place.
+
+    `out`: tensors of the gradients' shapes and types; one may be its gradient's own place, otherwise no output shares memory with a gradient or another output.  A norm that
+    is NaN makes every output NaN, one that is infinite makes finite elements zero."""
+    code = _norm_code(norm_type, "clip_grads")
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise _lib.GShellHipError(f"clip_grads: max_norm must not be negative or NaN, got {max_norm}")
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    if len(out) != len(grads):
+        raise _lib.GShellHipError(f"clip_grads: {len(grads)} gradients and {len(out)} outputs")
+    for g, o in zip(grads, out):
+        if o is not g and (o.shape != g.shape or o.dtype != g.dtype):
+            raise _lib.GShellHipError(f"clip_grads: an output is {tuple(o.shape)} {o.dtype}, its gradient {tuple(g.shape)} {g.dtype}")
+    if not grads:
+        return torch.zeros(())
+    _check_grads(grads, "clip_grads")
+    if out is not grads:
+        _check_grads(out, "clip_grads")
+        if out[0].device != grads[0].device:
+            raise _lib.GShellHipError(f"clip_grads: gradients are on {grads[0].device}, outputs on {out[0].device}")
+    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(s) for g, o, s in zip(grads, out, src)]
+    _check_apart(dst, None if out is grads else src, "clip_grads")
+    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    _launch_norm(src, dst, max_norm, code, norm)
+    for o, d in zip(out, dst):
+        if d is not o:
+            o.copy_(d)
+    torch.autograd.graph.increment_version([o for o, d in zip(out, dst) if d is o])
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ over parameters whose gradients live on one device: clips their .grad in place, returns the norm before (one fp32 value).
+
+    `error_if_nonfinite` waits for the norm and raises before anything is scaled."""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in params if p.grad is not None]
+    if error_if_nonfinite:
+        norm = grad_norm(grads, norm_type)
+        if not torch.isfinite(norm):
+            raise RuntimeError(f"clip_grad_norm_: the norm of order {float(norm_type)} is not finite, so the gradients cannot be clipped")
+    return clip_grads(grads, max_norm, norm_type)

@@ -874,6 +874,29 @@ int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, i
                   int64_t M, int64_t N, int64_t K, int dtype, void* dx, void* dw, void* db, void* workspace,
                   int64_t workspace_bytes, gs_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Table lookup with scaling, and its gradient by sorted row numbers
+ *   fwd: y [T,D] = scale * weight[ids], weight [V,D] with rows ldw elements apart; ids int64 (ids64 = 1) or int32.
+ *   bwd: dw [V,D] (written whole, unnamed rows zero) = scale * sum of g's rows (ldg apart) by id, in the order of the tokens, in 32 bits: the same
+ *        bits every time.  padding_idx: a row without gradient (-1: none).  An id outside [0, V) gives a NaN row and no gradient.
+ *   dtype as for gs_linear_fwd.
+ * ---------------------------------------------------------------------------------- */
+int gs_embedding_fwd(const void* ids, int ids64, const void* weight, int64_t ldw, int64_t T, int64_t V, int64_t D, int dtype,
+                     float scale, void* y, gs_stream_t stream);
+int64_t gs_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D);
+int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64_t ldg, int64_t T, int64_t V, int64_t D, int64_t padding_idx,
+                     int dtype, float scale, void* dw, void* workspace, int64_t workspace_bytes, gs_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Global norm of a list of gradients, and clipping by it   (torch.nn.utils.clip_grad_norm_ in the train script, :440-444)
+ *   norm (one fp32 on the device) = (sum |g|^p)^(1/p), summed in 64 bits; norm_type 0: p = 2, 1: p = 1, 2: the largest magnitude.
+ *   out not null: out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type; out[k] may be grads[k].
+ *   Host arrays of device pointers, element counts and dtypes (0 fp32, 1 bf16, 2 fp16); tensors are contiguous and may start at any element.
+ * ---------------------------------------------------------------------------------- */
+int64_t gs_grad_norm_workspace_bytes(int n_tensors);
+int gs_grad_norm(int n_tensors, const void* const* grads, void* const* out, const int64_t* numel, const int32_t* dtypes,
+                 int norm_type, float max_norm, float* norm, void* workspace, int64_t workspace_bytes, gs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,3 +58,66 @@ def test_linear_c_entry_refuses_bad_arguments():
     assert fwd(M=0) == 0
     assert L.gs_linear_fwd_workspace_bytes(i(-1), i(1), i(1), c_int(0)) == -1
     assert L.gs_linear_bwd_workspace_bytes(i(1), i(1), i(1), c_int(9), c_int(0), c_int(1), c_int(1), c_int(1)) == -1
+
+
+def test_embedding_refuses():
+    w, ids = torch.zeros(5, 4), torch.zeros(3, dtype=torch.int64)
+    for a, b, kw, what in ((ids, w[0], {}, "weight"), (ids, w.double(), {}, "weight"), (ids.float(), w, {}, "ids"), (ids.to(torch.int16), w, {}, "ids"),
+                           (ids, w, dict(padding_idx=5), "padding_idx"), (ids, w, dict(padding_idx=-1), "padding_idx"), (ids, w, {}, "HBM")):
+        with pytest.raises(GShellHipError, match=what):
+            nn.embedding(a, b, **kw)
+    assert set(nn.Embedding(5, 4).state_dict()) == {"weight"}
+
+
+def test_embedding_c_entry_refuses_bad_arguments():
+    from gshell_amd import _lib
+    from gshell_amd._lib import c_float, c_int, c_int64, c_void_p
+    L, i, n, p = _lib.lib(), c_int64, c_void_p(0), c_void_p(256)
+    for T, V, D, dtype, ids in ((-1, 4, 4, 0, p), (4, 1 << 31, 4, 0, p), (4, 4, -1, 0, p), (4, 4, 4, 3, p), (4, 4, 4, 0, n)):
+        assert L.gs_embedding_fwd(ids, c_int(1), p, i(4), i(T), i(V), i(D), c_int(dtype), c_float(1), p, n) != 0
+        assert L.gs_embedding_bwd(ids, c_int(1), p, i(4), i(T), i(V), i(D), i(-1), c_int(dtype), c_float(1), p, p, i(1 << 40), n) != 0
+    assert L.gs_embedding_bwd(p, c_int(1), p, i(4), i(4), i(4), i(4), i(-1), c_int(0), c_float(1), p, p, i(16), n) != 0 and b"workspace" in L.gs_last_error()
+    assert L.gs_embedding_bwd_workspace_bytes(i(-1), i(4), i(4)) == -1
+    assert L.gs_embedding_fwd(n, c_int(1), n, i(4), i(0), i(4), i(4), c_int(0), c_float(1), n, n) == 0
+
+
+def test_clip_refuses():
+    from gshell_amd import optim
+    g = [torch.zeros(4), torch.zeros(5)]
+    for kw, what in ((dict(max_norm=-1.0), "max_norm"), (dict(max_norm=float("nan")), "max_norm"), (dict(max_norm=1.0, norm_type=3.0), "norm_type"),
+                     (dict(max_norm=1.0, out=[g[0]]), "outputs"), (dict(max_norm=1.0, out=[torch.zeros(4), torch.zeros(6)]), "output"),
+                     (dict(max_norm=1.0, out=[torch.zeros(4), torch.zeros(5).half()]), "output"), (dict(max_norm=1.0), "HBM")):
+        with pytest.raises(GShellHipError, match=what):
+            optim.clip_grads(g, **kw)
+    with pytest.raises(GShellHipError, match="float32"):
+        optim.grad_norm([torch.zeros(4, dtype=torch.float64)])
+    with pytest.raises(GShellHipError, match="float32"):
+        optim.grad_norm([torch.zeros(4, 4).to_sparse()])
+    assert float(optim.clip_grads([], 1.0)) == 0.0 and float(optim.grad_norm([])) == 0.0
+
+
+def test_clip_refuses_shared_memory():
+    """The check by addresses is the same on any device."""
+    from gshell_amd import optim
+    t = torch.zeros(100)
+    for written, read in (([t[:50], t[49:]], None), ([t, t], None), ([t[10:20], t[0:11]], None), ([t[0:10]], [t[5:15]]), ([t[0:10], t[50:60]], [t[0:10], t[55:65]]),
+                          ([t[0:100]], [t[99:]])):
+        with pytest.raises(GShellHipError, match="memory"):
+            optim._check_apart(written, read, "clip_grads")
+    for written, read in (([t[:50], t[50:]], None), ([t[:50], t[:0], t[50:]], None), ([t[0:10]], [t[10:20]]), ([t[10:20]], [t[0:10]]), ([t[0:10], t[50:60]], [t[0:10], t[60:70]]),
+                          ([t[:0]], [t[:0]])):
+        optim._check_apart(written, read, "clip_grads")
+
+
+def test_clip_c_entry_refuses_bad_arguments():
+    import ctypes
+    from gshell_amd import _lib
+    from gshell_amd._lib import c_float, c_int, c_int64, c_void_p
+    L, n, p = _lib.lib(), c_void_p(0), c_void_p(256)
+
+    def call(ptr=256, numel=4, dtype=0, kind=0, max_norm=1.0, norm=p, ws=1 << 20, out=256):
+        return L.gs_grad_norm(c_int(1), (ctypes.c_void_p * 1)(ptr), (ctypes.c_void_p * 1)(out), (ctypes.c_int64 * 1)(numel), (ctypes.c_int32 * 1)(dtype), c_int(kind),
+                              c_float(max_norm), norm, p, c_int64(ws), n)
+    for kw in (dict(ptr=None), dict(out=None), dict(numel=-1), dict(dtype=3), dict(dtype=-1), dict(kind=3), dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(norm=n), dict(ws=8)):
+        assert call(**kw) != 0 and b"gs_grad_norm" in L.gs_last_error(), kw
+    assert L.gs_grad_norm_workspace_bytes(c_int(-1)) == -1
