@@ -66,7 +66,7 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
     L = _lib.lib()
     with _on(x.device) as stream:
         code = _DTYPES[x.dtype]
-        need = L.gs_linear_fwd_workspace_bytes(c_int64(M), c_int64(N), c_int64(K), c_int(code))
+        need = L.gs_linear_fwd_workspace_bytes(_p(x), c_int64(ldx), _p(w), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K), c_int(code))
         ws = _workspace(need, x.device)
         check(L.gs_linear_fwd(_p(x), c_int64(ldx), _p(w), c_int64(ldw), _p(b), _p(r), c_int64(ldr), c_int64(M), c_int64(N), c_int64(K), c_int(code), c_int(act),
                               c_float(beta), _p(y), c_int64(N), _p(dact), _p(ws), c_int64(need), stream), "gs_linear_fwd")
@@ -98,7 +98,8 @@ class _LinearFn(torch.autograd.Function):
             L = _lib.lib()
             with _on(g.device) as stream:
                 code = _DTYPES[g.dtype]
-                need = L.gs_linear_bwd_workspace_bytes(c_int64(M), c_int64(N), c_int64(K), c_int(code), c_int(dact is not None), c_int(want_x), c_int(want_w), c_int(want_b))
+                need = L.gs_linear_bwd_workspace_bytes(_p(gr), c_int64(ldg), c_int(dact is not None), _p(x), c_int64(ldx), _p(weight), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K),
+                                                       c_int(code), c_int(want_x), c_int(want_w), c_int(want_b))
                 ws = _workspace(need, g.device)
                 check(L.gs_linear_bwd(_p(gr), c_int64(ldg), _p(dact), _p(x), c_int64(ldx), _p(weight), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K), c_int(code),
                                       _p(dx), _p(dw), _p(db), _p(ws), c_int64(need), stream), "gs_linear_bwd")

@@ -863,13 +863,16 @@ int gs_flexi_cut_bwd(const int64_t* pa, const int64_t* pb, int64_t n, const floa
  *   dact [M,N] (contiguous; fp16 for bf16 layers, fp32 otherwise; null = not wanted) receives act'(z) for gs_linear_bwd.
  *   gs_linear_bwd: gz = g act'(z) -> dx = gz W [M,K], dW = gz^T x [N,K], db = column sums of gz; any of the three may be null.
  *   dact null = no activation.  Sums are taken in a fixed order: the same bits every time.
- *   The workspaces are the caller's and hold nothing between calls.
+ *   The workspaces are the caller's and hold nothing between calls; their sizes go by the addresses and strides too (16-bit operands
+ *   whose rows do not start on 16 bytes are repacked first).
  * ---------------------------------------------------------------------------------- */
-int64_t gs_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int64_t gs_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K,
+                                      int dtype);
 int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr,
                   int64_t M, int64_t N, int64_t K, int dtype, int act, float beta, void* y, int64_t ldy, void* dact,
                   void* workspace, int64_t workspace_bytes, gs_stream_t stream);
-int64_t gs_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int has_dact, int want_x, int want_w, int want_b);
+int64_t gs_linear_bwd_workspace_bytes(const void* g, int64_t ldg, int has_dact, const void* x, int64_t ldx, const void* weight,
+                                      int64_t ldw, int64_t M, int64_t N, int64_t K, int dtype, int want_x, int want_w, int want_b);
 int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int64_t ldx, const void* weight, int64_t ldw,
                   int64_t M, int64_t N, int64_t K, int dtype, void* dx, void* dw, void* db, void* workspace,
                   int64_t workspace_bytes, gs_stream_t stream);

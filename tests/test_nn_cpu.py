@@ -56,8 +56,8 @@ def test_linear_c_entry_refuses_bad_arguments():
     for kw in (dict(M=-1), dict(N=1 << 31), dict(dtype=3), dict(act=5), dict(act=2, beta=0.0), dict(x=n), dict(y=n), dict(ldy=3), dict(M=1, N=1, K=100000)):
         assert fwd(**kw) != 0 and b"gs_linear" in L.gs_last_error(), kw
     assert fwd(M=0) == 0
-    assert L.gs_linear_fwd_workspace_bytes(i(-1), i(1), i(1), c_int(0)) == -1
-    assert L.gs_linear_bwd_workspace_bytes(i(1), i(1), i(1), c_int(9), c_int(0), c_int(1), c_int(1), c_int(1)) == -1
+    assert L.gs_linear_fwd_workspace_bytes(p, i(8), p, i(8), i(-1), i(1), i(1), c_int(0)) == -1
+    assert L.gs_linear_bwd_workspace_bytes(p, i(8), c_int(0), p, i(8), p, i(8), i(1), i(1), i(1), c_int(9), c_int(1), c_int(1), c_int(1)) == -1
 
 
 def test_embedding_refuses():
