@@ -17,6 +17,10 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "gshell_hip.h")
 
 _lib = None
 
+# Entry points that are called with plain Python numbers and addresses: their argument types are declared, because a ctypes object for each argument would cost more
+# than the call.  The other gs_* functions take ctypes objects.
+PLAIN_CALLS = ("gs_linear_", "gs_embedding_", "gs_grad_norm")
+
 c_void_p, c_int64, c_int, c_float = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 
 
@@ -24,16 +28,30 @@ class GShellHipError(RuntimeError):
     pass
 
 
-def declared_prototypes():
-    """{name: return type} of every entry point declared in the public header."""
+def _prototypes():
     with open(HEADER_PATH) as f:
         src = f.read()
     src = re.sub(r"/\*.*?\*/", "", src, flags=re.S)
-    return {m.group(2): m.group(1) for m in re.finditer(r"\b(int64_t|int|const char\s*\*)\s+(gs_[a-z0-9_]+)\s*\(", src)}
+    return {m.group(2): (m.group(1), m.group(3)) for m in re.finditer(r"\b(int64_t|int|const char\s*\*)\s+(gs_[a-z0-9_]+)\s*\(([^;]*)\)\s*;", src)}
+
+
+def declared_prototypes():
+    """{name: return type} of every entry point declared in the public header."""
+    return {name: ret for name, (ret, _) in _prototypes().items()}
 
 
 def declared_symbols():
     return sorted(declared_prototypes())
+
+
+def _declare(L):
+    """Return types of every entry point, argument types of PLAIN_CALLS, from the public header."""
+    L.gs_last_error.restype = ctypes.c_char_p
+    for name, (ret, args) in _prototypes().items():
+        fn = getattr(L, name)          # AttributeError if the .so lacks a declared symbol
+        fn.restype = {"int": c_int, "int64_t": c_int64}.get(ret, ctypes.c_char_p)
+        if name.startswith(PLAIN_CALLS):
+            fn.argtypes = [c_void_p if "*" in a or "gs_stream_t" in a else c_int64 if "int64_t" in a else c_float if "float" in a else c_int for a in args.split(",")]
 
 
 def lib():
@@ -47,19 +65,13 @@ def lib():
             _lib = ctypes.CDLL(LIB_PATH)
         except OSError as e:  # pragma: no cover
             raise GShellHipError(f"failed to load {LIB_PATH}: {e}") from e
-        _lib.gs_last_error.restype = ctypes.c_char_p
-        for name, ret in declared_prototypes().items():
-            fn = getattr(_lib, name)          # AttributeError if the .so lacks a declared symbol
-            fn.restype = {"int": c_int, "int64_t": c_int64}.get(ret, ctypes.c_char_p)
+        _declare(_lib)
     return _lib
 
 
 def _load(path):
     L = ctypes.CDLL(path)
-    L.gs_last_error.restype = ctypes.c_char_p
-    for name, ret in declared_prototypes().items():
-        fn = getattr(L, name)
-        fn.restype = {"int": c_int, "int64_t": c_int64}.get(ret, ctypes.c_char_p)
+    _declare(L)
     return L
 
 

@@ -13,45 +13,34 @@ A backward pass that is captured into a graph must be the only live graph of its
 import torch
 
 from . import _lib
-from ._lib import GShellHipError, c_float, c_int, c_int64, c_void_p, check
+from ._lib import GShellHipError, check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "softplus": 2, "silu": 3, "gelu": 4}
+# The calls below are short next to what Python spends around them: plain numbers and addresses go to the C functions (_lib.PLAIN_CALLS), and the current device is
+# changed only where it is another one.
 
 
-def _p(t):
-    return c_void_p(0 if t is None else t.data_ptr())
+def _on(index, call):
+    """call(stream) with device `index` as the current one."""
+    before = torch.cuda.current_device()
+    if before == index:
+        return call(torch.cuda.current_stream(index).cuda_stream)
+    with torch.cuda.device(index):
+        return call(torch.cuda.current_stream(index).cuda_stream)
 
 
-class _on:
-    """The operands' device as the current one, without the context manager's cost where it is already."""
-
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return c_void_p(torch.cuda.current_stream(self.index).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _rows(t):
     """`t` [rows, n] with contiguous rows, and the stride between them (a copy only where a row's elements are apart)."""
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    ld, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
         t = t.contiguous()
-    return t, t.stride(0)
-
-
-def _workspace(nbytes, device):
-    if nbytes < 0:
-        raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        ld = t.stride(0)
+    return t, ld
 
 
 def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
@@ -59,18 +48,49 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
     N = weight.shape[0]
     x, ldx = _rows(x)
     w, ldw = _rows(weight)
-    b = None if bias is None else bias.contiguous()
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     r, ldr = (None, 0) if residual is None else _rows(residual)
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    dact = torch.empty((M, N), dtype=torch.float16 if x.dtype == torch.bfloat16 else torch.float32, device=x.device) if want_dact and act else None
+    y = x.new_empty((M, N))
+    code = _DTYPES[x.dtype]
+    dact = x.new_empty((M, N), dtype=torch.float16 if code == 1 else torch.float32) if want_dact and act else None
     L = _lib.lib()
-    with _on(x.device) as stream:
-        code = _DTYPES[x.dtype]
-        need = L.gs_linear_fwd_workspace_bytes(_p(x), c_int64(ldx), _p(w), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K), c_int(code))
-        ws = _workspace(need, x.device)
-        check(L.gs_linear_fwd(_p(x), c_int64(ldx), _p(w), c_int64(ldw), _p(b), _p(r), c_int64(ldr), c_int64(M), c_int64(N), c_int64(K), c_int(code), c_int(act),
-                              c_float(beta), _p(y), c_int64(N), _p(dact), _p(ws), c_int64(need), stream), "gs_linear_fwd")
+    xp, wp = x.data_ptr(), w.data_ptr()
+    need = L.gs_linear_fwd_workspace_bytes(xp, ldx, wp, ldw, M, N, K, code)
+    if need < 0:
+        raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    check(_on(x.get_device(), lambda stream: L.gs_linear_fwd(xp, ldx, wp, ldw, _at(b), _at(r), ldr, M, N, K, code, act, beta, y.data_ptr(), N,
+                                                             _at(dact), _at(ws), need, stream)), "gs_linear_fwd")
     return y, dact
+
+
+def _linear_backward(ctx, g):
+    x, weight, dact = ctx.saved_tensors
+    M, N, K = ctx.sizes
+    want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
+    dx = dw = db = None
+    if want_x or want_w or want_b:
+        gr, ldg = _rows(g)
+        xp = ldx = wp = ldw = 0
+        if want_w:
+            x, ldx = _rows(x)
+            xp = x.data_ptr()
+            dw = gr.new_empty((N, K))
+        if want_x:
+            weight, ldw = _rows(weight)
+            wp = weight.data_ptr()
+            dx = gr.new_empty((M, K))
+        if want_b:
+            db = gr.new_empty(N)
+        L = _lib.lib()
+        gp, dp, code = gr.data_ptr(), _at(dact), _DTYPES[gr.dtype]
+        need = L.gs_linear_bwd_workspace_bytes(gp, ldg, dact is not None, xp, ldx, wp, ldw, M, N, K, code, want_x, want_w, want_b)
+        if need < 0:
+            raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
+        ws = gr.new_empty(need, dtype=torch.uint8) if need else None
+        check(_on(gr.get_device(), lambda stream: L.gs_linear_bwd(gp, ldg, dp, xp, ldx, wp, ldw, M, N, K, code, _at(dx), _at(dw),
+                                                                  _at(db), _at(ws), need, stream)), "gs_linear_bwd")
+    return dx, dw, db, g if want_r else None, None, None
 
 
 class _LinearFn(torch.autograd.Function):
@@ -83,27 +103,43 @@ class _LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, weight, dact = ctx.saved_tensors
-        M, N, K = ctx.sizes
-        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if want_x or want_w or want_b:
-            gr, ldg = _rows(g)
-            x, ldx = _rows(x) if x is not None else (None, 0)
-            weight, ldw = _rows(weight) if weight is not None else (None, 0)
-            new = lambda *shape: torch.empty(shape, dtype=g.dtype, device=g.device)      # noqa: E731
-            dx, dw, db = new(M, K) if want_x else None, new(N, K) if want_w else None, new(N) if want_b else None
-            L = _lib.lib()
-            with _on(g.device) as stream:
-                code = _DTYPES[g.dtype]
-                need = L.gs_linear_bwd_workspace_bytes(_p(gr), c_int64(ldg), c_int(dact is not None), _p(x), c_int64(ldx), _p(weight), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K),
-                                                       c_int(code), c_int(want_x), c_int(want_w), c_int(want_b))
-                ws = _workspace(need, g.device)
-                check(L.gs_linear_bwd(_p(gr), c_int64(ldg), _p(dact), _p(x), c_int64(ldx), _p(weight), c_int64(ldw), c_int64(M), c_int64(N), c_int64(K), c_int(code),
-                                      _p(dx), _p(dw), _p(db), _p(ws), c_int64(need), stream), "gs_linear_bwd")
-        return dx, dw, db, g if want_r else None, None, None
+        return _once(_linear_backward, ctx, g)
+
+
+_once_differentiable = torch.autograd.function.once_differentiable
+
+
+def _once(body, ctx, g):
+    """A backward pass that cannot be differentiated again: where that is asked for (create_graph), its results carry a node that says so."""
+    return _once_differentiable(body)(ctx, g) if torch.is_grad_enabled() else body(ctx, g)
+
+
+def _linear_refuse(x, weight, bias, residual, activation, beta):
+    """What is wrong with a call's operands, said in full."""
+    if activation not in ACTIVATIONS:
+        raise GShellHipError(f"linear: activation {activation!r} is not one of {sorted(k for k in ACTIVATIONS if k)} or None")
+    if activation == "softplus" and not 0.0 < beta < 1e30:
+        raise GShellHipError(f"linear: softplus needs a positive finite beta, got {beta}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise GShellHipError(f"linear: x [..., K] and weight [N, K] are wanted, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and bias.shape != (N,):
+        raise GShellHipError(f"linear: bias must be [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise GShellHipError(f"linear: residual must have the output's shape {tuple(x.shape[:-1]) + (N,)}, got {tuple(residual.shape)}")
+    if x.dtype not in _DTYPES:
+        raise GShellHipError(f"linear: float32, bfloat16 or float16 operands are wanted, got {x.dtype}")
+    operands = [(n, t) for n, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)) if t is not None]
+    for name, t in operands:
+        if t.dtype != x.dtype:
+            raise GShellHipError(f"linear: {name} is {t.dtype}, x is {x.dtype}")
+    for name, t in operands:
+        if not t.is_cuda:
+            raise GShellHipError(f"linear: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
+        if t.device != x.device:
+            raise GShellHipError(f"linear: {name} is on {t.device}, x on {x.device}")
+    raise GShellHipError("linear: these operands are not supported")
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
@@ -113,40 +149,30 @@ def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
     output's shape (an expanded view may stand for it).  All operands have one type (float32, bfloat16, float16) and one device; x, weight and residual may be views whose rows are
     any stride apart.  fp32 operands keep fp32's accuracy.  Where the gradient is taken of an activation, act'(z) is kept for the backward pass: 2 bytes an output
     for bf16, 4 for the others."""
-    if activation not in ACTIVATIONS:
-        raise GShellHipError(f"linear: activation {activation!r} is not one of {sorted(k for k in ACTIVATIONS if k)} or None")
-    act = ACTIVATIONS[activation]
+    act = ACTIVATIONS.get(activation)
     beta = float(beta)
-    if act == 2 and not 0.0 < beta < 1e30:
-        raise GShellHipError(f"linear: softplus needs a positive finite beta, got {beta}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise GShellHipError(f"linear: x [..., K] and weight [N, K] are wanted, got {tuple(x.shape)} and {tuple(weight.shape)}")
-    N, K = weight.shape
-    shape = x.shape[:-1] + (N,)
-    if bias is not None and bias.shape != (N,):
-        raise GShellHipError(f"linear: bias must be [{N}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != shape:
-        raise GShellHipError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)}")
-    if x.dtype not in _DTYPES:
-        raise GShellHipError(f"linear: float32, bfloat16 or float16 operands are wanted, got {x.dtype}")
-    operands = (("x", x), ("weight", weight), ("bias", bias), ("residual", residual))
-    for name, t in operands:
-        if t is not None and t.dtype != x.dtype:
-            raise GShellHipError(f"linear: {name} is {t.dtype}, x is {x.dtype}")
-    for name, t in operands:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise GShellHipError(f"linear: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
-        if t.device != x.device:
-            raise GShellHipError(f"linear: {name} is on {t.device}, x on {x.device}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, K) if K else x.reshape(x.shape[:-1].numel(), 0)
-    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(x2.shape[0], N)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for _, t in operands):
-        y = _LinearFn.apply(x2, weight, bias, r2, act, beta)
+    dtype, device, xs, ws = x.dtype, x.get_device(), x.shape, weight.shape
+    ok = act is not None and (act != 2 or 0.0 < beta < 1e30) and len(ws) == 2 and len(xs) >= 1 and xs[-1] == ws[1] and dtype in _DTYPES and x.is_cuda \
+        and weight.dtype is dtype and weight.get_device() == device
+    grad = ok and (x.requires_grad or weight.requires_grad)
+    if ok and bias is not None:
+        ok = bias.dim() == 1 and bias.shape[0] == ws[0] and bias.dtype is dtype and bias.get_device() == device
+        grad = grad or bias.requires_grad
+    flat = len(xs) == 2
+    if ok and residual is not None:
+        ok = residual.shape == xs[:-1] + ws[:1] and residual.dtype is dtype and residual.get_device() == device
+        grad = grad or residual.requires_grad
+    if not ok:
+        _linear_refuse(x, weight, bias, residual, activation, beta)
+    if not flat:
+        rows = xs[:-1].numel()
+        x = x.reshape(rows, ws[1])
+        residual = None if residual is None else residual.reshape(rows, ws[0])
+    if grad and torch.is_grad_enabled():
+        y = _LinearFn.apply(x, weight, bias, residual, act, beta)
     else:
-        y, _ = _linear_forward(x2, weight, bias, r2, act, beta, False)
-    return y if x.dim() == 2 else y.reshape(shape)
+        y = _linear_forward(x, weight, bias, residual, act, beta, False)[0]
+    return y if flat else y.reshape(xs[:-1] + ws[:1])
 
 
 class Linear(torch.nn.Linear):
@@ -171,35 +197,37 @@ _ID_TYPES = {torch.int64: 1, torch.int32: 0}
 def _lookup(ids, weight, scale):
     w, ldw = _rows(weight)
     V, D = w.shape
-    y = torch.empty((ids.numel(), D), dtype=w.dtype, device=w.device)
-    with _on(w.device) as stream:
-        check(_lib.lib().gs_embedding_fwd(_p(ids), c_int(_ID_TYPES[ids.dtype]), _p(w), c_int64(ldw), c_int64(ids.numel()), c_int64(V), c_int64(D), c_int(_DTYPES[w.dtype]),
-                                          c_float(scale), _p(y), stream), "gs_embedding_fwd")
+    T = ids.numel()
+    y = w.new_empty((T, D))
+    check(_on(w.get_device(), lambda stream: _lib.lib().gs_embedding_fwd(ids.data_ptr(), _ID_TYPES[ids.dtype], w.data_ptr(), ldw, T, V, D, _DTYPES[w.dtype], scale,
+                                                                         y.data_ptr(), stream)), "gs_embedding_fwd")
     return y
+
+
+def _embedding_backward(ctx, g):
+    ids, = ctx.saved_tensors
+    V, D, scale, padding_idx = ctx.rest
+    g, ldg = _rows(g)
+    T = ids.numel()
+    dw = g.new_empty((V, D))
+    L = _lib.lib()
+    need = L.gs_embedding_bwd_workspace_bytes(T, V, D)
+    ws = g.new_empty(need, dtype=torch.uint8)
+    check(_on(g.get_device(), lambda stream: L.gs_embedding_bwd(ids.data_ptr(), _ID_TYPES[ids.dtype], g.data_ptr(), ldg, T, V, D, padding_idx, _DTYPES[g.dtype], scale,
+                                                                dw.data_ptr(), ws.data_ptr(), need, stream)), "gs_embedding_bwd")
+    return None, dw, None, None
 
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
-        ctx.rest = (weight.shape, scale, padding_idx)
+        ctx.rest = (*weight.shape, scale, padding_idx)
         return _lookup(ids, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        ids, = ctx.saved_tensors
-        (V, D), scale, padding_idx = ctx.rest
-        g, ldg = _rows(g)
-        T = ids.numel()
-        dw = torch.empty((V, D), dtype=g.dtype, device=g.device)
-        L = _lib.lib()
-        with _on(g.device) as stream:
-            need = L.gs_embedding_bwd_workspace_bytes(c_int64(T), c_int64(V), c_int64(D))
-            ws = _workspace(need, g.device)
-            check(L.gs_embedding_bwd(_p(ids), c_int(_ID_TYPES[ids.dtype]), _p(g), c_int64(ldg), c_int64(T), c_int64(V), c_int64(D), c_int64(padding_idx), c_int(_DTYPES[g.dtype]),
-                                     c_float(scale), _p(dw), _p(ws), c_int64(need), stream), "gs_embedding_bwd")
-        return None, dw, None, None
+        return _once(_embedding_backward, ctx, g)
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
@@ -211,24 +239,24 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
         raise GShellHipError(f"embedding: a weight [V, D] of float32, bfloat16 or float16 is wanted, got {tuple(weight.shape)} {weight.dtype}")
     if ids.dtype not in _ID_TYPES:
         raise GShellHipError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
-    if max(ids.numel(), *weight.shape) >= (1 << 31) - 1:
+    V, D = weight.shape
+    if max(ids.numel(), V, D) >= (1 << 31) - 1:
         raise GShellHipError("embedding: sizes are 0 .. 2^31 - 2")
     if padding_idx is None:
         padding_idx = -1
-    elif not 0 <= padding_idx < weight.shape[0]:
-        raise GShellHipError(f"embedding: padding_idx {padding_idx} is not a row of the table of {weight.shape[0]}")
-    scale = float(scale)
-    for name, t in (("ids", ids), ("weight", weight)):
-        if not t.is_cuda:
-            raise GShellHipError(f"embedding: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
-    if ids.device != weight.device:
+    elif not 0 <= padding_idx < V:
+        raise GShellHipError(f"embedding: padding_idx {padding_idx} is not a row of the table of {V}")
+    if not (ids.is_cuda and weight.is_cuda and ids.get_device() == weight.get_device()):
+        for name, t in (("ids", ids), ("weight", weight)):
+            if not t.is_cuda:
+                raise GShellHipError(f"embedding: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
         raise GShellHipError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
-    flat = ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        y = _EmbeddingFn.apply(flat, weight, scale, int(padding_idx))
+    flat = ids if ids.is_contiguous() else ids.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        y = _EmbeddingFn.apply(flat, weight, float(scale), int(padding_idx))
     else:
-        y = _lookup(flat, weight, scale)
-    return y if ids.dim() == 1 else y.view(ids.shape + (weight.shape[1],))
+        y = _lookup(flat, weight, float(scale))
+    return y if ids.dim() == 1 else y.view(ids.shape + (D,))
 
 
 class Embedding(torch.nn.Embedding):

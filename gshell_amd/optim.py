@@ -98,6 +98,9 @@ def _norm_code(norm_type, what):
 
 def _check_grads(tensors, what):
     """One device for all, dense, of a known type -- on the host, before anything is launched."""
+    if {t.layout for t in tensors} == {torch.strided} and all([t.dtype in _GRAD_TYPES for t in tensors]) and all([t.is_cuda for t in tensors]) \
+            and len({t.get_device() for t in tensors}) == 1:
+        return
     for t in tensors:
         if t.layout is not torch.strided or t.dtype not in _GRAD_TYPES:
             raise _lib.GShellHipError(f"{what}: dense float32, bfloat16 or float16 tensors are wanted, got {t.dtype} ({t.layout})")
@@ -108,42 +111,49 @@ def _check_grads(tensors, what):
             raise _lib.GShellHipError(f"{what}: tensors are on {tensors[0].device} and on {t.device}")
 
 
-def _spans(tensors):
-    at = np.array([t.data_ptr() for t in tensors], dtype=np.int64)
-    size = np.array([t.numel() * t.element_size() for t in tensors], dtype=np.int64)
-    return at, size
+def _addresses(tensors):
+    return np.array([t.data_ptr() for t in tensors], dtype=np.int64)
 
 
-def _check_apart(written, read, what):
-    """No two written tensors share memory, and none shares it with a tensor that is read, unless it is that tensor's own place."""
-    at, size = _spans(written)
-    order = np.argsort(at[size > 0], kind="stable")
-    a, z = at[size > 0][order], size[size > 0][order]
+def _check_apart(written, read, sizes, what):
+    """No two of the written stretches of memory overlap, and none overlaps one that is read, unless it is that gradient's own place.  Addresses and sizes in bytes."""
+    some = sizes > 0
+    order = np.argsort(written[some], kind="stable")
+    a, z = written[some][order], sizes[some][order]
     if (a[:-1] + z[:-1] > a[1:]).any():
         raise _lib.GShellHipError(f"{what}: two of the tensors that are written share memory")
-    if read is None or len(a) == 0:
-        return
-    r_at, r_size = _spans(read)
-    own = r_at == at
-    r_at, r_size = r_at[(r_size > 0) & ~own], r_size[(r_size > 0) & ~own]
-    if len(r_at):
-        # the last written span that starts before a read one ends must end before it starts
-        k = np.searchsorted(a, r_at + r_size, side="left") - 1
-        if ((k >= 0) & (a[k] + z[k] > r_at)).any():
+    other = some & (read != written)
+    if other.any():
+        # the last written stretch that starts before a read one ends must end before that starts
+        r, rz = read[other], sizes[other]
+        k = np.searchsorted(a, r + rz, side="left") - 1
+        if ((k >= 0) & (a[k] + z[k] > r)).any():
             raise _lib.GShellHipError(f"{what}: an output shares memory with another gradient")
 
 
-def _launch_norm(tensors, out, max_norm, code, norm):
-    n = len(tensors)
-    vp = ctypes.c_void_p * n
+def _launch_norm(like, src, dst, numel, types, max_norm, code):
+    """gs_grad_norm over addresses, element counts and type codes (numpy arrays)."""
+    n = len(src)
     L = _lib.lib()
-    dev = norm.device
-    with torch.cuda.device(dev):
-        need = L.gs_grad_norm_workspace_bytes(c_int(n))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        check(L.gs_grad_norm(c_int(n), vp(*[t.data_ptr() for t in tensors]), vp(*[t.data_ptr() for t in out]) if out is not None else None,
-                             (ctypes.c_int64 * n)(*[t.numel() for t in tensors]), (ctypes.c_int32 * n)(*[_GRAD_TYPES[t.dtype] for t in tensors]), c_int(code),
-                             ctypes.c_float(max_norm), _lib.ptr(norm), _lib.ptr(ws), ctypes.c_int64(need), stream()), "gs_grad_norm")
+    need = L.gs_grad_norm_workspace_bytes(n)
+    dev = like.get_device()
+    norm = like.new_empty((), dtype=torch.float32)
+    ws = like.new_empty(need, dtype=torch.uint8)
+
+    def call():
+        return L.gs_grad_norm(n, src.ctypes.data, None if dst is None else dst.ctypes.data, numel.ctypes.data, types.ctypes.data, code, max_norm, norm.data_ptr(), ws.data_ptr(),
+                              need, torch.cuda.current_stream(dev).cuda_stream)
+    if torch.cuda.current_device() == dev:
+        rc = call()
+    else:
+        with torch.cuda.device(dev):
+            rc = call()
+    check(rc, "gs_grad_norm")
+    return norm
+
+
+def _counts(tensors):
+    return np.array([t.numel() for t in tensors], dtype=np.int64), np.array([_GRAD_TYPES[t.dtype] for t in tensors], dtype=np.int32)
 
 
 @torch.no_grad()
@@ -155,9 +165,8 @@ def grad_norm(tensors, norm_type=2.0):
         return torch.zeros(())
     _check_grads(tensors, "grad_norm")
     tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-    _launch_norm(tensors, None, 0.0, code, norm)
-    return norm
+    numel, types = _counts(tensors)
+    return _launch_norm(tensors[0], _addresses(tensors), None, numel, types, 0.0, code)
 
 
 @torch.no_grad()
@@ -182,17 +191,19 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     _check_grads(grads, "clip_grads")
     if out is not grads:
         _check_grads(out, "clip_grads")
-        if out[0].device != grads[0].device:
+        if out[0].get_device() != grads[0].get_device():
             raise _lib.GShellHipError(f"clip_grads: gradients are on {grads[0].device}, outputs on {out[0].device}")
     src = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    dst = [s if o is g else o if o.is_contiguous() else torch.empty_like(s) for g, o, s in zip(grads, out, src)]
-    _check_apart(dst, None if out is grads else src, "clip_grads")
-    norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    _launch_norm(src, dst, max_norm, code, norm)
+    dst = src if out is grads else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in out]
+    numel, types = _counts(src)
+    at = _addresses(src)
+    to = at if dst is src else _addresses(dst)
+    _check_apart(to, at, numel * np.where(types == 0, 4, 2), "clip_grads")
+    norm = _launch_norm(src[0], at, to, numel, types, max_norm, code)
     for o, d in zip(out, dst):
         if d is not o:
             o.copy_(d)
-    torch.autograd.graph.increment_version([o for o, d in zip(out, dst) if d is o])
+    torch.autograd.graph.increment_version(out)
     return norm
 
 
