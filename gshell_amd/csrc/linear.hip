@@ -23,6 +23,7 @@ typedef __attribute__((ext_vector_type(8))) bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) f16 f16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SOFTPLUS = 2, ACT_SILU = 3, ACT_GELU = 4 };
@@ -39,10 +40,18 @@ template <> __device__ __forceinline__ f32x4 mfma<f16>(s16x8 a, s16x8 b, f32x4 c
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Value and derivative of the activation.  For 16-bit layers (FAST) the hardware's exp2, log2 and reciprocal (1 ulp each) and erfc by Abramowitz and Stegun
-// 7.1.26 (absolute error 1.5e-7): far below the rounding of the result.  For fp32 the library's functions.
-template <bool FAST> __device__ __forceinline__ float exp_(float x) { return FAST ? __builtin_amdgcn_exp2f(x * 1.44269504f) : expf(x); }
-template <bool FAST> __device__ __forceinline__ float rcp_(float x) { return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x; }
+// Value and derivative of the activation, on the hardware's exp2, log2 and reciprocal (1 ulp each).  For 16-bit layers (FAST) the exponent's product is rounded, and
+// erfc is Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7): far below the rounding of the result.  For fp32 the product's rounding error goes into the
+// exponential as a factor, and erfc is the library's.
+template <bool FAST> __device__ __forceinline__ float exp_(float x) {
+    const float p = x * 1.44269504f;
+    const float e = __builtin_amdgcn_exp2f(p);
+    if (FAST) return e;
+    // x log2(e) = p + r: r is what the product and the constant were rounded by; an infinite x has p right and r nonsense
+    const float r = __builtin_fmaf(x, 1.44269504f, -p) + x * 1.92596299e-8f;
+    return fabsf(p) < 1000.f ? __builtin_fmaf(e, r * 0.69314718f, e) : e;
+}
+__device__ __forceinline__ float rcp_(float x) { return __builtin_amdgcn_rcpf(x); }
 
 template <bool FAST> __device__ __forceinline__ void act_relu(float z, float& y, float& d) {
     y = z < 0.f ? 0.f : z;
@@ -50,19 +59,14 @@ template <bool FAST> __device__ __forceinline__ void act_relu(float z, float& y,
 }
 template <bool FAST> __device__ __forceinline__ void act_softplus(float beta, float inv_beta, float z, float& y, float& d) {
     const float t = exp_<FAST>(-fabsf(beta * z));          // in [0, 1]: neither end of z overflows
-    float l;
-    if (FAST) {
-        // log(1 + t) from log of the rounded 1 + t, put right by the ratio of t to what was added in fact
-        const float u = 1.f + t, added = u - 1.f;
-        l = added == 0.f ? t : __builtin_amdgcn_logf(u) * 0.69314718f * t * __builtin_amdgcn_rcpf(added);
-    } else {
-        l = log1pf(t);
-    }
+    // log(1 + t) from the logarithm of the rounded 1 + t, put right by the ratio of t to what was added in fact
+    const float u = 1.f + t, added = u - 1.f;
+    const float l = added == 0.f ? t : __builtin_amdgcn_logf(u) * 0.69314718f * t * rcp_(added);
     y = (z < 0.f ? 0.f : z) + l * inv_beta;
-    d = (z >= 0.f ? 1.f : t) * rcp_<FAST>(1.f + t);
+    d = (z >= 0.f ? 1.f : t) * rcp_(1.f + t);
 }
 template <bool FAST> __device__ __forceinline__ void act_silu(float z, float& y, float& d) {
-    const float s = rcp_<FAST>(1.f + exp_<FAST>(-z));
+    const float s = rcp_(1.f + exp_<FAST>(-z));
     y = z * s;
     d = s * (1.f + z * (1.f - s));
 }
@@ -164,54 +168,14 @@ template <typename T> struct Operand {
     int64_t ld;
 };
 
-// 16 values of the contraction c0 .. c0+15 of line `i` (zero outside of the operand)
-template <typename T, bool COLS> __device__ __forceinline__ void fetch16(const Operand<T>& A, int64_t i, int64_t lines, int64_t c0, int64_t c_end, T (&v)[16]) {
-    const bool ok = i < lines;
-    if (!COLS) {
-        const T* q = A.p + i * A.ld + c0;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = ok && c0 + k < c_end ? q[k] : (T)0.f;
-    } else {
-        const T* q = A.p + c0 * A.ld + i;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = ok && c0 + k < c_end ? q[(int64_t)k * A.ld] : (T)0.f;
-    }
-}
-
-__device__ __forceinline__ short raw(bf16 v) { return __builtin_bit_cast(short, v); }
-__device__ __forceinline__ short raw(f16 v) { return __builtin_bit_cast(short, v); }
-
-constexpr int TILE = 128, BK = 32, LDS_ROW = 40;          // 40 shorts a line: 16-byte aligned, and 16 lines read side by side fall on distinct banks
-
-template <typename T> __device__ __forceinline__ void stage16(const T (&v)[16], short* lds) {
-    s16x8 a, b;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = raw(v[k]), b[k] = raw(v[k + 8]);
-    *(s16x8*)lds = a;
-    *(s16x8*)(lds + 8) = b;
-}
-template <> __device__ __forceinline__ void stage16<float>(const float (&v)[16], short* lds) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        s16x8 p[3];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float x = v[8 * h + k];
-            const bf16 x1 = (bf16)x;
-            const float r1 = x - (float)x1;
-            const bf16 x2 = (bf16)r1;
-            p[0][k] = raw(x1), p[1][k] = raw(x2), p[2][k] = raw((bf16)(r1 - (float)x2));
-        }
-#pragma unroll
-        for (int q = 0; q < 3; ++q) *(s16x8*)(lds + q * TILE * LDS_ROW + 8 * h) = p[q];
-    }
-}
-
-// A non-finite sum of the split operands, done again in fp32
-template <bool ACOLS, bool BCOLS> __device__ __noinline__ float plain_dot(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t i, int64_t j, int64_t c0, int64_t c1) {
-    float s = 0.f;
-    for (int64_t c = c0; c < c1; ++c) s = fmaf(ACOLS ? a[c * lda + i] : a[i * lda + c], BCOLS ? b[c * ldb + j] : b[j * ldb + c], s);
-    return s;
+// Workgroups are dealt to the 8 XCDs in turn: give each XCD one stretch of the tiles, and walk a stretch in bands of BAND tile rows, so that the operands' lines that
+// its workgroups share stay in its own L2.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t& ti, uint32_t& tj) {
+    constexpr uint32_t XCDS = 8, BAND = 8;
+    const uint32_t total = tiles_m * tiles_n, per = total / XCDS, extra = total % XCDS, x = id % XCDS, k = id / XCDS;
+    const uint32_t t = x * per + (x < extra ? x : extra) + k;
+    const uint32_t band = t / (BAND * tiles_n), first = band * BAND, rows = tiles_m - first < BAND ? tiles_m - first : BAND, in = t - first * tiles_n;
+    ti = first + in % rows, tj = in / rows;
 }
 
 // A wave's TM x 4 tiles of sums, through 16 KB of LDS of its own, 64 lines at a time: the lanes then hold 16 bytes of neighbouring outputs each, and 8 (16-bit) or 16 (fp32)
@@ -256,65 +220,194 @@ __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&a
     }
 }
 
-template <typename T, bool ACOLS, bool BCOLS>
-__global__ void __launch_bounds__(256) k_product(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<T> E) {
-    constexpr int P = sizeof(T) == 4 ? 3 : 1;
+// ---- fp32 products ------------------------------------------------------------------------------------------------------------------------------------
+// Tiles of 128 x 128, 32 of the contraction a step, two workgroups a compute unit.  While a step is multiplied the next one comes
+// to registers and is split there; each of the three parts has a plane of its own in LDS: [line][32], 4 pieces of 16 bytes a line, piece p of line l at p ^ (l >> 1 & 3), so that the 16
+// lines of a fragment fall on distinct banks.  96 matrix instructions a wave and step stand against 24 fragments read and 32 values split a lane.
+//   rows operand     a lane loads 8 neighbours of the contraction; columns operand: 16 of one line, neighbouring lanes neighbouring lines
+// A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
+constexpr int TILE = 128, BK = 32;
+constexpr int PLANE = TILE * BK;
+
+__device__ __forceinline__ short raw(bf16 v) { return __builtin_bit_cast(short, v); }
+__device__ __forceinline__ short raw(f16 v) { return __builtin_bit_cast(short, v); }
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) bf16 bf16x2;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
+// the parts of two values, each pair in one register
+__device__ __forceinline__ void split2(float x, float y, uint32_t (&part)[3]) {
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        part[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+        if (q == 2) break;
+        x -= __builtin_bit_cast(float, part[q] << 16);
+        y -= __builtin_bit_cast(float, part[q] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ int piece_at(int line, int at) { return line * BK + (((at >> 3) ^ ((line >> 1) & 3)) * 8) + (at & 7); }
+
+template <bool COLS, bool GATE> struct Feed32 {
+    const float *p, *gate;
+    int64_t ld, ldgate, line0, lines, c_end;
+    bool whole;                    // every line of the tile is in the operand
+    // what is in flight: rows operands 2 pieces of 8 neighbours, of lines 64 apart; columns operands 16 neighbours of one line
+    struct Values { float v[16], d[GATE ? 16 : 1]; };
+    __device__ __forceinline__ void fetch(int64_t c, Values& V) const {
+        const bool all = whole && c + BK <= c_end;
+        if constexpr (!COLS) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int64_t l = line0 + j * 64 + (threadIdx.x >> 2), at = c + (threadIdx.x & 3) * 8;
+                const int64_t left = all ? 8 : l < lines ? c_end - at : 0;
+#pragma unroll
+                for (int h = 0; h < 8; h += 4) {
+                    load_some<float, 4>(p + l * ld + at + h, left - h, *(float(*)[4])(V.v + 8 * j + h));
+                    if constexpr (GATE) load_some<float, 4>(gate + l * ldgate + at + h, left - h, *(float(*)[4])(V.d + 8 * j + h));
+                }
+            }
+        } else {
+            const int64_t at = c + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7)) * 16;          // the same for a wave
+            const uint32_t l = threadIdx.x & 127;
+            const float* q = p + at * ld + line0;
+            const float* e = GATE ? gate + at * ldgate + line0 : nullptr;
+            if (all) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    V.v[k] = q[l];
+                    q += ld;
+                    if constexpr (GATE) V.d[k] = e[l], e += ldgate;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const bool ok = line0 + l < lines && at + k < c_end;
+                    V.v[k] = ok ? q[l] : 0.f;
+                    q += ld;
+                    if constexpr (GATE) V.d[k] = ok ? e[l] : 0.f, e += ldgate;
+                }
+            }
+        }
+    }
+    struct Parts { uint32_t p[3][8]; };          // two neighbours a register
+    // split; returns the sum of the values (of one line, for columns operands)
+    __device__ __forceinline__ float split(Values& V, Parts& S) const {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float x = V.v[2 * k], y = V.v[2 * k + 1];
+            if constexpr (GATE) x *= V.d[2 * k], y *= V.d[2 * k + 1];
+            if constexpr (COLS) t += x + y;
+            uint32_t part[3];
+            split2(x, y, part);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) S.p[q][k] = part[q];
+        }
+        return t;
+    }
+    __device__ __forceinline__ void store(short* lds, const Parts& S) const {
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int line = COLS ? threadIdx.x & 127 : h * 64 + (threadIdx.x >> 2), at = COLS ? (threadIdx.x >> 7) * 16 + 8 * h : (threadIdx.x & 3) * 8;
+                *(u32x4*)(lds + q * PLANE + piece_at(line, at)) = u32x4{S.p[q][4 * h], S.p[q][4 * h + 1], S.p[q][4 * h + 2], S.p[q][4 * h + 3]};
+            }
+        }
+    }
+};
+
+template <bool ACOLS, bool BCOLS, bool GATE>
+__global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<float> E,
+                                                      float* column_sums) {
     __shared__ __attribute__((aligned(16))) union {
-        struct { short a[P * TILE * LDS_ROW], b[P * TILE * LDS_ROW]; } in;
+        struct { short a[3 * PLANE], b[3 * PLANE]; } in;
         float out[4 * 64 * 64];
     } lds;
-    short *lds_a = lds.in.a, *lds_b = lds.in.b;
-    const int64_t tiles_n = (N + TILE - 1) / TILE;
-    const int64_t i0 = (int64_t)(blockIdx.x / tiles_n) * TILE, j0 = (int64_t)(blockIdx.x % tiles_n) * TILE;
+    uint32_t ti, tj;
+    tile_of(blockIdx.x, (uint32_t)((M + TILE - 1) / TILE), (uint32_t)((N + TILE - 1) / TILE), ti, tj);
+    const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
     const int64_t c_begin = (int64_t)blockIdx.y * slice, c_end = c_begin + slice < K ? c_begin + slice : K;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-    // rows: two threads share a line; columns: neighbouring threads take neighbouring lines, so that a load of theirs is one stretch of memory
-    const int la = ACOLS ? t & 127 : t >> 1, ca = (ACOLS ? t >> 7 : t & 1) * 16;
-    const int lb = BCOLS ? t & 127 : t >> 1, cb = (BCOLS ? t >> 7 : t & 1) * 16;
-    T va[16], vb[16];
+    Feed32<ACOLS, GATE> fa;
+    Feed32<BCOLS, false> fb;
+    fa.p = A.p, fa.ld = A.ld, fa.gate = gate, fa.ldgate = ldgate, fa.line0 = i0, fa.lines = M, fa.c_end = c_end, fa.whole = i0 + TILE <= M;
+    fb.p = B.p, fb.ld = B.ld, fb.line0 = j0, fb.lines = N, fb.c_end = c_end, fb.whole = j0 + TILE <= N;
+    const bool sums = ACOLS && column_sums && tj == 0;
+    float total = 0.f;
     f32x4 acc[4][4] = {};
-    fetch16<T, ACOLS>(A, i0 + la, M, c_begin + ca, c_end, va);
-    fetch16<T, BCOLS>(B, j0 + lb, N, c_begin + cb, c_end, vb);
+    typename Feed32<ACOLS, GATE>::Values ra;
+    typename Feed32<BCOLS, false>::Values rb;
+    typename Feed32<ACOLS, GATE>::Parts sa;
+    typename Feed32<BCOLS, false>::Parts sb;
+    if (c_begin < c_end) {
+        fa.fetch(c_begin, ra);
+        fb.fetch(c_begin, rb);
+        total += fa.split(ra, sa);
+        fb.split(rb, sb);
+    }
     for (int64_t c = c_begin; c < c_end; c += BK) {
         __syncthreads();
-        stage16<T>(va, lds_a + la * LDS_ROW + ca);
-        stage16<T>(vb, lds_b + lb * LDS_ROW + cb);
+        fa.store(lds.in.a, sa);
+        fb.store(lds.in.b, sb);
         __syncthreads();
-        if (c + BK < c_end) {
-            fetch16<T, ACOLS>(A, i0 + la, M, c + BK + ca, c_end, va);
-            fetch16<T, BCOLS>(B, j0 + lb, N, c + BK + cb, c_end, vb);
+        // behind the end every value is outside and comes as zero
+        fa.fetch(c + BK, ra);
+        fb.fetch(c + BK, rb);
+        s16x8 vb[3][4];
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vb[q][w] = *(const s16x8*)(lds.in.b + q * PLANE + piece_at(wj + w * 16 + (lane & 15), (lane >> 4) * 8));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            s16x8 va[3];
+#pragma unroll
+            for (int q = 0; q < 3; ++q) va[q] = *(const s16x8*)(lds.in.a + q * PLANE + piece_at(wi + u * 16 + (lane & 15), (lane >> 4) * 8));
+            // B goes in as the instruction's first operand: a lane then holds four neighbouring j of one line i.  Small terms first.
+#pragma unroll
+            for (int term = 0; term < 6; ++term) {
+                constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) acc[u][w] = mfma<bf16>(vb[PB[term]][w], va[PA[term]], acc[u][w]);
+            }
         }
-        s16x8 fa[P][4], fb[P][4];
+        // the next step is split in the shadow of the second half of the products
+        total += fa.split(ra, sa);
+        fb.split(rb, sb);
 #pragma unroll
-        for (int q = 0; q < P; ++q)
+        for (int k = 0; k < 48; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                fa[q][u] = *(const s16x8*)(lds_a + q * TILE * LDS_ROW + (wi + u * 16 + (lane & 15)) * LDS_ROW + (lane >> 4) * 8);
-                fb[q][u] = *(const s16x8*)(lds_b + q * TILE * LDS_ROW + (wj + u * 16 + (lane & 15)) * LDS_ROW + (lane >> 4) * 8);
-            }
-        // B goes in as the instruction's first operand: a lane then holds four neighbouring j of one line i
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                if (P == 3) {
-                    acc[u][w] = mfma<T>(fb[P - 1][w], fa[0][u], acc[u][w]);
-                    acc[u][w] = mfma<T>(fb[0][w], fa[P - 1][u], acc[u][w]);
-                    acc[u][w] = mfma<T>(fb[P / 2][w], fa[P / 2][u], acc[u][w]);
-                    acc[u][w] = mfma<T>(fb[P / 2][w], fa[0][u], acc[u][w]);
-                    acc[u][w] = mfma<T>(fb[0][w], fa[P / 2][u], acc[u][w]);
-                }
-                acc[u][w] = mfma<T>(fb[0][w], fa[0][u], acc[u][w]);
-            }
+        for (int k = 0; k < 48; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        }
     }
     __syncthreads();
-    store_wave<T, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, [&](int64_t i, int64_t j, auto& z) {
-        if constexpr (P == 3) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (!(fabsf(z[k]) < __builtin_inff()) && j + k < N) z[k] = plain_dot<ACOLS, BCOLS>(A.p, A.ld, B.p, B.ld, i, j + k, c_begin, c_end);
-        }
+    if (sums) {          // two lanes hold the halves of a line's sum
+        lds.out[threadIdx.x] = total;
+        __syncthreads();
+        if (threadIdx.x < TILE && i0 + threadIdx.x < M) column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = lds.out[threadIdx.x] + lds.out[threadIdx.x + TILE];
+        __syncthreads();
+    }
+    store_wave<float, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, [&](int64_t i, int64_t j, auto& z) {
+        // a sum that is not finite is done again without the split, in fp32
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k)
+            if (!(fabsf(z[k]) < __builtin_inff()) && j + k < N) {
+                float t = 0.f;
+                for (int64_t c = c_begin; c < c_end; ++c) {
+                    float a = ACOLS ? A.p[c * A.ld + i] : A.p[i * A.ld + c];
+                    if (GATE) a *= ACOLS ? gate[c * ldgate + i] : gate[i * ldgate + c];
+                    t = fmaf(a, BCOLS ? B.p[c * B.ld + j + k] : B.p[(j + k) * B.ld + c], t);
+                }
+                z[k] = t;
+            }
     });
 }
 
@@ -325,7 +418,6 @@ __global__ void __launch_bounds__(256) k_product(Operand<T> A, Operand<T> B, int
 //   columns operand  LDS holds [64][line]; fragments come out transposed by ds_read_b64_tr_b16 (4 contraction rows x 16 lines a 16-lane group); the 32-byte
 //                    piece q of row k sits at q ^ h(k), with h different for the 16 rows that one instruction reads
 // Lines and contraction beyond the operand are loaded as zero (an offset outside of the buffer's range).
-typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int STEP = 64;
 constexpr uint32_t OUTSIDE = 0x80000000u;          // every buffer's range: an offset of this size is outside, a tile's own offsets are below
@@ -386,16 +478,6 @@ template <bool COLS, int LINES> __device__ __forceinline__ s16x8 fragment(const 
         }
         return out;
     }
-}
-
-// Workgroups are dealt to the 8 XCDs in turn: give each XCD one stretch of the tiles, and walk a stretch in bands of BAND tile rows, so that the operands' lines that
-// its workgroups share stay in its own L2.
-__device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint32_t& ti, uint32_t& tj) {
-    constexpr uint32_t XCDS = 8, BAND = 8;
-    const uint32_t total = tiles_m * tiles_n, per = total / XCDS, extra = total % XCDS, x = id % XCDS, k = id / XCDS;
-    const uint32_t t = x * per + (x < extra ? x : extra) + k;
-    const uint32_t band = t / (BAND * tiles_n), first = band * BAND, rows = tiles_m - first < BAND ? tiles_m - first : BAND, in = t - first * tiles_n;
-    ti = first + in % rows, tj = in / rows;
 }
 
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
@@ -483,19 +565,35 @@ template <typename T> __global__ void __launch_bounds__(256) k_pack(const T* p, 
     *(s16x8*)(out + r * ldo + c) = v;
 }
 
-// the slices of a contraction joined in their order, then the epilogue
-template <typename T> __global__ void __launch_bounds__(256) k_join(const float* part, int splits, int64_t M, int64_t N, Epilogue<T> E) {
+// The slices of a contraction joined, then the epilogue.  `groups` lanes of a workgroup share the slices of four outputs in equal stretches, in their order.
+template <typename T> __global__ void __launch_bounds__(256) k_join(const float* part, int splits, int groups, int64_t M, int64_t N, Epilogue<T> E) {
     constexpr int V = 4;
-    const int64_t vectors = (N + V - 1) / V, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= M * vectors) return;
-    const int64_t i = at / vectors, j = at % vectors * V;
-    float z[V] = {}, q[V];
-    for (int s = 0; s < splits; ++s) {
-        load_some<float, V>(part + ((int64_t)s * M + i) * N + j, N - j, q);
+    __shared__ f32x4 sums[256];
+    const int each = 256 / groups, group = threadIdx.x / each, x = threadIdx.x % each;
+    const int64_t vectors = (N + V - 1) / V, at = (int64_t)blockIdx.x * each + x;
+    const int share = (splits + groups - 1) / groups, s0 = group * share, s1 = s0 + share < splits ? s0 + share : splits;
+    const bool ok = at < M * vectors;
+    const int64_t i = ok ? at / vectors : 0, j = ok ? at % vectors * V : 0;
+    float z[V] = {};
+    if (ok)
+        for (int s = s0; s < s1; s += 4) {
+            float q[4][V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] += q[k];
+            for (int k = 0; k < 4; ++k) load_some<float, V>(part + ((int64_t)(s + k) * M + i) * N + j, s + k < s1 ? N - j : 0, q[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) z[e] += q[k][e];
+        }
+    if (groups > 1) {
+        sums[threadIdx.x] = f32x4{z[0], z[1], z[2], z[3]};
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 1; g < groups; ++g)
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] += sums[g * each + x][e];
     }
-    finish<T, V>(E, i, j, N, z);
+    if (ok) finish<T, V>(E, i, j, N, z);
 }
 
 // gz = g act'(z), rounded to the layer's type for the two products that read it (rows that start on 16 bytes, zeros behind their ends), and its column sums (of
@@ -561,10 +659,10 @@ static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // How a product is run: the kernel, the slices of its contraction, what is repacked first, and what of the workspace each takes.
 struct Plan {
-    int tile = TILE;                    // 256, 128: the 16-bit kernels; 0: the kernel for any operands
+    int tile = TILE;                    // 256 or 128
     int64_t splits = 1, slice = 0;
     int64_t pack_a = 0, pack_b = 0;          // row strides of the repacked operands, 0: as they are
-    int64_t at_a = 0, at_b = 0, at_part = 0, bytes = 0;
+    int64_t at_a = 0, at_b = 0, at_part = 0, at_cols = 0, bytes = 0;
 };
 struct Line {          // an operand as the plan sees it
     const void* p;
@@ -574,17 +672,12 @@ struct Line {          // an operand as the plan sees it
 // The 16-bit kernels load 16 bytes at a time into LDS, by 31-bit offsets within a tile.
 static bool direct(const Line& a) { return ((uintptr_t)a.p & 15) == 0 && a.ld % 8 == 0 && (a.cols % 8 == 0 || a.zeros) && a.ld < (1 << 21); }
 
-static Plan plan(int es, Line a, int64_t rows_a, Line b, int64_t rows_b, int64_t M, int64_t N, int64_t K) {
+static Plan plan(int es, Line a, int64_t rows_a, Line b, int64_t rows_b, int64_t M, int64_t N, int64_t K, bool column_sums = false) {
     Plan p;
-    const bool fast = es == 2 && up8(a.cols) < (1 << 21) && up8(b.cols) < (1 << 21) && K > 0;
-    int64_t tiles;
-    if (!fast) {
-        p.tile = 0;
-        tiles = gs::cdiv(M, TILE) * gs::cdiv(N, TILE);
-    } else {
+    int64_t tiles = gs::cdiv(M, TILE) * gs::cdiv(N, TILE);
+    if (es == 2) {
         const int64_t big = gs::cdiv(M, 256) * gs::cdiv(N, 256);
-        p.tile = big >= 192 ? 256 : 128;
-        tiles = p.tile == 256 ? big : gs::cdiv(M, 128) * gs::cdiv(N, 128);
+        if (big >= 192) p.tile = 256, tiles = big;
         if (!direct(a)) p.pack_a = up8(a.cols);
         if (!direct(b)) p.pack_b = up8(b.cols);
     }
@@ -601,6 +694,7 @@ static Plan plan(int es, Line a, int64_t rows_a, Line b, int64_t rows_b, int64_t
     p.at_a = at, at += p.pack_a ? align256(rows_a * p.pack_a * es) : 0;
     p.at_b = at, at += p.pack_b ? align256(rows_b * p.pack_b * es) : 0;
     p.at_part = at, at += p.splits > 1 ? align256(p.splits * M * N * 4) : 0;
+    p.at_cols = at, at += column_sums ? align256(p.splits * M * 4) : 0;
     p.bytes = at;
     return p;
 }
@@ -612,22 +706,27 @@ template <typename T> int pack(const void* p, int64_t ld, int64_t rows, int64_t 
     return 0;
 }
 
-// C [M,N] over a contraction of K.
+// C [M,N] over a contraction of K.  fp32: A times `gate` (row stride ldgate), where there is one, and the sums of A's lines (dW only) to column_join.
 template <typename T, bool ACOLS, bool BCOLS>
-int product(Line a, Line b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+int product(Line a, Line b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, void* workspace, int64_t workspace_bytes, hipStream_t stream, const float* gate = nullptr,
+            int64_t ldgate = 0, T* column_join = nullptr) {
     if (M == 0 || N == 0) return 0;
     const int64_t rows_a = ACOLS ? K : M, rows_b = BCOLS ? K : N;
-    const Plan p = plan(sizeof(T), a, rows_a, b, rows_b, M, N, K);
+    const Plan p = plan(sizeof(T), a, rows_a, b, rows_b, M, N, K, column_join != nullptr);
     GS_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), "gs_linear: workspace too small");
     char* ws = (char*)workspace;
-    const int64_t t = p.tile ? p.tile : TILE, tiles = gs::cdiv(M, t) * gs::cdiv(N, t);
-    GS_REQUIRE(tiles < (1ll << 31) && M * gs::cdiv(N, 4) < (255ll << 31), "gs_linear: too many tiles");
+    const int64_t tiles = gs::cdiv(M, p.tile) * gs::cdiv(N, p.tile);
+    GS_REQUIRE(tiles < (1ll << 31) && M * gs::cdiv(N, 4) < (31ll << 31), "gs_linear: too many tiles");
     Epilogue<T> first = E;
     first.part = p.splits > 1 ? (float*)(ws + p.at_part) : nullptr;
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
-    if (p.tile == 0) {
-        hipLaunchKernelGGL((k_product<T, ACOLS, BCOLS>), grid, dim3(256), 0, stream, (Operand<T>{(const T*)a.p, a.ld}), (Operand<T>{(const T*)b.p, b.ld}), M, N, K, p.slice, first);
-    } else if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 4) {
+        const Operand<float> A{(const float*)a.p, a.ld}, B{(const float*)b.p, b.ld};
+        float* cols = column_join ? (float*)(ws + p.at_cols) : nullptr;
+        if (gate) hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, true>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
+        else hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, false>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
+        if (cols) hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)gs::cdiv(M, 32)), dim3(1024), 0, stream, (const float*)cols, (int)p.splits, M, column_join);
+    } else {
         int64_t lines_a = M, lines_b = N;
         if (p.pack_a) {
             if (const int rc = pack<T>(a.p, a.ld, rows_a, a.cols, ws + p.at_a, p.pack_a, stream)) return rc;
@@ -645,8 +744,10 @@ int product(Line a, Line b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, void
         else
             hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
     }
-    if (p.splits > 1)
-        hipLaunchKernelGGL(k_join<T>, dim3((unsigned)gs::cdiv(M * gs::cdiv(N, 4), 256)), dim3(256), 0, stream, (const float*)(ws + p.at_part), (int)p.splits, M, N, E);
+    if (p.splits > 1) {
+        const int groups = p.splits >= 32 ? 16 : p.splits >= 8 ? 4 : 1;
+        hipLaunchKernelGGL(k_join<T>, dim3((unsigned)gs::cdiv(M * gs::cdiv(N, 4), 256 / groups)), dim3(256), 0, stream, (const float*)(ws + p.at_part), (int)p.splits, groups, M, N, E);
+    }
     GS_LAUNCH_CHECK();
     return 0;
 }
@@ -659,15 +760,17 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
 }
 
 struct BackwardPlan {
-    bool gz_made, pass;                // gz has a place of its own (an activation, or rows that the products cannot read as they are); a pass over g is made
+    bool gz_made, pass, sums_with_w;          // gz has a place of its own; a pass over g is made; db comes with dW
     int64_t ldgz, slab, slabs;
     int64_t gz, cols, prod, total;          // byte offsets of gz, the column sums' slabs and the products' workspace
 };
 static BackwardPlan backward_plan(const void* g, int64_t ldg, bool has_dact, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int es,
                                   bool want_x, bool want_w, bool want_b) {
     BackwardPlan p;
-    p.gz_made = has_dact || (es == 2 && (want_x || want_w) && !direct({g, ldg, N, false}));
-    p.pass = p.gz_made || want_b;
+    // fp32 products take the gate as they load g, and the sums with dW; 16-bit ones read gz from memory
+    p.gz_made = es == 2 && (want_x || want_w) && (has_dact || !direct({g, ldg, N, false}));
+    p.sums_with_w = es == 4 && want_w && want_b && K > 0;
+    p.pass = p.gz_made || (want_b && !p.sums_with_w);
     p.ldgz = p.gz_made ? up8(N) : ldg;
     const int64_t across = gs::cdiv(N, GZ_LANES * 16 / es);
     p.slab = gs::cdiv(gs::cdiv(M * across, 2048), GZ_LINES) * GZ_LINES;
@@ -676,12 +779,12 @@ static BackwardPlan backward_plan(const void* g, int64_t ldg, bool has_dact, con
     p.slabs = gs::cdiv(M, p.slab);
     p.gz = 0;
     p.cols = p.gz + (p.gz_made ? align256(M * p.ldgz * es) : 0);
-    p.prod = p.cols + (want_b ? align256(p.slabs * N * 4) : 0);
+    p.prod = p.cols + (want_b && !p.sums_with_w ? align256(p.slabs * N * 4) : 0);
     const Line gl{p.gz_made ? nullptr : g, p.ldgz, N, p.gz_made};
     int64_t b = 0;
     if (want_x) b = plan(es, gl, M, {w, ldw, K, false}, N, M, K, N).bytes;
     if (want_w) {
-        const int64_t c = plan(es, gl, M, {x, ldx, K, false}, M, N, K, M).bytes;
+        const int64_t c = plan(es, gl, M, {x, ldx, K, false}, M, N, K, M, p.sums_with_w).bytes;
         if (c > b) b = c;
     }
     p.total = p.prod + b;
@@ -696,43 +799,45 @@ int linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int6
     char* base = (char*)ws;
     Line gz{p.gz_made ? base + p.gz : g, p.ldgz, N, p.gz_made};
     if (N > 0 && p.pass) {
-        float* part = db ? (float*)(base + p.cols) : nullptr;
+        float* part = db && !p.sums_with_w ? (float*)(base + p.cols) : nullptr;
         const int64_t across = gs::cdiv(N, GZ_LANES * width<T>());
         if (M > 0)
             hipLaunchKernelGGL(k_gz<T>, dim3((unsigned)across, (unsigned)p.slabs), dim3(256), 0, stream, (const T*)g, ldg, (const typename dact_type<T>::type*)dact, M, N, p.slab,
                                p.gz_made ? (T*)(base + p.gz) : nullptr, p.ldgz, part);
-        if (db) hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)gs::cdiv(N, 32)), dim3(1024), 0, stream, (const float*)part, (int)p.slabs, N, (T*)db);
+        if (db && !p.sums_with_w) hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)gs::cdiv(N, 32)), dim3(1024), 0, stream, (const float*)part, (int)p.slabs, N, (T*)db);
         GS_LAUNCH_CHECK();
     }
     Epilogue<T> E{};
+    const float* gate = sizeof(T) == 4 ? (const float*)dact : nullptr;
     int rc = 0;
     if (dx) {
         E.out = (T*)dx, E.ldo = K;
-        rc = product<T, false, true>(gz, {w, ldw, K, false}, M, K, N, E, base + p.prod, ws_bytes - p.prod, stream);
+        rc = product<T, false, true>(gz, {w, ldw, K, false}, M, K, N, E, base + p.prod, ws_bytes - p.prod, stream, gate, N);
     }
     if (!rc && dw) {
         E.out = (T*)dw, E.ldo = K;
-        rc = product<T, true, true>(gz, {x, ldx, K, false}, N, K, M, E, base + p.prod, ws_bytes - p.prod, stream);
+        rc = product<T, true, true>(gz, {x, ldx, K, false}, N, K, M, E, base + p.prod, ws_bytes - p.prod, stream, gate, N, p.sums_with_w ? (T*)db : nullptr);
     }
     return rc;
 }
 
-static bool sizes_ok(int64_t M, int64_t N, int64_t K) {
-    const int64_t top = 1ll << 31;
-    return M >= 0 && N >= 0 && K >= 0 && M < top && N < top && K < top;
+// 16-bit tiles are addressed by 31-bit offsets: 256 rows of 2^21 elements fit
+static bool sizes_ok(int64_t M, int64_t N, int64_t K, int dtype) {
+    const int64_t top = 1ll << 31, wide = dtype == DT_F32 ? top : 1ll << 21;
+    return M >= 0 && N >= 0 && K >= 0 && M < top && N < wide && K < wide;
 }
 
 }  // namespace
 
 extern "C" int64_t gs_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K, int dtype) {
-    if (!sizes_ok(M, N, K) || dtype < 0 || dtype > 2) return -1;
+    if (dtype < 0 || dtype > 2 || !sizes_ok(M, N, K, dtype)) return -1;
     return M == 0 || N == 0 ? 0 : plan(dtype == DT_F32 ? 4 : 2, {x, ldx, K, false}, M, {weight, ldw, K, false}, N, M, N, K).bytes;
 }
 
 extern "C" int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr, int64_t M, int64_t N,
                              int64_t K, int dtype, int act, float beta, void* y, int64_t ldy, void* dact, void* workspace, int64_t workspace_bytes, gs_stream_t stream) {
-    GS_REQUIRE(sizes_ok(M, N, K), "gs_linear_fwd: sizes are 0 .. 2^31 - 1");
     GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_linear_fwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    GS_REQUIRE(sizes_ok(M, N, K, dtype), "gs_linear_fwd: sizes are 0 .. 2^31 - 1, of 16-bit rows 0 .. 2^21 - 1");
     GS_REQUIRE(act >= 0 && act <= 4, "gs_linear_fwd: unknown activation");
     GS_REQUIRE(act != ACT_SOFTPLUS || (beta > 0.f && beta < 1e30f), "gs_linear_fwd: softplus needs a positive finite beta");
     if (M == 0 || N == 0) return 0;
@@ -744,14 +849,14 @@ extern "C" int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int
 
 extern "C" int64_t gs_linear_bwd_workspace_bytes(const void* g, int64_t ldg, int has_dact, const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N,
                                                  int64_t K, int dtype, int want_x, int want_w, int want_b) {
-    if (!sizes_ok(M, N, K) || dtype < 0 || dtype > 2) return -1;
+    if (dtype < 0 || dtype > 2 || !sizes_ok(M, N, K, dtype)) return -1;
     return backward_plan(g, ldg, has_dact, x, ldx, weight, ldw, M, N, K, dtype == DT_F32 ? 4 : 2, want_x, want_w, want_b).total;
 }
 
 extern "C" int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K,
                              int dtype, void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, gs_stream_t stream) {
-    GS_REQUIRE(sizes_ok(M, N, K), "gs_linear_bwd: sizes are 0 .. 2^31 - 1");
     GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_linear_bwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
+    GS_REQUIRE(sizes_ok(M, N, K, dtype), "gs_linear_bwd: sizes are 0 .. 2^31 - 1, of 16-bit rows 0 .. 2^21 - 1");
     GS_REQUIRE(M == 0 || N == 0 || (g && ldg >= 0), "gs_linear_bwd: null gradient");
     GS_REQUIRE(M == 0 || N == 0 || K == 0 || ((!dx || weight) && (!dw || x)), "gs_linear_bwd: null operand");
     const auto run = dtype == DT_F32 ? linear_bwd<float> : dtype == DT_BF16 ? linear_bwd<bf16> : linear_bwd<f16>;

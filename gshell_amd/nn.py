@@ -57,7 +57,7 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
     xp, wp = x.data_ptr(), w.data_ptr()
     need = L.gs_linear_fwd_workspace_bytes(xp, ldx, wp, ldw, M, N, K, code)
     if need < 0:
-        raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
+        raise GShellHipError("linear: sizes are 0 .. 2^31 - 1, of 16-bit rows (in and out) 0 .. 2^21 - 1")
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
     check(_on(x.get_device(), lambda stream: L.gs_linear_fwd(xp, ldx, wp, ldw, _at(b), _at(r), ldr, M, N, K, code, act, beta, y.data_ptr(), N,
                                                              _at(dact), _at(ws), need, stream)), "gs_linear_fwd")
@@ -86,7 +86,7 @@ def _linear_backward(ctx, g):
         gp, dp, code = gr.data_ptr(), _at(dact), _DTYPES[gr.dtype]
         need = L.gs_linear_bwd_workspace_bytes(gp, ldg, dact is not None, xp, ldx, wp, ldw, M, N, K, code, want_x, want_w, want_b)
         if need < 0:
-            raise GShellHipError("linear: sizes are 0 .. 2^31 - 1")
+            raise GShellHipError("linear: sizes are 0 .. 2^31 - 1, of 16-bit rows (in and out) 0 .. 2^21 - 1")
         ws = gr.new_empty(need, dtype=torch.uint8) if need else None
         check(_on(gr.get_device(), lambda stream: L.gs_linear_bwd(gp, ldg, dp, xp, ldx, wp, ldw, M, N, K, code, _at(dx), _at(dw),
                                                                   _at(db), _at(ws), need, stream)), "gs_linear_bwd")

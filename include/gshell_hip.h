@@ -862,7 +862,7 @@ int gs_flexi_cut_bwd(const int64_t* pa, const int64_t* pb, int64_t n, const floa
  *   log(1 + exp(beta z)) / beta, 3 silu, 4 gelu (erf form).  bias, residual may be null.
  *   dact [M,N] (contiguous; fp16 for bf16 layers, fp32 otherwise; null = not wanted) receives act'(z) for gs_linear_bwd.
  *   gs_linear_bwd: gz = g act'(z) -> dx = gz W [M,K], dW = gz^T x [N,K], db = column sums of gz; any of the three may be null.
- *   dact null = no activation.  Sums are taken in a fixed order: the same bits every time.
+ *   dact null = no activation.  M, N, K < 2^31; N, K < 2^21 for 16-bit layers.  Sums are taken in a fixed order: the same bits every time.
  *   The workspaces are the caller's and hold nothing between calls; their sizes go by the addresses and strides too (16-bit operands
  *   whose rows do not start on 16 bytes are repacked first).
  * ---------------------------------------------------------------------------------- */
