@@ -83,28 +83,24 @@ template <bool FAST> __device__ __forceinline__ void act_gelu(float z, float& y,
     y = z * phi;
     d = phi + z * (e * 0.39894228040143268f);
 }
-// V values at once: the choice is the same for the whole launch
-template <bool FAST, int V> __device__ __forceinline__ void act_eval(int act, float beta, float inv_beta, float (&z)[V], float (&d)[V]) {
+// BATCH x V values at once: the choice is the same for the whole launch
+template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, float beta, float inv_beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
     switch (act) {
         case ACT_RELU:
 #pragma unroll
-            for (int k = 0; k < V; ++k) act_relu<FAST>(z[k], z[k], d[k]);
+            for (int k = 0; k < V * BATCH; ++k) act_relu<FAST>(z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
             break;
         case ACT_SOFTPLUS:
 #pragma unroll
-            for (int k = 0; k < V; ++k) act_softplus<FAST>(beta, inv_beta, z[k], z[k], d[k]);
+            for (int k = 0; k < V * BATCH; ++k) act_softplus<FAST>(beta, inv_beta, z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
             break;
         case ACT_SILU:
 #pragma unroll
-            for (int k = 0; k < V; ++k) act_silu<FAST>(z[k], z[k], d[k]);
-            break;
-        case ACT_GELU:
-#pragma unroll
-            for (int k = 0; k < V; ++k) act_gelu<FAST>(z[k], z[k], d[k]);
+            for (int k = 0; k < V * BATCH; ++k) act_silu<FAST>(z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
             break;
         default:
 #pragma unroll
-            for (int k = 0; k < V; ++k) d[k] = 1.f;
+            for (int k = 0; k < V * BATCH; ++k) act_gelu<FAST>(z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
     }
 }
 
@@ -146,21 +142,36 @@ template <typename T, int V> __device__ __forceinline__ void store_some(T* p, in
             if (k < in_row) p[k] = (T)v[k];
     }
 }
-template <typename T, int V> __device__ __forceinline__ void finish(const Epilogue<T>& E, int64_t i, int64_t j, int64_t N, float (&z)[V]) {
+// BATCH x V outputs of the lines i[0 .. BATCH-1] (those below M), columns j ..
+template <typename T, int V, int BATCH> __device__ __forceinline__ void finish(const Epilogue<T>& E, const int64_t (&i)[BATCH], int64_t j, int64_t M, int64_t N, float (&z)[BATCH][V]) {
     const int64_t in_row = N - j;
-    float d[V], r[V];
-    if (E.bias) {
-        load_some<T, V>(E.bias + j, in_row, r);
-#pragma unroll
-        for (int k = 0; k < V; ++k) z[k] += r[k];
-    }
-    if (E.res) load_some<T, V>(E.res + i * E.ldr + j, in_row, r);
-    act_eval<sizeof(T) == 2, V>(E.act, E.beta, E.inv_beta, z, d);
-    if (E.dact) store_some<typename dact_type<T>::type, V>(E.dact + i * N + j, in_row, d);
+    float r[BATCH][V];
     if (E.res)
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] += r[k];
-    store_some<T, V>(E.out + i * E.ldo + j, in_row, z);
+        for (int b = 0; b < BATCH; ++b) load_some<T, V>(E.res + i[b] * E.ldr + j, i[b] < M ? in_row : 0, r[b]);
+    if (E.bias) {
+        float q[V];
+        load_some<T, V>(E.bias + j, in_row, q);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+            for (int k = 0; k < V; ++k) z[b][k] += q[k];
+    }
+    if (E.act != ACT_NONE) {
+        float d[BATCH][V];
+        act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta, E.inv_beta, z, d);
+        if (E.dact)
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (i[b] < M) store_some<typename dact_type<T>::type, V>(E.dact + i[b] * N + j, in_row, d[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+        if (E.res)
+#pragma unroll
+            for (int k = 0; k < V; ++k) z[b][k] += r[b][k];
+        if (i[b] < M) store_some<T, V>(E.out + i[b] * E.ldo + j, in_row, z[b]);
+    }
 }
 
 template <typename T> struct Operand {
@@ -198,21 +209,32 @@ __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&a
                     }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        // BATCH lines a lane side by side: what they read of the residual is in flight together
+        constexpr int BATCH = TM > 4 ? 2 : 4;          // as many as the registers beside the sums hold
 #pragma unroll 1
-        for (int l0 = 0; l0 < 64; l0 += LINES) {
-            const int l = l0 + lane / LANES, c = lane % LANES * V;
-            const int64_t i = i0 + part * 64 + l, j = j0 + c;
-            float z[V];
+        for (int l0 = 0; l0 < 64; l0 += LINES * BATCH) {
+            const int c = lane % LANES * V;
+            const int64_t j = j0 + c;
+            int64_t i[BATCH];
+            float z[BATCH][V];
 #pragma unroll
-            for (int k = 0; k < V; k += 4) {
-                const f32x4 q = *(const f32x4*)(lds + l * 64 + (((c + k) >> 2) ^ (l & 15)) * 4);
+            for (int b = 0; b < BATCH; ++b) {
+                const int l = l0 + b * LINES + lane / LANES;
+                i[b] = i0 + part * 64 + l;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[k + e] = q[e];
+                for (int k = 0; k < V; k += 4) {
+                    const f32x4 q = *(const f32x4*)(lds + l * 64 + (((c + k) >> 2) ^ (l & 15)) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) z[b][k + e] = q[e];
+                }
+                if (i[b] < M && j < N) fix(i[b], j, z[b]);
             }
-            if (i < M && j < N) {
-                fix(i, j, z);
-                if (E.part) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i) * N + j, N - j, z);
-                else finish<T, V>(E, i, j, N, z);
+            if (E.part) {
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b)
+                    if (i[b] < M && j < N) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i[b]) * N + j, N - j, z[b]);
+            } else if (j < N) {
+                finish<T, V, BATCH>(E, i, j, M, N, z);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -480,11 +502,19 @@ template <bool COLS, int LINES> __device__ __forceinline__ s16x8 fragment(const 
     }
 }
 
-template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E) {
+template <int LEFT> __device__ __forceinline__ void wait_and_meet() {
+    // this wave's loads but for the last LEFT have arrived and its reads of LDS are done; then everybody's
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, int BUFFERS>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BUFFERS == 2 ? 2 : 1) k_product16(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E) {
 #if defined(__HIP_DEVICE_COMPILE__)          // the host pass has no type for a buffer's descriptor
     constexpr int THREADS = BM / WM * (BN / WN) * 64, TM = WM / 16, TN = WN / 16, PARTS = TM / 4, CLUSTERS = 2 * PARTS;
-    __shared__ __attribute__((aligned(1024))) short a0[BM * STEP], a1[BM * STEP], b0[BN * STEP], b1[BN * STEP];
+    // each buffer (A's tile, then B's) is a variable of its own: the compiler then knows which loads a read of LDS has to wait for
+    constexpr int BUFFER = (BM + BN) * STEP;
+    __shared__ __attribute__((aligned(1024))) short s0[BUFFER], s1[BUFFER], s2[BUFFERS > 2 ? BUFFER : 8], s3[BUFFERS > 2 ? BUFFER : 8];
+    static_assert(BUFFERS == 2 || BUFFERS == 4, "buffers");
     uint32_t ti, tj;
     tile_of(blockIdx.x, (uint32_t)((M + BM - 1) / BM), (uint32_t)((N + BN - 1) / BN), ti, tj);
     const int64_t i0 = (int64_t)ti * BM, j0 = (int64_t)tj * BN;
@@ -493,20 +523,26 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Opera
     const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
     Feed<ACOLS, BM, THREADS> fa;
     Feed<BCOLS, BN, THREADS> fb;
+    constexpr int LOADS = Feed<ACOLS, BM, THREADS>::LOADS + Feed<BCOLS, BN, THREADS>::LOADS;
     fa.init(A.p, A.ld, i0, lines_a, c_begin);
     fb.init(B.p, B.ld, j0, lines_b, c_begin);
     f32x4 acc[TM][TN] = {};
     s16x8 va[2][4], vb[2][TN];
     const int steps = (int)((len + STEP - 1) / STEP);
     int64_t left = len;
+    const auto load = [&](short* s) __attribute__((always_inline)) {
+        fa.load(s, left);
+        fb.load(s + BM * STEP, left);
+        left -= STEP;
+    };
     // one cluster: 4 x TN products of half `ks`, part `part` of the wave's lines
-    const auto read = [&](const short* a, const short* b, int cluster) __attribute__((always_inline)) {
+    const auto read = [&](const short* s, int cluster) __attribute__((always_inline)) {
         const int ks = cluster / PARTS, part = cluster % PARTS;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) va[cluster & 1][u] = fragment<ACOLS, BM>(a, wi + (part * 4 + u) * 16, ks);
+        for (int u = 0; u < 4; ++u) va[cluster & 1][u] = fragment<ACOLS, BM>(s, wi + (part * 4 + u) * 16, ks);
         if (part == 0)
 #pragma unroll
-            for (int w = 0; w < TN; ++w) vb[ks][w] = fragment<BCOLS, BN>(b, wj + w * 16, ks);
+            for (int w = 0; w < TN; ++w) vb[ks][w] = fragment<BCOLS, BN>(s + BM * STEP, wj + w * 16, ks);
     };
     const auto multiply = [&](int cluster) __attribute__((always_inline)) {
         const int ks = cluster / PARTS, part = cluster % PARTS;
@@ -515,41 +551,50 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Opera
 #pragma unroll
             for (int w = 0; w < TN; ++w) acc[part * 4 + u][w] = mfma<T>(vb[ks][w], va[cluster & 1][u], acc[part * 4 + u][w]);
     };
-    const auto step = [&](int k, short* a, short* b, short* a_next, short* b_next) __attribute__((always_inline)) {
+    int k = 0;
+    const auto step = [&](short* s, short* next) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c + 1 < CLUSTERS; ++c) {
-            read(a, b, c + 1);
+            read(s, c + 1);
             multiply(c);
         }
-        __syncthreads();          // the next step's tiles have arrived, and nobody reads this step's any more
-        if (k + 1 < steps) read(a_next, b_next, 0);
-        if (k + 2 < steps) {
-            fa.load(a, left);
-            fb.load(b, left);
-            left -= STEP;
-        }
+        // the next step's tiles have arrived, and nobody reads this step's any more
+        wait_and_meet<(BUFFERS - 2) * LOADS>();
+        // With four buffers every step loads and reads ahead, behind the end too (nothing but zeros comes from there): without branches the compiler sees which loads a
+        // read waits for.  With two it waits for all of them anyway, and the branches keep the loads in front of the last products.
+        if (BUFFERS > 2 || ++k < steps) read(next, 0);
+        if (BUFFERS > 2 || k + 1 < steps) load(s);
         multiply(CLUSTERS - 1);
     };
-    if (steps > 0) {
-        fa.load(a0, left);
-        fb.load(b0, left);
-        left -= STEP;
-        __syncthreads();
-        if (steps > 1) {
-            fa.load(a1, left);
-            fb.load(b1, left);
-            left -= STEP;
-        }
-        read(a0, b0, 0);
-        for (int k = 0; k < steps; k += 2) {
-            step(k, a0, b0, a1, b1);
-            if (k + 1 < steps) step(k + 1, a1, b1, a0, b0);
-        }
+    load(s0);
+    load(s1);
+    if constexpr (BUFFERS > 2) {
+        load(s2);
+        load(s3);
     }
-    // after the last barrier nobody reads the tiles: each wave takes a quarter, or half a quarter, of them for its sums
-    static_assert(WN == 64 && BM * STEP * 2 * 2 + BN * STEP * 2 * 2 >= THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
-    constexpr int SHARE = THREADS / 64 / 4;
-    short* mine = wave / SHARE == 0 ? a0 : wave / SHARE == 1 ? a1 : wave / SHARE == 2 ? b0 : b1;
+    wait_and_meet<(BUFFERS - 1) * LOADS>();
+    read(s0, 0);
+    if constexpr (BUFFERS == 2) {
+        while (k < steps) {
+            step(s0, s1);
+            if (k < steps) step(s1, s0);
+        }
+    } else {
+        for (; k + 4 <= steps; k += 4) {
+            step(s0, s1);
+            step(s1, s2);
+            step(s2, s3);
+            step(s3, s0);
+        }
+        if (k < steps) step(s0, s1);
+        if (k + 1 < steps) step(s1, s2);
+        if (k + 2 < steps) step(s2, s3);
+    }
+    wait_and_meet<0>();
+    // nobody reads or loads tiles any more: the first two buffers hold the waves' sums
+    static_assert(WN == 64 && BUFFER * 2 * 2 == THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
+    constexpr int SHARE = THREADS / 64 / 2;
+    short* mine = wave < SHARE ? s0 : s1;
     store_wave<T, TM>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
 #endif
 }
@@ -574,7 +619,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
     const int share = (splits + groups - 1) / groups, s0 = group * share, s1 = s0 + share < splits ? s0 + share : splits;
     const bool ok = at < M * vectors;
     const int64_t i = ok ? at / vectors : 0, j = ok ? at % vectors * V : 0;
-    float z[V] = {};
+    float z[1][V] = {};
     if (ok)
         for (int s = s0; s < s1; s += 4) {
             float q[4][V];
@@ -583,17 +628,18 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int e = 0; e < V; ++e) z[e] += q[k][e];
+                for (int e = 0; e < V; ++e) z[0][e] += q[k][e];
         }
     if (groups > 1) {
-        sums[threadIdx.x] = f32x4{z[0], z[1], z[2], z[3]};
+        sums[threadIdx.x] = f32x4{z[0][0], z[0][1], z[0][2], z[0][3]};
         __syncthreads();
         if (group > 0) return;
         for (int g = 1; g < groups; ++g)
 #pragma unroll
-            for (int e = 0; e < V; ++e) z[e] += sums[g * each + x][e];
+            for (int e = 0; e < V; ++e) z[0][e] += sums[g * each + x][e];
     }
-    if (ok) finish<T, V>(E, i, j, N, z);
+    const int64_t line[1] = {i};
+    if (ok) finish<T, V, 1>(E, line, j, M, N, z);
 }
 
 // gz = g act'(z), rounded to the layer's type for the two products that read it (rows that start on 16 bytes, zeros behind their ends), and its column sums (of
@@ -660,6 +706,7 @@ static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 // How a product is run: the kernel, the slices of its contraction, what is repacked first, and what of the workspace each takes.
 struct Plan {
     int tile = TILE;                    // 256 or 128
+    bool deep = false;                  // 128 with four buffers, one workgroup a compute unit, rather than two with two buffers each
     int64_t splits = 1, slice = 0;
     int64_t pack_a = 0, pack_b = 0;          // row strides of the repacked operands, 0: as they are
     int64_t at_a = 0, at_b = 0, at_part = 0, at_cols = 0, bytes = 0;
@@ -681,10 +728,11 @@ static Plan plan(int es, Line a, int64_t rows_a, Line b, int64_t rows_b, int64_t
         if (!direct(a)) p.pack_a = up8(a.cols);
         if (!direct(b)) p.pack_b = up8(b.cols);
     }
-    const int64_t slots = p.tile == 256 ? CUS : 2 * CUS;
-    if (tiles < slots && K >= 512) {
+    if (es == 2 && p.tile == 128) p.deep = tiles <= CUS;
+    const int64_t slots = p.tile == 256 || p.deep ? CUS : 2 * CUS, least = p.deep ? 512 : 256;
+    if (tiles < slots && K >= 2 * least) {
         p.splits = slots / tiles;
-        if (p.splits > K / 256) p.splits = K / 256;
+        if (p.splits > K / least) p.splits = K / least;
         if (p.splits > 256) p.splits = 256;
         if (p.splits < 1) p.splits = 1;
     }
@@ -740,9 +788,11 @@ int product(Line a, Line b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, void
         if (BCOLS && b.zeros) lines_b = up8(N);
         const Operand<T> A{(const T*)a.p, a.ld}, B{(const T*)b.p, b.ld};
         if (p.tile == 256)
-            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 256, 256, 128, 64>), grid, dim3(512), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
+            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 256, 256, 128, 64, 2>), grid, dim3(512), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
+        else if (p.deep)
+            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64, 4>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
         else
-            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
+            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64, 2>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
     }
     if (p.splits > 1) {
         const int groups = p.splits >= 32 ? 16 : p.splits >= 8 ? 4 : 1;
