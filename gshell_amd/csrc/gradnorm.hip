@@ -9,6 +9,10 @@
 // elements from the end: what the first has read last is still in the 256 MB cache.  In place and with a factor of one it writes nothing.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "../../include/gshell_hip.h"
 #include "common.hpp"
 
@@ -185,6 +189,27 @@ int run(int n, const void* const* src, void* const* dst, const int64_t* numel, c
     return 0;
 }
 
+// Whether a stretch of memory that is written overlaps another that is written, or one that is read from somewhere else.
+static bool overlap(int n, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* type) {
+    struct Stretch { uintptr_t at, end; bool written; };
+    std::vector<Stretch> all;
+    all.reserve(2 * (size_t)n);
+    for (int k = 0; k < n; ++k) {
+        if (numel[k] == 0) continue;
+        const uintptr_t bytes = (uintptr_t)numel[k] * (type[k] == 0 ? 4 : 2);
+        all.push_back({(uintptr_t)dst[k], (uintptr_t)dst[k] + bytes, true});
+        if (src[k] != dst[k]) all.push_back({(uintptr_t)src[k], (uintptr_t)src[k] + bytes, false});
+    }
+    std::sort(all.begin(), all.end(), [](const Stretch& a, const Stretch& b) { return a.at < b.at; });
+    uintptr_t end = 0, written = 0;          // ends of what came before: of all, of what is written
+    for (const Stretch& s : all) {
+        if (s.at < (s.written ? end : written)) return true;
+        end = s.end > end ? s.end : end;
+        if (s.written && s.end > written) written = s.end;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" int64_t gs_grad_norm_workspace_bytes(int n_tensors) { return n_tensors < 0 ? -1 : (gs::cdiv(n_tensors, TABLE) + 1) * MAX_BLOCKS * 8; }
@@ -194,8 +219,14 @@ extern "C" int gs_grad_norm(int n_tensors, const void* const* grads, void* const
     GS_REQUIRE(n_tensors >= 0 && norm && (n_tensors == 0 || (grads && numel && dtypes)), "gs_grad_norm: null argument");
     GS_REQUIRE(norm_type == 0 || norm_type == 1 || norm_type == 2, "gs_grad_norm: norm_type is 0 (2-norm), 1 (1-norm) or 2 (largest magnitude)");
     GS_REQUIRE(!out || max_norm >= 0.f, "gs_grad_norm: max_norm must not be negative or NaN");
-    GS_REQUIRE(workspace && workspace_bytes >= gs_grad_norm_workspace_bytes(n_tensors), "gs_grad_norm: workspace too small");
     for (int k = 0; k < n_tensors; ++k) GS_REQUIRE(numel[k] == 0 || (numel[k] > 0 && grads[k] && (!out || out[k]) && dtypes[k] >= 0 && dtypes[k] <= 2), "gs_grad_norm: null tensor or unknown type");
+    try {
+        GS_REQUIRE(!out || !overlap(n_tensors, grads, out, numel, dtypes), "gs_grad_norm: an output shares memory with another output or another gradient");
+    } catch (const std::bad_alloc&) {
+        gs::set_error("gs_grad_norm: out of host memory");
+        return 3;
+    }
+    GS_REQUIRE(workspace && workspace_bytes >= gs_grad_norm_workspace_bytes(n_tensors), "gs_grad_norm: workspace too small");
     const auto go = norm_type == 0 ? run<NORM_2> : norm_type == 1 ? run<NORM_1> : run<NORM_INF>;
     return go(n_tensors, grads, out, numel, dtypes, max_norm, norm, (double*)workspace, (hipStream_t)stream);
 }

@@ -191,7 +191,7 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t 
 
 // A wave's TM x 4 tiles of sums, through 16 KB of LDS of its own, 64 lines at a time: the lanes then hold 16 bytes of neighbouring outputs each, and 8 (16-bit) or 16 (fp32)
 // lanes a whole line of 64.  The 16-byte piece p of line l is kept at p ^ (l & 15).  fix(i, j, z): what a sum is replaced by.
-template <typename T, int TM, typename F>
+template <typename T, int TM, int BATCH, typename F>
 __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&acc)[TM][4], float* lds, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
     constexpr int V = width<T>(), LANES = 64 / V, LINES = 64 / LANES;
     const int lane = threadIdx.x & 63;
@@ -209,8 +209,8 @@ __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&a
                     }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        // BATCH lines a lane side by side: what they read of the residual is in flight together
-        constexpr int BATCH = TM > 4 ? 2 : 4;          // as many as the registers beside the sums hold
+        // BATCH lines a lane side by side, as many as the registers beside the sums hold: what they read of the residual is in flight together
+
 #pragma unroll 1
         for (int l0 = 0; l0 < 64; l0 += LINES * BATCH) {
             const int c = lane % LANES * V;
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const fl
         if (threadIdx.x < TILE && i0 + threadIdx.x < M) column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = lds.out[threadIdx.x] + lds.out[threadIdx.x + TILE];
         __syncthreads();
     }
-    store_wave<float, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, [&](int64_t i, int64_t j, auto& z) {
+    store_wave<float, 4, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, [&](int64_t i, int64_t j, auto& z) {
         // a sum that is not finite is done again without the split, in fp32
 #pragma unroll 1
         for (int k = 0; k < 4; ++k)
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BUFFERS == 2 ? 2 : 1
     static_assert(WN == 64 && BUFFER * 2 * 2 == THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
     constexpr int SHARE = THREADS / 64 / 2;
     short* mine = wave < SHARE ? s0 : s1;
-    store_wave<T, TM>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+    store_wave<T, TM, (BUFFERS > 2 ? 8 : TM > 4 ? 2 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
 #endif
 }
 

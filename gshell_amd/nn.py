@@ -17,17 +17,10 @@ from ._lib import GShellHipError, check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "softplus": 2, "silu": 3, "gelu": 4}
-# The calls below are short next to what Python spends around them: plain numbers and addresses go to the C functions (_lib.PLAIN_CALLS), and the current device is
-# changed only where it is another one.
-
-
-def _on(index, call):
-    """call(stream) with device `index` as the current one."""
-    before = torch.cuda.current_device()
-    if before == index:
-        return call(torch.cuda.current_stream(index).cuda_stream)
-    with torch.cuda.device(index):
-        return call(torch.cuda.current_stream(index).cuda_stream)
+# The calls below are short next to what Python spends around them, and a backward pass runs in a thread of its own, where every Python object comes from another core's
+# cache: plain numbers and addresses go to the C functions (_lib.PLAIN_CALLS), what a backward pass needs is worked out in the forward pass, and the current device is changed
+# only where it is another one.
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
 
 
 def _at(t):
@@ -59,47 +52,63 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
     if need < 0:
         raise GShellHipError("linear: sizes are 0 .. 2^31 - 1, of 16-bit rows (in and out) 0 .. 2^21 - 1")
     ws = x.new_empty(need, dtype=torch.uint8) if need else None
-    check(_on(x.get_device(), lambda stream: L.gs_linear_fwd(xp, ldx, wp, ldw, _at(b), _at(r), ldr, M, N, K, code, act, beta, y.data_ptr(), N,
-                                                             _at(dact), _at(ws), need, stream)), "gs_linear_fwd")
+    device = x.get_device()
+    args = (xp, ldx, wp, ldw, _at(b), _at(r), ldr, M, N, K, code, act, beta, y.data_ptr(), N, _at(dact), _at(ws), need, _stream_of(device))
+    if _current_device() == device:
+        rc = L.gs_linear_fwd(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = L.gs_linear_fwd(*args)
+    if rc:
+        check(rc, "gs_linear_fwd")
     return y, dact
 
 
 def _linear_backward(ctx, g):
     x, weight, dact = ctx.saved_tensors
-    M, N, K = ctx.sizes
-    want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
+    M, K, N, code, want_x, want_w, want_b, want_r = ctx.rest
     dx = dw = db = None
     if want_x or want_w or want_b:
         gr, ldg = _rows(g)
-        xp = ldx = wp = ldw = 0
+        xp = ldx = wp = ldw = xo = wo = bo = 0
         if want_w:
             x, ldx = _rows(x)
             xp = x.data_ptr()
             dw = gr.new_empty((N, K))
+            wo = dw.data_ptr()
         if want_x:
             weight, ldw = _rows(weight)
             wp = weight.data_ptr()
             dx = gr.new_empty((M, K))
+            xo = dx.data_ptr()
         if want_b:
             db = gr.new_empty(N)
+            bo = db.data_ptr()
         L = _lib.lib()
-        gp, dp, code = gr.data_ptr(), _at(dact), _DTYPES[gr.dtype]
+        gp, dp = gr.data_ptr(), _at(dact)
         need = L.gs_linear_bwd_workspace_bytes(gp, ldg, dact is not None, xp, ldx, wp, ldw, M, N, K, code, want_x, want_w, want_b)
         if need < 0:
             raise GShellHipError("linear: sizes are 0 .. 2^31 - 1, of 16-bit rows (in and out) 0 .. 2^21 - 1")
         ws = gr.new_empty(need, dtype=torch.uint8) if need else None
-        check(_on(gr.get_device(), lambda stream: L.gs_linear_bwd(gp, ldg, dp, xp, ldx, wp, ldw, M, N, K, code, _at(dx), _at(dw),
-                                                                  _at(db), _at(ws), need, stream)), "gs_linear_bwd")
+        device = gr.get_device()
+        args = (gp, ldg, dp, xp, ldx, wp, ldw, M, N, K, code, xo, wo, bo, _at(ws), need, _stream_of(device))
+        if _current_device() == device:
+            rc = L.gs_linear_bwd(*args)
+        else:
+            with torch.cuda.device(device):
+                rc = L.gs_linear_bwd(*args)
+        if rc:
+            check(rc, "gs_linear_bwd")
     return dx, dw, db, g if want_r else None, None, None
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, beta):
-        need = ctx.needs_input_grad
-        y, dact = _linear_forward(x, weight, bias, residual, act, beta, need[0] or need[1] or need[2])
-        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, dact)
-        ctx.sizes = (x.shape[0], weight.shape[0], x.shape[1])
+        want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
+        y, dact = _linear_forward(x, weight, bias, residual, act, beta, want_x or want_w or want_b)
+        ctx.save_for_backward(x if want_w else None, weight if want_x else None, dact)
+        ctx.rest = (*x.shape, weight.shape[0], _DTYPES[x.dtype], want_x, want_w, want_b, want_r)
         return y
 
     @staticmethod
@@ -199,22 +208,33 @@ def _lookup(ids, weight, scale):
     V, D = w.shape
     T = ids.numel()
     y = w.new_empty((T, D))
-    check(_on(w.get_device(), lambda stream: _lib.lib().gs_embedding_fwd(ids.data_ptr(), _ID_TYPES[ids.dtype], w.data_ptr(), ldw, T, V, D, _DTYPES[w.dtype], scale,
-                                                                         y.data_ptr(), stream)), "gs_embedding_fwd")
+    device = w.get_device()
+    args = (ids.data_ptr(), _ID_TYPES[ids.dtype], w.data_ptr(), ldw, T, V, D, _DTYPES[w.dtype], scale, y.data_ptr(), _stream_of(device))
+    if _current_device() == device:
+        rc = _lib.lib().gs_embedding_fwd(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = _lib.lib().gs_embedding_fwd(*args)
+    if rc:
+        check(rc, "gs_embedding_fwd")
     return y
 
 
 def _embedding_backward(ctx, g):
     ids, = ctx.saved_tensors
-    V, D, scale, padding_idx = ctx.rest
+    kind, T, V, D, padding_idx, code, scale, need = ctx.rest
     g, ldg = _rows(g)
-    T = ids.numel()
     dw = g.new_empty((V, D))
-    L = _lib.lib()
-    need = L.gs_embedding_bwd_workspace_bytes(T, V, D)
     ws = g.new_empty(need, dtype=torch.uint8)
-    check(_on(g.get_device(), lambda stream: L.gs_embedding_bwd(ids.data_ptr(), _ID_TYPES[ids.dtype], g.data_ptr(), ldg, T, V, D, padding_idx, _DTYPES[g.dtype], scale,
-                                                                dw.data_ptr(), ws.data_ptr(), need, stream)), "gs_embedding_bwd")
+    device = g.get_device()
+    args = (ids.data_ptr(), kind, g.data_ptr(), ldg, T, V, D, padding_idx, code, scale, dw.data_ptr(), ws.data_ptr(), need, _stream_of(device))
+    if _current_device() == device:
+        rc = _lib.lib().gs_embedding_bwd(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = _lib.lib().gs_embedding_bwd(*args)
+    if rc:
+        check(rc, "gs_embedding_bwd")
     return None, dw, None, None
 
 
@@ -222,7 +242,8 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
-        ctx.rest = (*weight.shape, scale, padding_idx)
+        T, (V, D) = ids.numel(), weight.shape
+        ctx.rest = (_ID_TYPES[ids.dtype], T, V, D, padding_idx, _DTYPES[weight.dtype], scale, _lib.lib().gs_embedding_bwd_workspace_bytes(T, V, D))
         return _lookup(ids, weight, scale)
 
     @staticmethod

@@ -6,8 +6,8 @@ arithmetic (ATen/native/cuda/fused_adam_utils.cuh).  The reference trains with t
 
 And the gradient's global norm with clipping by it, two HIP launches over all tensors (csrc/gradnorm.hip: gs_grad_norm): grad_norm, clip_grads, clip_grad_norm_."""
 import ctypes
+from array import array
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -96,11 +96,7 @@ def _norm_code(norm_type, what):
     return code
 
 
-def _check_grads(tensors, what):
-    """One device for all, dense, of a known type -- on the host, before anything is launched."""
-    if {t.layout for t in tensors} == {torch.strided} and all([t.dtype in _GRAD_TYPES for t in tensors]) and all([t.is_cuda for t in tensors]) \
-            and len({t.get_device() for t in tensors}) == 1:
-        return
+def _refuse_grads(tensors, what):
     for t in tensors:
         if t.layout is not torch.strided or t.dtype not in _GRAD_TYPES:
             raise _lib.GShellHipError(f"{what}: dense float32, bfloat16 or float16 tensors are wanted, got {t.dtype} ({t.layout})")
@@ -111,49 +107,35 @@ def _check_grads(tensors, what):
             raise _lib.GShellHipError(f"{what}: tensors are on {tensors[0].device} and on {t.device}")
 
 
-def _addresses(tensors):
-    return np.array([t.data_ptr() for t in tensors], dtype=np.int64)
+def _check_grads(tensors, what):
+    """Type codes of `tensors`: dense, on one device, of known types -- on the host, before anything is launched."""
+    types = [_GRAD_TYPES.get(t.dtype) for t in tensors]
+    devices = {t.get_device() for t in tensors if t.layout is torch.strided and t.is_cuda}
+    if None in types or len(devices) != 1 or not all([t.layout is torch.strided and t.is_cuda for t in tensors]):
+        _refuse_grads(tensors, what)
+    return types
 
 
-def _check_apart(written, read, sizes, what):
-    """No two of the written stretches of memory overlap, and none overlaps one that is read, unless it is that gradient's own place.  Addresses and sizes in bytes."""
-    some = sizes > 0
-    order = np.argsort(written[some], kind="stable")
-    a, z = written[some][order], sizes[some][order]
-    if (a[:-1] + z[:-1] > a[1:]).any():
-        raise _lib.GShellHipError(f"{what}: two of the tensors that are written share memory")
-    other = some & (read != written)
-    if other.any():
-        # the last written stretch that starts before a read one ends must end before that starts
-        r, rz = read[other], sizes[other]
-        k = np.searchsorted(a, r + rz, side="left") - 1
-        if ((k >= 0) & (a[k] + z[k] > r)).any():
-            raise _lib.GShellHipError(f"{what}: an output shares memory with another gradient")
-
-
-def _launch_norm(like, src, dst, numel, types, max_norm, code):
-    """gs_grad_norm over addresses, element counts and type codes (numpy arrays)."""
-    n = len(src)
+def _launch_norm(src, dst, types, max_norm, code):
+    """gs_grad_norm over contiguous tensors (dst None: the norm alone)."""
+    n, like = len(src), src[0]
     L = _lib.lib()
     need = L.gs_grad_norm_workspace_bytes(n)
     dev = like.get_device()
     norm = like.new_empty((), dtype=torch.float32)
     ws = like.new_empty(need, dtype=torch.uint8)
-
-    def call():
-        return L.gs_grad_norm(n, src.ctypes.data, None if dst is None else dst.ctypes.data, numel.ctypes.data, types.ctypes.data, code, max_norm, norm.data_ptr(), ws.data_ptr(),
-                              need, torch.cuda.current_stream(dev).cuda_stream)
+    at, numel, kinds = array("q", [t.data_ptr() for t in src]), array("q", [t.numel() for t in src]), array("i", types)
+    to = None if dst is None else at if dst is src else array("q", [t.data_ptr() for t in dst])
+    args = (n, at.buffer_info()[0], None if to is None else to.buffer_info()[0], numel.buffer_info()[0], kinds.buffer_info()[0], code, max_norm, norm.data_ptr(), ws.data_ptr(),
+            need, torch.cuda.current_stream(dev).cuda_stream)
     if torch.cuda.current_device() == dev:
-        rc = call()
+        rc = L.gs_grad_norm(*args)
     else:
         with torch.cuda.device(dev):
-            rc = call()
-    check(rc, "gs_grad_norm")
+            rc = L.gs_grad_norm(*args)
+    if rc:
+        check(rc, "gs_grad_norm")
     return norm
-
-
-def _counts(tensors):
-    return np.array([t.numel() for t in tensors], dtype=np.int64), np.array([_GRAD_TYPES[t.dtype] for t in tensors], dtype=np.int32)
 
 
 @torch.no_grad()
@@ -163,43 +145,38 @@ def grad_norm(tensors, norm_type=2.0):
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     if not tensors:
         return torch.zeros(())
-    _check_grads(tensors, "grad_norm")
-    tensors = [t if t.is_contiguous() else t.contiguous() for t in tensors]
-    numel, types = _counts(tensors)
-    return _launch_norm(tensors[0], _addresses(tensors), None, numel, types, 0.0, code)
+    types = _check_grads(tensors, "grad_norm")
+    return _launch_norm([t if t.is_contiguous() else t.contiguous() for t in tensors], None, types, 0.0, code)
 
 
 @torch.no_grad()
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)) -> norm, one fp32 value on the device.  Without `out`, in place.
 
-    `out`: tensors of the gradients' shapes and types; one may be its gradient's own place, otherwise no output shares memory with a gradient or another output.  A norm that
-    is NaN makes every output NaN, one that is infinite makes finite elements zero."""
+    `out`: tensors of the gradients' shapes and types; one may be its gradient's own place, otherwise no output shares memory with a gradient or another output (such a
+    call is refused).  A norm that is NaN makes every output NaN, one that is infinite makes finite elements zero."""
     code = _norm_code(norm_type, "clip_grads")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise _lib.GShellHipError(f"clip_grads: max_norm must not be negative or NaN, got {max_norm}")
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
-    if len(out) != len(grads):
-        raise _lib.GShellHipError(f"clip_grads: {len(grads)} gradients and {len(out)} outputs")
-    for g, o in zip(grads, out):
-        if o is not g and (o.shape != g.shape or o.dtype != g.dtype):
-            raise _lib.GShellHipError(f"clip_grads: an output is {tuple(o.shape)} {o.dtype}, its gradient {tuple(g.shape)} {g.dtype}")
+    if out is not grads:
+        if len(out) != len(grads):
+            raise _lib.GShellHipError(f"clip_grads: {len(grads)} gradients and {len(out)} outputs")
+        for g, o in zip(grads, out):
+            if o.shape != g.shape or o.dtype != g.dtype:
+                raise _lib.GShellHipError(f"clip_grads: an output is {tuple(o.shape)} {o.dtype}, its gradient {tuple(g.shape)} {g.dtype}")
     if not grads:
         return torch.zeros(())
-    _check_grads(grads, "clip_grads")
+    types = _check_grads(grads, "clip_grads")
     if out is not grads:
         _check_grads(out, "clip_grads")
         if out[0].get_device() != grads[0].get_device():
             raise _lib.GShellHipError(f"clip_grads: gradients are on {grads[0].device}, outputs on {out[0].device}")
     src = [g if g.is_contiguous() else g.contiguous() for g in grads]
     dst = src if out is grads else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in out]
-    numel, types = _counts(src)
-    at = _addresses(src)
-    to = at if dst is src else _addresses(dst)
-    _check_apart(to, at, numel * np.where(types == 0, 4, 2), "clip_grads")
-    norm = _launch_norm(src[0], at, to, numel, types, max_norm, code)
+    norm = _launch_norm(src, dst, types, max_norm, code)
     for o, d in zip(out, dst):
         if d is not o:
             o.copy_(d)

@@ -893,7 +893,8 @@ int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64_t ldg, int
 /* ------------------------------------------------------------------------------------
  * Global norm of a list of gradients, and clipping by it   (torch.nn.utils.clip_grad_norm_ in the train script, :440-444)
  *   norm (one fp32 on the device) = (sum |g|^p)^(1/p), summed in 64 bits; norm_type 0: p = 2, 1: p = 1, 2: the largest magnitude.
- *   out not null: out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type; out[k] may be grads[k].
+ *   out not null: out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type; out[k] may be grads[k],
+ *   otherwise no output may overlap a gradient or another output (refused).
  *   Host arrays of device pointers, element counts and dtypes (0 fp32, 1 bf16, 2 fp16); tensors are contiguous and may start at any element.
  * ---------------------------------------------------------------------------------- */
 int64_t gs_grad_norm_workspace_bytes(int n_tensors);

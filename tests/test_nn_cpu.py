@@ -103,16 +103,17 @@ def test_clip_refuses():
     ([(0, 10), (50, 10)], [(0, 10), (60, 10)], True), ([(5, 0)], [(5, 0)], True), ([(5, 0), (0, 20)], [(3, 0), (0, 20)], True),
 ])
 def test_clip_refuses_shared_memory(written, read, fine):
-    """(address, bytes) of the outputs and of the gradients."""
-    import numpy as np
-    from gshell_amd import optim
-    at = lambda v: np.array([a for a, _ in v], dtype=np.int64)      # noqa: E731
-    sizes = np.array([z for _, z in written], dtype=np.int64)
+    """(address, elements of 4 bytes) of the outputs and of the gradients: the C entry's check on the host.  A list that passes is stopped by its workspace's size."""
+    import ctypes
+    from gshell_amd import _lib
+    L, n = _lib.lib(), len(written)
+    base = 1 << 20
+    at = lambda v: (ctypes.c_void_p * n)(*[base + 4 * a for a, _ in v])      # noqa: E731
+    call = lambda ws: L.gs_grad_norm(n, at(read or written), at(written), (ctypes.c_int64 * n)(*[z for _, z in written]), (ctypes.c_int32 * n)(), 0, 1.0, 256, 256, ws, 0)      # noqa: E731
     if fine:
-        optim._check_apart(at(written), at(read or written), sizes, "clip_grads")
+        assert call(0) != 0 and b"workspace" in L.gs_last_error()
     else:
-        with pytest.raises(GShellHipError, match="memory"):
-            optim._check_apart(at(written), at(read or written), sizes, "clip_grads")
+        assert call(1 << 30) != 0 and b"shares memory" in L.gs_last_error()
 
 
 def test_clip_c_entry_refuses_bad_arguments():
