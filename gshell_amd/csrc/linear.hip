@@ -189,56 +189,94 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t tiles_m, uint32_t 
     ti = first + in % rows, tj = in / rows;
 }
 
-// A wave's TM x 4 tiles of sums, through 16 KB of LDS of its own, 64 lines at a time: the lanes then hold 16 bytes of neighbouring outputs each, and 8 (16-bit) or 16 (fp32)
-// lanes a whole line of 64.  The 16-byte piece p of line l is kept at p ^ (l & 15).  fix(i, j, z): what a sum is replaced by.
+// A wave's sums go to memory through 16 KB of LDS, 64 x 64 at a time: the lanes then hold 16 bytes of neighbouring outputs each, and 8 (16-bit) or 16 (fp32) lanes a whole
+// line of 64.  The 16-byte piece p of line l is kept at p ^ (l & 15).
+__device__ __forceinline__ int piece_of_sums(int line, int piece) { return line * 64 + (piece ^ (line & 15)) * 4; }
+template <int TM> __device__ __forceinline__ void put_sums(const f32x4 (&acc)[TM][4], int first, float* lds) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) *(f32x4*)(lds + piece_of_sums(u * 16 + (lane & 15), w * 4 + (lane >> 4))) = acc[first + u][w];
+}
+// Lines l_begin .. l_end of them, BATCH lines a lane side by side, as many as the registers hold: what they read of the residual is in flight together.
+// fix(i, j, z): what a sum is replaced by.
+template <typename T, int BATCH, typename F>
+__device__ __forceinline__ void drain_sums(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
+    constexpr int V = width<T>(), LANES = 64 / V, LINES = 64 / LANES;
+    const int lane = threadIdx.x & 63, c = lane % LANES * V;
+    const int64_t j = j0 + c;
+#pragma unroll 1
+    for (int l0 = l_begin; l0 < l_end; l0 += LINES * BATCH) {
+        int64_t i[BATCH];
+        float z[BATCH][V];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int l = l0 + b * LINES + lane / LANES;
+            i[b] = i0 + l;
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const f32x4 q = *(const f32x4*)(lds + piece_of_sums(l, (c + k) >> 2));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[b][k + e] = q[e];
+            }
+            if (i[b] < M && j < N) fix(i[b], j, z[b]);
+        }
+        if (E.part) {
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (i[b] < M && j < N) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i[b]) * N + j, N - j, z[b]);
+        } else if (j < N) {
+            finish<T, V, BATCH>(E, i, j, M, N, z);
+        }
+    }
+}
 template <typename T, int TM, int BATCH, typename F>
 __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&acc)[TM][4], float* lds, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
-    constexpr int V = width<T>(), LANES = 64 / V, LINES = 64 / LANES;
-    const int lane = threadIdx.x & 63;
 #pragma unroll 1
     for (int part = 0; part < TM / 4; ++part) {
 #pragma unroll
         for (int p = 0; p < TM / 4; ++p)
-            if (p == part)
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int l = u * 16 + (lane & 15);
-                        *(f32x4*)(lds + l * 64 + ((w * 4 + (lane >> 4)) ^ (l & 15)) * 4) = acc[p * 4 + u][w];
-                    }
+            if (p == part) put_sums<TM>(acc, 4 * p, lds);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        // BATCH lines a lane side by side, as many as the registers beside the sums hold: what they read of the residual is in flight together
+        drain_sums<T, BATCH>(E, lds, 0, 64, i0 + part * 64, j0, M, N, fix);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
 
-#pragma unroll 1
-        for (int l0 = 0; l0 < 64; l0 += LINES * BATCH) {
-            const int c = lane % LANES * V;
-            const int64_t j = j0 + c;
-            int64_t i[BATCH];
-            float z[BATCH][V];
+// Sums of columns by slabs of rows, joined: 32 columns a workgroup, the slabs in stretches side by side, in their order.  Done by workgroups that a later launch has
+// beside its own.
+template <typename T> struct Columns {
+    const float* part;          // [slabs][N]
+    T* db;
+    int64_t N;
+    int slabs;
+    uint32_t blocks;
+};
+template <typename T> __device__ __forceinline__ void join_columns(const Columns<T>& C, uint32_t block, float* lds) {
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, groups = blockDim.x >> 5;
+    const int64_t j = (int64_t)block * 32 + x;
+    const int share = (C.slabs + groups - 1) / groups, k0 = y * share, k1 = k0 + share < C.slabs ? k0 + share : C.slabs;
+    float s = 0.f;
+    if (j < C.N) {
+        int k = k0;
+        for (; k + 8 <= k1; k += 8) {
+            float q[8];
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int l = l0 + b * LINES + lane / LANES;
-                i[b] = i0 + part * 64 + l;
+            for (int e = 0; e < 8; ++e) q[e] = C.part[(int64_t)(k + e) * C.N + j];
 #pragma unroll
-                for (int k = 0; k < V; k += 4) {
-                    const f32x4 q = *(const f32x4*)(lds + l * 64 + (((c + k) >> 2) ^ (l & 15)) * 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) z[b][k + e] = q[e];
-                }
-                if (i[b] < M && j < N) fix(i[b], j, z[b]);
-            }
-            if (E.part) {
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b)
-                    if (i[b] < M && j < N) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i[b]) * N + j, N - j, z[b]);
-            } else if (j < N) {
-                finish<T, V, BATCH>(E, i, j, M, N, z);
-            }
+            for (int e = 0; e < 8; ++e) s += q[e];
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        for (; k < k1; ++k) s += C.part[(int64_t)k * C.N + j];
+    }
+    lds[y * 33 + x] = s;
+    __syncthreads();
+    if (y == 0 && j < C.N) {
+        float t = 0.f;
+        for (int q = 0; q < groups; ++q) t += lds[q * 33 + x];
+        C.db[j] = (T)t;
     }
 }
 
@@ -342,7 +380,7 @@ template <bool COLS, bool GATE> struct Feed32 {
 
 template <bool ACOLS, bool BCOLS, bool GATE>
 __global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<float> E,
-                                                      float* column_sums) {
+                                                      float* column_sums /* [slices][M], or db itself where there is one slice */) {
     __shared__ __attribute__((aligned(16))) union {
         struct { short a[3 * PLANE], b[3 * PLANE]; } in;
         float out[4 * 64 * 64];
@@ -507,23 +545,27 @@ template <int LEFT> __device__ __forceinline__ void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, int BUFFERS>
-__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BUFFERS == 2 ? 2 : 1) k_product16(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E) {
+template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E,
+                                                                           Columns<T> C) {
 #if defined(__HIP_DEVICE_COMPILE__)          // the host pass has no type for a buffer's descriptor
     constexpr int THREADS = BM / WM * (BN / WN) * 64, TM = WM / 16, TN = WN / 16, PARTS = TM / 4, CLUSTERS = 2 * PARTS;
     // each buffer (A's tile, then B's) is a variable of its own: the compiler then knows which loads a read of LDS has to wait for
     constexpr int BUFFER = (BM + BN) * STEP;
-    __shared__ __attribute__((aligned(1024))) short s0[BUFFER], s1[BUFFER], s2[BUFFERS > 2 ? BUFFER : 8], s3[BUFFERS > 2 ? BUFFER : 8];
-    static_assert(BUFFERS == 2 || BUFFERS == 4, "buffers");
+    __shared__ __attribute__((aligned(1024))) short s0[BUFFER], s1[BUFFER];
+    const uint32_t tiles_m = (uint32_t)((M + BM - 1) / BM), tiles_n = (uint32_t)((N + BN - 1) / BN);
+    if (blockIdx.x >= tiles_m * tiles_n) {
+        if (blockIdx.y == 0) join_columns<T>(C, blockIdx.x - tiles_m * tiles_n, (float*)s0);
+        return;
+    }
     uint32_t ti, tj;
-    tile_of(blockIdx.x, (uint32_t)((M + BM - 1) / BM), (uint32_t)((N + BN - 1) / BN), ti, tj);
+    tile_of(blockIdx.x, tiles_m, tiles_n, ti, tj);
     const int64_t i0 = (int64_t)ti * BM, j0 = (int64_t)tj * BN;
     const int64_t c_begin = (int64_t)blockIdx.y * slice, len = (c_begin + slice < K ? c_begin + slice : K) - c_begin;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
     Feed<ACOLS, BM, THREADS> fa;
     Feed<BCOLS, BN, THREADS> fb;
-    constexpr int LOADS = Feed<ACOLS, BM, THREADS>::LOADS + Feed<BCOLS, BN, THREADS>::LOADS;
     fa.init(A.p, A.ld, i0, lines_a, c_begin);
     fb.init(B.p, B.ld, j0, lines_b, c_begin);
     f32x4 acc[TM][TN] = {};
@@ -558,62 +600,123 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, BUFFERS == 2 ? 2 : 1
             read(s, c + 1);
             multiply(c);
         }
-        // the next step's tiles have arrived, and nobody reads this step's any more
-        wait_and_meet<(BUFFERS - 2) * LOADS>();
-        // With four buffers every step loads and reads ahead, behind the end too (nothing but zeros comes from there): without branches the compiler sees which loads a
-        // read waits for.  With two it waits for all of them anyway, and the branches keep the loads in front of the last products.
-        if (BUFFERS > 2 || ++k < steps) read(next, 0);
-        if (BUFFERS > 2 || k + 1 < steps) load(s);
+        wait_and_meet<0>();          // the next step's tiles have arrived, and nobody reads this step's any more
+        if (++k < steps) read(next, 0);
+        if (k + 1 < steps) load(s);
         multiply(CLUSTERS - 1);
     };
-    load(s0);
-    load(s1);
-    if constexpr (BUFFERS > 2) {
-        load(s2);
-        load(s3);
-    }
-    wait_and_meet<(BUFFERS - 1) * LOADS>();
-    read(s0, 0);
-    if constexpr (BUFFERS == 2) {
-        while (k < steps) {
-            step(s0, s1);
-            if (k < steps) step(s1, s0);
-        }
-    } else {
-        for (; k + 4 <= steps; k += 4) {
-            step(s0, s1);
-            step(s1, s2);
-            step(s2, s3);
-            step(s3, s0);
-        }
-        if (k < steps) step(s0, s1);
-        if (k + 1 < steps) step(s1, s2);
-        if (k + 2 < steps) step(s2, s3);
-    }
+    if (steps > 0) load(s0);
+    if (steps > 1) load(s1);
     wait_and_meet<0>();
-    // nobody reads or loads tiles any more: the first two buffers hold the waves' sums
+    if (steps > 0) read(s0, 0);
+    while (k < steps) {
+        step(s0, s1);
+        if (k < steps) step(s1, s0);
+    }
+    // nobody reads or loads tiles any more: the buffers hold the waves' sums
     static_assert(WN == 64 && BUFFER * 2 * 2 == THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
     constexpr int SHARE = THREADS / 64 / 2;
     short* mine = wave < SHARE ? s0 : s1;
-    store_wave<T, TM, (BUFFERS > 2 ? 8 : TM > 4 ? 2 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+    store_wave<T, TM, (TM > 4 ? 2 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
 #endif
 }
 
-// rows copied to rows that start on 16 bytes, zeros behind their ends
-template <typename T> __global__ void __launch_bounds__(256) k_pack(const T* p, int64_t ld, int64_t rows, int64_t cols, T* out, int64_t ldo) {
-    const int64_t vectors = ldo / 8, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= rows * vectors) return;
-    const int64_t r = at / vectors, c = at % vectors * 8;
-    s16x8 v;
+// The same product where the tiles do not fill the chip and latency is what counts: one workgroup a compute unit, tiles of BM x 128, four buffers, so that three steps are
+// on their way while one is multiplied, and twice the waves: each 64 x 64 of the tile is done by two of them, one for either half of a step, whose sums are added in the end.
+// Every step loads and reads ahead, behind the end too (nothing but zeros comes from there): without branches the compiler sees which loads a read waits for.
+template <typename T, bool ACOLS, bool BCOLS, int BM>
+__global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E, Columns<T> C) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int THREADS = BM * 4, QUARTERS = BM / 32, BUFFER = (BM + TILE) * STEP;
+    __shared__ __attribute__((aligned(1024))) short s0[BUFFER], s1[BUFFER], s2[BUFFER], s3[BUFFER];
+    const uint32_t tiles_m = (uint32_t)((M + BM - 1) / BM), tiles_n = (uint32_t)((N + TILE - 1) / TILE);
+    if (blockIdx.x >= tiles_m * tiles_n) {
+        if (blockIdx.y == 0) join_columns<T>(C, blockIdx.x - tiles_m * tiles_n, (float*)s0);
+        return;
+    }
+    uint32_t ti, tj;
+    tile_of(blockIdx.x, tiles_m, tiles_n, ti, tj);
+    const int64_t i0 = (int64_t)ti * BM, j0 = (int64_t)tj * TILE;
+    const int64_t c_begin = (int64_t)blockIdx.y * slice, len = (c_begin + slice < K ? c_begin + slice : K) - c_begin;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quarter = wave % QUARTERS, half = wave / QUARTERS, wi = (quarter >> 1) * 64, wj = (quarter & 1) * 64;
+    Feed<ACOLS, BM, THREADS> fa;
+    Feed<BCOLS, TILE, THREADS> fb;
+    constexpr int LOADS = Feed<ACOLS, BM, THREADS>::LOADS + Feed<BCOLS, TILE, THREADS>::LOADS;
+    fa.init(A.p, A.ld, i0, lines_a, c_begin);
+    fb.init(B.p, B.ld, j0, lines_b, c_begin);
+    f32x4 acc[4][4] = {};
+    s16x8 va[4], vb[4];
+    const int steps = (int)((len + STEP - 1) / STEP);
+    int64_t left = len;
+    const auto load = [&](short* s) __attribute__((always_inline)) {
+        fa.load(s, left);
+        fb.load(s + BM * STEP, left);
+        left -= STEP;
+    };
+    const auto read = [&](const short* s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? raw(p[r * ld + c + k]) : (short)0;
-    *(s16x8*)(out + r * ldo + c) = v;
+        for (int u = 0; u < 4; ++u) va[u] = fragment<ACOLS, BM>(s, wi + u * 16, half);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) vb[w] = fragment<BCOLS, TILE>(s + BM * STEP, wj + w * 16, half);
+    };
+    const auto step = [&](short* s, short* next) __attribute__((always_inline)) {
+        wait_and_meet<2 * LOADS>();          // the next step's tiles have arrived, and nobody reads this step's any more
+        s16x8 xa[4], xb[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) xa[u] = va[u], xb[u] = vb[u];
+        read(next);
+        load(s);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) acc[u][w] = mfma<T>(xb[w], xa[u], acc[u][w]);
+    };
+    load(s0);
+    load(s1);
+    load(s2);
+    load(s3);
+    wait_and_meet<3 * LOADS>();
+    read(s0);
+    int k = 0;
+    for (; k + 4 <= steps; k += 4) {
+        step(s0, s1);
+        step(s1, s2);
+        step(s2, s3);
+        step(s3, s0);
+    }
+    if (k < steps) step(s0, s1);
+    if (k + 1 < steps) step(s1, s2);
+    if (k + 2 < steps) step(s2, s3);
+    wait_and_meet<0>();
+    // nobody reads or loads tiles any more: one half's sums into LDS, the other's onto them, and each wave takes half of the lines to memory
+    constexpr int PER = BUFFER * 2 / (64 * 64 * 4);          // 64 x 64 sums that a buffer holds
+    static_assert(QUARTERS <= 2 * PER, "LDS for the sums");
+    float* sums = (float*)(quarter < PER ? s0 : s1) + quarter % PER * 64 * 64;
+    if (half == 1) put_sums<4>(acc, 0, sums);
+    __syncthreads();
+    if (half == 0) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f32x4* at = (f32x4*)(sums + piece_of_sums(u * 16 + (lane & 15), w * 4 + (lane >> 4)));
+                const f32x4 other = *at;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][w][e] += other[e];
+                *at = acc[u][w];
+            }
+    }
+    __syncthreads();
+    drain_sums<T, 4>(E, sums, half * 32, half * 32 + 32, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+#endif
 }
 
 // The slices of a contraction joined, then the epilogue.  `groups` lanes of a workgroup share the slices of four outputs in equal stretches, in their order.
-template <typename T> __global__ void __launch_bounds__(256) k_join(const float* part, int splits, int groups, int64_t M, int64_t N, Epilogue<T> E) {
+template <typename T> __global__ void __launch_bounds__(256) k_join(const float* part, int splits, int groups, int64_t M, int64_t N, Epilogue<T> E, uint32_t blocks, Columns<T> C) {
     constexpr int V = 4;
-    __shared__ f32x4 sums[256];
+    __shared__ f32x4 sums[256 + 16];
+    if (blockIdx.x >= blocks) return join_columns<T>(C, blockIdx.x - blocks, (float*)sums);
     const int each = 256 / groups, group = threadIdx.x / each, x = threadIdx.x % each;
     const int64_t vectors = (N + V - 1) / V, at = (int64_t)blockIdx.x * each + x;
     const int share = (splits + groups - 1) / groups, s0 = group * share, s1 = s0 + share < splits ? s0 + share : splits;
@@ -642,60 +745,72 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
     if (ok) finish<T, V, 1>(E, line, j, M, N, z);
 }
 
-// gz = g act'(z), rounded to the layer's type for the two products that read it (rows that start on 16 bytes, zeros behind their ends), and its column sums (of
-// the unrounded values) by slabs of rows
+// What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type, in rows that start on 16 bytes with zeros behind their ends, and its
+// column sums (of the unrounded values) by slabs of rows.  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
 constexpr int GZ_LANES = 32, GZ_LINES = 8;
-template <typename T>
-__global__ void __launch_bounds__(256) k_gz(const T* g, int64_t ldg, const typename dact_type<T>::type* dact, int64_t M, int64_t N, int64_t slab, T* gz, int64_t ldgz, float* part) {
+template <typename T> struct Gz {
+    const T* g;
+    const typename dact_type<T>::type* dact;
+    T* gz;                          // null: the sums alone
+    float* part;                    // [slabs][N], or null
+    int64_t ldg, ldgz, M, N, slab;
+    uint32_t across, blocks;
+};
+template <typename T> struct Pack2 {
+    const T* p[2];
+    T* out[2];
+    int64_t ld[2], ldo[2], rows[2], cols[2];
+    uint32_t first, blocks[2];
+};
+template <typename T> __global__ void __launch_bounds__(256) k_prepare(Gz<T> G, Pack2<T> P) {
     constexpr int V = width<T>();
     __shared__ float sums[GZ_LINES][GZ_LANES * V];
+    if (blockIdx.x >= G.blocks) {
+        uint32_t block = blockIdx.x - G.blocks;
+        const int q = block >= P.blocks[0] ? 1 : 0;
+        block -= q ? P.blocks[0] : 0;
+        const int64_t vectors = P.ldo[q] / V, at = (int64_t)block * 256 + threadIdx.x;
+        if (at >= P.rows[q] * vectors) return;
+        const int64_t r = at / vectors, c = at % vectors * V;
+        float v[V];
+        load_some<T, V>(P.p[q] + r * P.ld[q] + c, P.cols[q] - c, v);
+        store_some<T, V>(P.out[q] + r * P.ldo[q] + c, V, v);
+        return;
+    }
     const int x = threadIdx.x % GZ_LANES, y = threadIdx.x / GZ_LANES;
-    const int64_t j = ((int64_t)blockIdx.x * GZ_LANES + x) * V, in_row = N - j;
-    const int64_t m0 = (int64_t)blockIdx.y * slab, m1 = m0 + slab < M ? m0 + slab : M;
+    const int64_t bx = blockIdx.x % G.across, by = blockIdx.x / G.across;
+    const int64_t j = (bx * GZ_LANES + x) * V, in_row = G.N - j;
+    const int64_t m0 = by * G.slab, m1 = m0 + G.slab < G.M ? m0 + G.slab : G.M;
     float s[V] = {};
     if (in_row > 0)
         for (int64_t m = m0 + y; m < m1; m += GZ_LINES) {
             float v[V], d[V];
-            load_some<T, V>(g + m * ldg + j, in_row, v);
-            if (dact) {
-                load_some<typename dact_type<T>::type, V>(dact + m * N + j, in_row, d);
+            load_some<T, V>(G.g + m * G.ldg + j, in_row, v);
+            if (G.dact) {
+                load_some<typename dact_type<T>::type, V>(G.dact + m * G.N + j, in_row, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) v[k] *= d[k];
             }
-            if (gz) store_some<T, V>(gz + m * ldgz + j, V, v);
+            if (G.gz) store_some<T, V>(G.gz + m * G.ldgz + j, V, v);
 #pragma unroll
             for (int k = 0; k < V; ++k) s[k] += v[k];
         }
-    if (!part) return;
+    if (!G.part) return;
 #pragma unroll
     for (int k = 0; k < V; ++k) sums[y][x * V + k] = s[k];
     __syncthreads();
     for (int c = threadIdx.x; c < GZ_LANES * V; c += 256) {
-        const int64_t at = (int64_t)blockIdx.x * GZ_LANES * V + c;
+        const int64_t at = bx * GZ_LANES * V + c;
         float t = 0.f;
 #pragma unroll
         for (int q = 0; q < GZ_LINES; ++q) t += sums[q][c];
-        if (at < N) part[(int64_t)blockIdx.y * N + at] = t;
+        if (at < G.N) G.part[by * G.N + at] = t;
     }
 }
 
-// the slabs of a column, 32 stretches of them side by side
-template <typename T> __global__ void __launch_bounds__(1024) k_column_join(const float* part, int slabs, int64_t N, T* db) {
-    __shared__ float sums[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    const int64_t j = (int64_t)blockIdx.x * 32 + x;
-    const int share = (slabs + 31) / 32, k1 = (y + 1) * share < slabs ? (y + 1) * share : slabs;
-    float s = 0.f;
-    if (j < N)
-        for (int k = y * share; k < k1; ++k) s += part[(int64_t)k * N + j];
-    sums[y][x] = s;
-    __syncthreads();
-    if (y == 0 && j < N) {
-        float t = 0.f;
-#pragma unroll
-        for (int q = 0; q < 32; ++q) t += sums[q][x];
-        db[j] = (T)t;
-    }
+template <typename T> __global__ void __launch_bounds__(1024) k_join_columns(Columns<T> C) {
+    __shared__ float lds[32 * 33];
+    join_columns<T>(C, blockIdx.x, lds);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -703,138 +818,151 @@ constexpr int CUS = 256;
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
-// How a product is run: the kernel, the slices of its contraction, what is repacked first, and what of the workspace each takes.
+// How a product is run: the kernel, the slices of its contraction, and what of the workspace it takes.
 struct Plan {
-    int tile = TILE;                    // 256 or 128
-    bool deep = false;                  // 128 with four buffers, one workgroup a compute unit, rather than two with two buffers each
-    int64_t splits = 1, slice = 0;
-    int64_t pack_a = 0, pack_b = 0;          // row strides of the repacked operands, 0: as they are
-    int64_t at_a = 0, at_b = 0, at_part = 0, at_cols = 0, bytes = 0;
+    int rows = TILE, cols = TILE;          // of a tile
+    bool deep = false;                     // k_product16_deep
+    int64_t tiles = 0, splits = 1, slice = 0;
+    int64_t at_cols = 0, bytes = 0;          // the slices' sums come first, then their column sums
 };
-struct Line {          // an operand as the plan sees it
-    const void* p;
-    int64_t ld, cols;          // row stride, elements of a row that are read
-    bool zeros;                // rows have zeros up to a multiple of 8 behind their ends
-};
-// The 16-bit kernels load 16 bytes at a time into LDS, by 31-bit offsets within a tile.
-static bool direct(const Line& a) { return ((uintptr_t)a.p & 15) == 0 && a.ld % 8 == 0 && (a.cols % 8 == 0 || a.zeros) && a.ld < (1 << 21); }
-
-static Plan plan(int es, Line a, int64_t rows_a, Line b, int64_t rows_b, int64_t M, int64_t N, int64_t K, bool column_sums = false) {
+static Plan plan(int es, int64_t M, int64_t N, int64_t K, bool column_sums) {
     Plan p;
-    int64_t tiles = gs::cdiv(M, TILE) * gs::cdiv(N, TILE);
+    const auto tiles = [&](int64_t r, int64_t c) { return gs::cdiv(M, r) * gs::cdiv(N, c); };
+    p.tiles = tiles(TILE, TILE);
+    int64_t slots = 2 * CUS, least = 256;
     if (es == 2) {
-        const int64_t big = gs::cdiv(M, 256) * gs::cdiv(N, 256);
-        if (big >= 192) p.tile = 256, tiles = big;
-        if (!direct(a)) p.pack_a = up8(a.cols);
-        if (!direct(b)) p.pack_b = up8(b.cols);
+        if (tiles(256, 256) >= 192) {
+            p.rows = p.cols = 256, slots = CUS;
+        } else if (p.tiles <= CUS) {
+            p.deep = true, slots = CUS, least = 512;
+            if (tiles(64, TILE) <= CUS) p.rows = 64;
+        }
+        p.tiles = tiles(p.rows, p.cols);
     }
-    if (es == 2 && p.tile == 128) p.deep = tiles <= CUS;
-    const int64_t slots = p.tile == 256 || p.deep ? CUS : 2 * CUS, least = p.deep ? 512 : 256;
-    if (tiles < slots && K >= 2 * least) {
-        p.splits = slots / tiles;
+    if (p.tiles < slots && K >= 2 * least) {
+        p.splits = slots / p.tiles;
         if (p.splits > K / least) p.splits = K / least;
         if (p.splits > 256) p.splits = 256;
         if (p.splits < 1) p.splits = 1;
     }
     p.slice = p.splits > 1 ? gs::cdiv(gs::cdiv(K, p.splits), 64) * 64 : K;
     p.splits = p.splits > 1 ? gs::cdiv(K, p.slice) : 1;
-    int64_t at = 0;
-    p.at_a = at, at += p.pack_a ? align256(rows_a * p.pack_a * es) : 0;
-    p.at_b = at, at += p.pack_b ? align256(rows_b * p.pack_b * es) : 0;
-    p.at_part = at, at += p.splits > 1 ? align256(p.splits * M * N * 4) : 0;
-    p.at_cols = at, at += column_sums ? align256(p.splits * M * 4) : 0;
-    p.bytes = at;
+    p.at_cols = p.splits > 1 ? align256(p.splits * M * N * 4) : 0;
+    p.bytes = p.at_cols + (column_sums && p.splits > 1 ? align256(p.splits * M * 4) : 0);
     return p;
 }
 
-template <typename T> int pack(const void* p, int64_t ld, int64_t rows, int64_t cols, void* out, int64_t ldo, hipStream_t stream) {
-    const int64_t blocks = gs::cdiv(rows * (ldo / 8), 256);
-    GS_REQUIRE(blocks < (1ll << 31), "gs_linear: operand too large");
-    hipLaunchKernelGGL(k_pack<T>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T*)p, ld, rows, cols, (T*)out, ldo);
+// An operand: the 16-bit kernels read its rows 16 bytes at a time, by 31-bit offsets within a tile; rows that do not start on 16 bytes, or end inside of them, are
+// repacked first.
+struct Line {
+    const void* p;
+    int64_t ld, cols;          // row stride, elements of a row that are read
+    bool zeros;                // rows have zeros up to a multiple of 8 behind their ends
+};
+static bool direct(const Line& a) { return ((uintptr_t)a.p & 15) == 0 && a.ld % 8 == 0 && (a.cols % 8 == 0 || a.zeros) && a.ld < (1 << 21); }
+static int64_t packed_bytes(int es, const Line& a, int64_t rows) { return es == 2 && !direct(a) ? align256(rows * up8(a.cols) * es) : 0; }
+
+// One more operand for the repacking launch, where it needs it.
+template <typename T> int64_t repack(Pack2<T>& P, int q, Line& a, int64_t rows, char* to) {
+    const int64_t bytes = packed_bytes(sizeof(T), a, rows);
+    if (!bytes) return 0;
+    P.p[q] = (const T*)a.p, P.ld[q] = a.ld, P.rows[q] = rows, P.cols[q] = a.cols, P.out[q] = (T*)to, P.ldo[q] = up8(a.cols);
+    P.blocks[q] = (uint32_t)gs::cdiv(rows * (P.ldo[q] / width<T>()), 256);
+    a = {to, P.ldo[q], a.cols, true};
+    return bytes;
+}
+template <typename T> int prepare(const Gz<T>& G, const Pack2<T>& P, hipStream_t stream) {
+    const uint64_t blocks = (uint64_t)G.blocks + P.blocks[0] + P.blocks[1];
+    GS_REQUIRE(blocks < (1ull << 31), "gs_linear: operands too large for one launch");
+    if (blocks) hipLaunchKernelGGL(k_prepare<T>, dim3((unsigned)blocks), dim3(256), 0, stream, G, P);
     return 0;
 }
 
-// C [M,N] over a contraction of K.  fp32: A times `gate` (row stride ldgate), where there is one, and the sums of A's lines (dW only) to column_join.
+// C [M,N] over a contraction of K; operands that the kernels can read as they are.  fp32: A times `gate` (row stride ldgate), where there is one, and A's sums to db (dW only).
+// columns: sums that are joined beside the product; its `blocks` is set to zero once that is launched.
 template <typename T, bool ACOLS, bool BCOLS>
-int product(Line a, Line b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, void* workspace, int64_t workspace_bytes, hipStream_t stream, const float* gate = nullptr,
-            int64_t ldgate = 0, T* column_join = nullptr) {
+int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, char* ws, int64_t ws_bytes, hipStream_t stream, const float* gate, int64_t ldgate, T* db,
+            Columns<T>& columns) {
     if (M == 0 || N == 0) return 0;
-    const int64_t rows_a = ACOLS ? K : M, rows_b = BCOLS ? K : N;
-    const Plan p = plan(sizeof(T), a, rows_a, b, rows_b, M, N, K, column_join != nullptr);
-    GS_REQUIRE(workspace_bytes >= p.bytes && (workspace || p.bytes == 0), "gs_linear: workspace too small");
-    char* ws = (char*)workspace;
-    const int64_t tiles = gs::cdiv(M, p.tile) * gs::cdiv(N, p.tile);
-    GS_REQUIRE(tiles < (1ll << 31) && M * gs::cdiv(N, 4) < (31ll << 31), "gs_linear: too many tiles");
+    const Plan p = plan(sizeof(T), M, N, K, db != nullptr);
+    GS_REQUIRE(ws_bytes >= p.bytes, "gs_linear: workspace too small");
+    GS_REQUIRE(p.tiles + (int64_t)columns.blocks < (1ll << 31) && M * gs::cdiv(N, 4) < (31ll << 31), "gs_linear: too many tiles");
     Epilogue<T> first = E;
-    first.part = p.splits > 1 ? (float*)(ws + p.at_part) : nullptr;
-    const dim3 grid((unsigned)tiles, (unsigned)p.splits);
+    first.part = p.splits > 1 ? (float*)ws : nullptr;
+    Columns<T> none{}, beside = none;
     if constexpr (sizeof(T) == 4) {
+        const dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
         const Operand<float> A{(const float*)a.p, a.ld}, B{(const float*)b.p, b.ld};
-        float* cols = column_join ? (float*)(ws + p.at_cols) : nullptr;
+        float* cols = db ? (p.splits > 1 ? (float*)(ws + p.at_cols) : db) : nullptr;
         if (gate) hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, true>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
         else hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, false>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
-        if (cols) hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)gs::cdiv(M, 32)), dim3(1024), 0, stream, (const float*)cols, (int)p.splits, M, column_join);
+        if (db && p.splits > 1) beside = Columns<T>{cols, db, M, (int)p.splits, (uint32_t)gs::cdiv(M, 32)};
     } else {
-        int64_t lines_a = M, lines_b = N;
-        if (p.pack_a) {
-            if (const int rc = pack<T>(a.p, a.ld, rows_a, a.cols, ws + p.at_a, p.pack_a, stream)) return rc;
-            a = {ws + p.at_a, p.pack_a, a.cols, true};
-        }
-        if (p.pack_b) {
-            if (const int rc = pack<T>(b.p, b.ld, rows_b, b.cols, ws + p.at_b, p.pack_b, stream)) return rc;
-            b = {ws + p.at_b, p.pack_b, b.cols, true};
-        }
-        if (ACOLS && a.zeros) lines_a = up8(M);
-        if (BCOLS && b.zeros) lines_b = up8(N);
+        const dim3 grid((unsigned)(p.tiles + columns.blocks), (unsigned)p.splits);
+        const int64_t lines_a = ACOLS && a.zeros ? up8(M) : M, lines_b = BCOLS && b.zeros ? up8(N) : N;
         const Operand<T> A{(const T*)a.p, a.ld}, B{(const T*)b.p, b.ld};
-        if (p.tile == 256)
-            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 256, 256, 128, 64, 2>), grid, dim3(512), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
-        else if (p.deep)
-            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64, 4>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
+        if (p.rows == 256)
+            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 256, 256, 128, 64>), grid, dim3(512), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first, columns);
+        else if (!p.deep)
+            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first, columns);
+        else if (p.rows == 128)
+            hipLaunchKernelGGL((k_product16_deep<T, ACOLS, BCOLS, 128>), grid, dim3(512), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first, columns);
         else
-            hipLaunchKernelGGL((k_product16<T, ACOLS, BCOLS, 128, 128, 64, 64, 2>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first);
+            hipLaunchKernelGGL((k_product16_deep<T, ACOLS, BCOLS, 64>), grid, dim3(256), 0, stream, A, B, M, N, lines_a, lines_b, K, p.slice, first, columns);
+        columns.blocks = 0;
     }
     if (p.splits > 1) {
         const int groups = p.splits >= 32 ? 16 : p.splits >= 8 ? 4 : 1;
-        hipLaunchKernelGGL(k_join<T>, dim3((unsigned)gs::cdiv(M * gs::cdiv(N, 4), 256 / groups)), dim3(256), 0, stream, (const float*)(ws + p.at_part), (int)p.splits, groups, M, N, E);
+        const uint32_t blocks = (uint32_t)gs::cdiv(M * gs::cdiv(N, 4), 256 / groups);
+        hipLaunchKernelGGL(k_join<T>, dim3(blocks + beside.blocks), dim3(256), 0, stream, (const float*)ws, (int)p.splits, groups, M, N, E, blocks, beside);
     }
     GS_LAUNCH_CHECK();
     return 0;
 }
 
+static int64_t forward_bytes(int es, const Line& x, const Line& w, int64_t M, int64_t N, int64_t K) {
+    return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, M, N, K, false).bytes;
+}
+
 template <typename T>
 int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, int64_t M, int64_t N, int64_t K, int act,
                float beta, void* y, int64_t ldy, void* dact, void* ws, int64_t ws_bytes, hipStream_t stream) {
+    Line lx{x, ldx, K, false}, lw{w, ldw, K, false};
+    const int64_t need = forward_bytes(sizeof(T), lx, lw, M, N, K);
+    GS_REQUIRE(ws_bytes >= need && (ws || need == 0), "gs_linear_fwd: workspace too small");
+    char* at = (char*)ws;
+    Pack2<T> P{};
+    at += repack<T>(P, 0, lx, M, at);
+    at += repack<T>(P, 1, lw, N, at);
+    if (const int rc = prepare<T>(Gz<T>{}, P, stream)) return rc;
     Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta, act == ACT_SOFTPLUS ? 1.f / beta : 0.f};
-    return product<T, false, false>({x, ldx, K, false}, {w, ldw, K, false}, M, N, K, E, ws, ws_bytes, stream);
+    Columns<T> none{};
+    return product<T, false, false>(lx, lw, M, N, K, E, at, (char*)ws + ws_bytes - at, stream, nullptr, 0, nullptr, none);
 }
 
 struct BackwardPlan {
     bool gz_made, pass, sums_with_w;          // gz has a place of its own; a pass over g is made; db comes with dW
-    int64_t ldgz, slab, slabs;
-    int64_t gz, cols, prod, total;          // byte offsets of gz, the column sums' slabs and the products' workspace
+    int64_t ldgz, slab, slabs, across;
+    int64_t cols, packs, prod, total;          // byte offsets (gz comes first): the column sums' slabs, the repacked operands, the products' workspace
 };
-static BackwardPlan backward_plan(const void* g, int64_t ldg, bool has_dact, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int es,
-                                  bool want_x, bool want_w, bool want_b) {
+static BackwardPlan backward_plan(const Line& g, bool has_dact, const Line& x, const Line& w, int64_t M, int64_t N, int64_t K, int es, bool want_x, bool want_w, bool want_b) {
     BackwardPlan p;
     // fp32 products take the gate as they load g, and the sums with dW; 16-bit ones read gz from memory
-    p.gz_made = es == 2 && (want_x || want_w) && (has_dact || !direct({g, ldg, N, false}));
+    p.gz_made = es == 2 && (want_x || want_w) && (has_dact || !direct(g));
     p.sums_with_w = es == 4 && want_w && want_b && K > 0;
     p.pass = p.gz_made || (want_b && !p.sums_with_w);
-    p.ldgz = p.gz_made ? up8(N) : ldg;
-    const int64_t across = gs::cdiv(N, GZ_LANES * 16 / es);
-    p.slab = gs::cdiv(gs::cdiv(M * across, 2048), GZ_LINES) * GZ_LINES;
+    p.ldgz = p.gz_made ? up8(N) : g.ld;
+    p.across = gs::cdiv(N, GZ_LANES * 16 / es);
+    p.slab = gs::cdiv(gs::cdiv(M * p.across, 2048), GZ_LINES) * GZ_LINES;
     if (p.slab < 64) p.slab = 64;
-    if (M / p.slab >= 65535) p.slab = gs::cdiv(M, 65535);
     p.slabs = gs::cdiv(M, p.slab);
-    p.gz = 0;
-    p.cols = p.gz + (p.gz_made ? align256(M * p.ldgz * es) : 0);
-    p.prod = p.cols + (want_b && !p.sums_with_w ? align256(p.slabs * N * 4) : 0);
-    const Line gl{p.gz_made ? nullptr : g, p.ldgz, N, p.gz_made};
+    p.cols = p.gz_made ? align256(M * p.ldgz * es) : 0;
+    p.packs = p.cols + (p.pass && want_b ? align256(p.slabs * N * 4) : 0);
+    p.prod = p.packs + (want_x ? packed_bytes(es, w, N) : 0) + (want_w ? packed_bytes(es, x, M) : 0);
     int64_t b = 0;
-    if (want_x) b = plan(es, gl, M, {w, ldw, K, false}, N, M, K, N).bytes;
+    if (want_x) b = plan(es, M, K, N, false).bytes;
     if (want_w) {
-        const int64_t c = plan(es, gl, M, {x, ldx, K, false}, M, N, K, M, p.sums_with_w).bytes;
+        const int64_t c = plan(es, N, K, M, p.sums_with_w).bytes;
         if (c > b) b = c;
     }
     p.total = p.prod + b;
@@ -844,31 +972,40 @@ static BackwardPlan backward_plan(const void* g, int64_t ldg, bool has_dact, con
 template <typename T>
 int linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, void* dx,
                void* dw, void* db, void* ws, int64_t ws_bytes, hipStream_t stream) {
-    const BackwardPlan p = backward_plan(g, ldg, dact != nullptr, x, ldx, w, ldw, M, N, K, sizeof(T), dx != nullptr, dw != nullptr, db != nullptr);
+    Line gz{g, ldg, N, false}, lx{x, ldx, K, false}, lw{w, ldw, K, false};
+    const BackwardPlan p = backward_plan(gz, dact != nullptr, lx, lw, M, N, K, sizeof(T), dx != nullptr, dw != nullptr, db != nullptr);
     GS_REQUIRE(ws_bytes >= p.total && (ws || p.total == 0), "gs_linear_bwd: workspace too small");
+    if (N == 0 && K == 0) return 0;
     char* base = (char*)ws;
-    Line gz{p.gz_made ? base + p.gz : g, p.ldgz, N, p.gz_made};
+    Gz<T> G{};
+    Pack2<T> P{};
+    Columns<T> columns{};
     if (N > 0 && p.pass) {
-        float* part = db && !p.sums_with_w ? (float*)(base + p.cols) : nullptr;
-        const int64_t across = gs::cdiv(N, GZ_LANES * width<T>());
-        if (M > 0)
-            hipLaunchKernelGGL(k_gz<T>, dim3((unsigned)across, (unsigned)p.slabs), dim3(256), 0, stream, (const T*)g, ldg, (const typename dact_type<T>::type*)dact, M, N, p.slab,
-                               p.gz_made ? (T*)(base + p.gz) : nullptr, p.ldgz, part);
-        if (db && !p.sums_with_w) hipLaunchKernelGGL(k_column_join<T>, dim3((unsigned)gs::cdiv(N, 32)), dim3(1024), 0, stream, (const float*)part, (int)p.slabs, N, (T*)db);
-        GS_LAUNCH_CHECK();
+        const bool sums = db && !p.sums_with_w;
+        G = Gz<T>{(const T*)g, (const typename dact_type<T>::type*)dact, p.gz_made ? (T*)base : nullptr, sums ? (float*)(base + p.cols) : nullptr, ldg, p.ldgz, M, N, p.slab,
+                  (uint32_t)p.across, (uint32_t)(p.across * p.slabs)};
+        GS_REQUIRE(p.across * p.slabs < (1ll << 31), "gs_linear_bwd: gradient too large for one launch");
+        if (sums) columns = Columns<T>{(const float*)(base + p.cols), (T*)db, N, (int)p.slabs, (uint32_t)gs::cdiv(N, 32)};
+        if (p.gz_made) gz = {base, p.ldgz, N, true};
     }
+    int64_t at = p.packs;
+    if (dx) at += repack<T>(P, 0, lw, N, base + at);
+    if (dw) at += repack<T>(P, 1, lx, M, base + at);
+    if (const int rc = prepare<T>(G, P, stream)) return rc;
     Epilogue<T> E{};
     const float* gate = sizeof(T) == 4 ? (const float*)dact : nullptr;
-    int rc = 0;
+    E.ldo = K;
     if (dx) {
-        E.out = (T*)dx, E.ldo = K;
-        rc = product<T, false, true>(gz, {w, ldw, K, false}, M, K, N, E, base + p.prod, ws_bytes - p.prod, stream, gate, N);
+        E.out = (T*)dx;
+        if (const int rc = product<T, false, true>(gz, lw, M, K, N, E, base + p.prod, ws_bytes - p.prod, stream, gate, N, nullptr, columns)) return rc;
     }
-    if (!rc && dw) {
-        E.out = (T*)dw, E.ldo = K;
-        rc = product<T, true, true>(gz, {x, ldx, K, false}, N, K, M, E, base + p.prod, ws_bytes - p.prod, stream, gate, N, p.sums_with_w ? (T*)db : nullptr);
+    if (dw) {
+        E.out = (T*)dw;
+        if (const int rc = product<T, true, true>(gz, lx, N, K, M, E, base + p.prod, ws_bytes - p.prod, stream, gate, N, p.sums_with_w ? (T*)db : nullptr, columns)) return rc;
     }
-    return rc;
+    if (columns.blocks) hipLaunchKernelGGL(k_join_columns<T>, dim3(columns.blocks), dim3(1024), 0, stream, columns);          // no 16-bit product was there to do it beside
+    GS_LAUNCH_CHECK();
+    return 0;
 }
 
 // 16-bit tiles are addressed by 31-bit offsets: 256 rows of 2^21 elements fit
@@ -881,7 +1018,7 @@ static bool sizes_ok(int64_t M, int64_t N, int64_t K, int dtype) {
 
 extern "C" int64_t gs_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K, int dtype) {
     if (dtype < 0 || dtype > 2 || !sizes_ok(M, N, K, dtype)) return -1;
-    return M == 0 || N == 0 ? 0 : plan(dtype == DT_F32 ? 4 : 2, {x, ldx, K, false}, M, {weight, ldw, K, false}, N, M, N, K).bytes;
+    return M == 0 || N == 0 ? 0 : forward_bytes(dtype == DT_F32 ? 4 : 2, {x, ldx, K, false}, {weight, ldw, K, false}, M, N, K);
 }
 
 extern "C" int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, const void* residual, int64_t ldr, int64_t M, int64_t N,
@@ -900,7 +1037,7 @@ extern "C" int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int
 extern "C" int64_t gs_linear_bwd_workspace_bytes(const void* g, int64_t ldg, int has_dact, const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N,
                                                  int64_t K, int dtype, int want_x, int want_w, int want_b) {
     if (dtype < 0 || dtype > 2 || !sizes_ok(M, N, K, dtype)) return -1;
-    return backward_plan(g, ldg, has_dact, x, ldx, weight, ldw, M, N, K, dtype == DT_F32 ? 4 : 2, want_x, want_w, want_b).total;
+    return backward_plan({g, ldg, N, false}, has_dact, {x, ldx, K, false}, {weight, ldw, K, false}, M, N, K, dtype == DT_F32 ? 4 : 2, want_x, want_w, want_b).total;
 }
 
 extern "C" int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K,
