@@ -712,6 +712,97 @@ __global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand
 #endif
 }
 
+// ---- few rows -------------------------------------------------------------------------------------------------------------------------------------------
+// y for at most 32 rows of x (serving): bound by the weight's bytes and by latency.  A workgroup takes 16 NT rows of W, its 8 waves share the contraction out in stretches of
+// CHUNK, and fragments come straight from memory: each matrix instruction takes 16 bytes a lane of 16 rows of W, so W is read once, with nothing staged, and the loads of the
+// next stretch are on their way while one is multiplied.  16-bit: one instruction a load; fp32: the fp32 matrix instruction four times (its rate does not matter here, and it
+// rounds like a chain of fused multiply-adds).  The waves' sums meet in LDS.
+constexpr int ROWS_THREADS = 512, ROWS_WAVES = ROWS_THREADS / 64;
+template <typename T, int MT, int NT>
+__global__ void __launch_bounds__(ROWS_THREADS) k_rows(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<T> E) {
+    constexpr int V = width<T>(), PER = 4 * V, U = MT * NT == 1 ? 8 : 4, CHUNK = PER * U;          // PER of the contraction a load
+    typedef Pack<T, V> Vec;
+    __shared__ float sums[ROWS_WAVES][MT * NT][16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = (lane >> 4) * V;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+    const int64_t c_begin = (int64_t)blockIdx.y * slice, c_end = c_begin + slice < K ? c_begin + slice : K;
+    // lines beyond the end repeat the last one; nobody stores what comes of them
+    const T* line[NT + MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int64_t n = n0 + t * 16 + (lane & 15);
+        line[t] = w + (n < N ? n : N - 1) * ldw + at;
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t m = t * 16 + (lane & 15);
+        line[NT + t] = x + (m < M ? m : M - 1) * ldx + at;
+    }
+    struct Chunk { Vec v[NT + MT][U]; };
+    const auto fetch = [&](int64_t c, Chunk& q) __attribute__((always_inline)) {
+        if (c + CHUNK <= c_end) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < NT + MT; ++t) q.v[t][u] = *(const Vec*)(line[t] + c + u * PER);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < NT + MT; ++t)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) q.v[t][u].v[e] = c + u * PER + at + e < c_end ? line[t][c + u * PER + e] : (T)0.f;
+        }
+    };
+    f32x4 acc[NT][MT] = {};
+    const auto multiply = [&](const Chunk& q) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const Vec &a = q.v[n][u], &b = q.v[NT + m][u];
+                    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc[n][m], 0, 0, 0);
+                    } else {
+                        acc[n][m] = mfma<T>(__builtin_bit_cast(s16x8, a), __builtin_bit_cast(s16x8, b), acc[n][m]);
+                    }
+                }
+    };
+    constexpr int64_t ROUND = ROWS_WAVES * CHUNK;
+    int64_t c = c_begin + wave * CHUNK;
+    Chunk p, q;
+    if (c < c_end) fetch(c, p);
+    for (; c < c_end; c += 2 * ROUND) {
+        if (c + ROUND < c_end) fetch(c + ROUND, q);
+        multiply(p);
+        if (c + ROUND >= c_end) break;
+        if (c + 2 * ROUND < c_end) fetch(c + 2 * ROUND, p);
+        multiply(q);
+    }
+    // a lane holds 4 neighbouring columns (rows of W) of one row of x
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[wave][n * MT + m][lane & 15][(lane >> 4) * 4 + e] = acc[n][m][e];
+    __syncthreads();
+    for (int k = threadIdx.x; k < MT * NT * 256; k += ROWS_THREADS) {
+        const int n = k / (MT * 256), m16 = k / 16 % (16 * MT);
+        const int64_t m = m16, j = n0 + n * 16 + (k & 15);
+        if (m >= M || j >= N) continue;
+        float z[1][1] = {{0.f}};
+#pragma unroll
+        for (int s = 0; s < ROWS_WAVES; ++s) z[0][0] += sums[s][n * MT + (m16 >> 4)][m16 & 15][k & 15];
+        const int64_t row[1] = {m};
+        if (E.part) E.part[((int64_t)blockIdx.y * M + m) * N + j] = z[0][0];
+        else finish<T, 1, 1>(E, row, j, M, N, z);
+    }
+}
+
 // The slices of a contraction joined, then the epilogue.  `groups` lanes of a workgroup share the slices of four outputs in equal stretches, in their order.
 template <typename T> __global__ void __launch_bounds__(256) k_join(const float* part, int splits, int groups, int64_t M, int64_t N, Epilogue<T> E, uint32_t blocks, Columns<T> C) {
     constexpr int V = 4;
@@ -829,21 +920,29 @@ static Plan plan(int es, int64_t M, int64_t N, int64_t K, bool column_sums) {
     Plan p;
     const auto tiles = [&](int64_t r, int64_t c) { return gs::cdiv(M, r) * gs::cdiv(N, c); };
     p.tiles = tiles(TILE, TILE);
-    int64_t slots = 2 * CUS, least = 256;
-    if (es == 2) {
-        if (tiles(256, 256) >= 192) {
-            p.rows = p.cols = 256, slots = CUS;
-        } else if (p.tiles <= CUS) {
-            p.deep = true, slots = CUS, least = 512;
-            if (tiles(64, TILE) <= CUS) p.rows = 64;
+    if (es == 2 && tiles(256, 256) >= 192) p.rows = p.cols = 256, p.tiles = tiles(256, 256);
+    if (es == 2 && p.rows == TILE && p.tiles <= CUS) {
+        // Tiles that do not fill the chip: rows of a tile and slices of the contraction by what they cost.  Measured: 0.5 us a step for 128 rows (2048 x 2048 x 2048:
+        // 23 us), 0.37 us for 64 (512 x 4096 x 4096: 28 us), 4 us for a second launch that reads and writes the slices' sums at 4 TB/s.
+        p.deep = true;
+        const int64_t steps = gs::cdiv(K, 64);
+        double best = 1e30;
+        for (int r = 64; r <= TILE; r += 64) {
+            const int64_t t = tiles(r, TILE);
+            for (int64_t s = 1; s == 1 || (t * s <= CUS && s * 4 <= steps); s *= 2) {
+                if (t > CUS) break;
+                const double cost = gs::cdiv(steps, s) * (r == 64 ? 0.37 : 0.5) + (s > 1 ? 4.0 + 2.0 * s * M * N * 4 / 4e6 : 0.0);
+                if (cost < best) best = cost, p.rows = r, p.splits = s, p.tiles = t;
+            }
         }
-        p.tiles = tiles(p.rows, p.cols);
-    }
-    if (p.tiles < slots && K >= 2 * least) {
-        p.splits = slots / p.tiles;
-        if (p.splits > K / least) p.splits = K / least;
-        if (p.splits > 256) p.splits = 256;
-        if (p.splits < 1) p.splits = 1;
+    } else {
+        const int64_t slots = p.rows == 256 ? CUS : 2 * CUS;
+        if (p.tiles < slots && K >= 512) {
+            p.splits = slots / p.tiles;
+            if (p.splits > K / 256) p.splits = K / 256;
+            if (p.splits > 256) p.splits = 256;
+            if (p.splits < 1) p.splits = 1;
+        }
     }
     p.slice = p.splits > 1 ? gs::cdiv(gs::cdiv(K, p.splits), 64) * 64 : K;
     p.splits = p.splits > 1 ? gs::cdiv(K, p.slice) : 1;
@@ -878,6 +977,10 @@ template <typename T> int prepare(const Gz<T>& G, const Pack2<T>& P, hipStream_t
     return 0;
 }
 
+static unsigned join_blocks(int64_t M, int64_t N, int64_t splits, int& groups) {
+    groups = splits >= 32 ? 16 : splits >= 8 ? 4 : 1;
+    return (unsigned)gs::cdiv(M * gs::cdiv(N, 4), 256 / groups);
+}
 // C [M,N] over a contraction of K; operands that the kernels can read as they are.  fp32: A times `gate` (row stride ldgate), where there is one, and A's sums to db (dW only).
 // columns: sums that are joined beside the product; its `blocks` is set to zero once that is launched.
 template <typename T, bool ACOLS, bool BCOLS>
@@ -912,15 +1015,48 @@ int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilo
         columns.blocks = 0;
     }
     if (p.splits > 1) {
-        const int groups = p.splits >= 32 ? 16 : p.splits >= 8 ? 4 : 1;
-        const uint32_t blocks = (uint32_t)gs::cdiv(M * gs::cdiv(N, 4), 256 / groups);
+        int groups;
+        const uint32_t blocks = join_blocks(M, N, p.splits, groups);
         hipLaunchKernelGGL(k_join<T>, dim3(blocks + beside.blocks), dim3(256), 0, stream, (const float*)ws, (int)p.splits, groups, M, N, E, blocks, beside);
     }
     GS_LAUNCH_CHECK();
     return 0;
 }
 
+// k_rows: at most 32 rows, and where its workgroups of 16 columns do not fill the chip slices of the contraction, each of one round of the waves or more
+constexpr int64_t FEW_ROWS = 32;
+static Plan rows_plan(int64_t M, int64_t N, int64_t K) {
+    Plan p;
+    p.cols = gs::cdiv(N, 32) >= CUS ? 32 : 16;          // x is read by every workgroup: twice the columns where that leaves a workgroup for each compute unit
+    p.tiles = gs::cdiv(N, p.cols);
+    if (p.tiles < CUS / 2 && K >= 4096) {
+        p.splits = CUS / p.tiles < K / 2048 ? CUS / p.tiles : K / 2048;
+        p.slice = gs::cdiv(gs::cdiv(K, p.splits), 1024) * 1024;
+        p.splits = gs::cdiv(K, p.slice);
+    }
+    if (p.splits == 1) p.slice = K;
+    p.bytes = p.splits > 1 ? align256(p.splits * M * N * 4) : 0;
+    return p;
+}
+template <typename T>
+int product_rows(const Line& x, const Line& w, int64_t M, int64_t N, int64_t K, Epilogue<T> E, char* ws, hipStream_t stream) {
+    const Plan p = rows_plan(M, N, K);
+    Epilogue<T> first = E;
+    first.part = p.splits > 1 ? (float*)ws : nullptr;
+    const dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
+    const auto kernel = p.cols == 32 ? (M <= 16 ? k_rows<T, 1, 2> : k_rows<T, 2, 2>) : (M <= 16 ? k_rows<T, 1, 1> : k_rows<T, 2, 1>);
+    hipLaunchKernelGGL(kernel, grid, dim3(ROWS_THREADS), 0, stream, (const T*)x.p, x.ld, (const T*)w.p, w.ld, M, N, K, p.slice, first);
+    if (p.splits > 1) {
+        int groups;
+        const unsigned blocks = join_blocks(M, N, p.splits, groups);
+        hipLaunchKernelGGL(k_join<T>, dim3(blocks), dim3(256), 0, stream, (const float*)ws, (int)p.splits, groups, M, N, E, blocks, Columns<T>{});
+    }
+    GS_LAUNCH_CHECK();
+    return 0;
+}
+
 static int64_t forward_bytes(int es, const Line& x, const Line& w, int64_t M, int64_t N, int64_t K) {
+    if (M <= FEW_ROWS) return rows_plan(M, N, K).bytes;
     return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, M, N, K, false).bytes;
 }
 
@@ -931,11 +1067,12 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
     const int64_t need = forward_bytes(sizeof(T), lx, lw, M, N, K);
     GS_REQUIRE(ws_bytes >= need && (ws || need == 0), "gs_linear_fwd: workspace too small");
     char* at = (char*)ws;
+    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta, act == ACT_SOFTPLUS ? 1.f / beta : 0.f};
+    if (M <= FEW_ROWS) return product_rows<T>(lx, lw, M, N, K, E, at, stream);
     Pack2<T> P{};
     at += repack<T>(P, 0, lx, M, at);
     at += repack<T>(P, 1, lw, N, at);
     if (const int rc = prepare<T>(Gz<T>{}, P, stream)) return rc;
-    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta, act == ACT_SOFTPLUS ? 1.f / beta : 0.f};
     Columns<T> none{};
     return product<T, false, false>(lx, lw, M, N, K, E, at, (char*)ws + ws_bytes - at, stream, nullptr, 0, nullptr, none);
 }
