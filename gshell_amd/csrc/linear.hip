@@ -57,31 +57,35 @@ template <bool FAST> __device__ __forceinline__ void act_relu(float z, float& y,
     y = z < 0.f ? 0.f : z;
     d = z <= 0.f ? 0.f : 1.f;
 }
+// With t = exp(-|beta z|) in [0, 1] (neither end of z overflows): log(1 + t) = 2 artanh(t / (2 + t)) by its series -- the argument is at most 1/3, and the term
+// after the last one below 2e-8 of the sum -- and one reciprocal of (1 + t)(2 + t) serves that and the derivative.
 template <bool FAST> __device__ __forceinline__ void act_softplus(float beta, float inv_beta, float z, float& y, float& d) {
-    const float t = exp_<FAST>(-fabsf(beta * z));          // in [0, 1]: neither end of z overflows
-    // log(1 + t) from the logarithm of the rounded 1 + t, put right by the ratio of t to what was added in fact
-    const float u = 1.f + t, added = u - 1.f;
-    const float l = added == 0.f ? t : __builtin_amdgcn_logf(u) * 0.69314718f * t * rcp_(added);
-    y = (z < 0.f ? 0.f : z) + l * inv_beta;
-    d = (z >= 0.f ? 1.f : t) * rcp_(1.f + t);
+    const float t = exp_<FAST>(-fabsf(beta * z));
+    const float u = 1.f + t, v = 2.f + t, r = rcp_(u * v), q = t * (r * u), w = q * q;
+    float s = 0.07692308f;
+    for (const float c : {0.09090909f, 0.11111111f, 0.14285714f, 0.2f, 0.33333333f, 1.f}) s = fmaf(s, w, c);
+    y = (z < 0.f ? 0.f : z) + 2.f * q * s * inv_beta;
+    d = (z >= 0.f ? 1.f : t) * (r * v);
 }
 template <bool FAST> __device__ __forceinline__ void act_silu(float z, float& y, float& d) {
     const float s = rcp_(1.f + exp_<FAST>(-z));
     y = z * s;
-    d = s * (1.f + z * (1.f - s));
+    d = s * fmaf(z, 1.f - s, 1.f);
 }
 template <bool FAST> __device__ __forceinline__ void act_gelu(float z, float& y, float& d) {
     const float e = exp_<FAST>(-0.5f * z * z);
     float phi;
     if (FAST) {
-        const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
-        const float c = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float t = rcp_(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+        float c = 1.061405429f;
+        for (const float k : {-1.453152027f, 1.421413741f, -0.284496736f, 0.254829592f}) c = fmaf(c, t, k);
+        c *= 0.5f * e * t;
         phi = z < 0.f ? c : 1.f - c;
     } else {
         phi = 0.5f * erfcf(z * -0.70710678118654752f);
     }
     y = z * phi;
-    d = phi + z * (e * 0.39894228040143268f);
+    d = fmaf(z, e * 0.39894228040143268f, phi);
 }
 // BATCH x V values at once: the choice is the same for the whole launch
 template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, float beta, float inv_beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
@@ -281,13 +285,13 @@ template <typename T> __device__ __forceinline__ void join_columns(const Columns
 }
 
 // ---- fp32 products ------------------------------------------------------------------------------------------------------------------------------------
-// Tiles of 128 x 128, 32 of the contraction a step, two workgroups a compute unit.  While a step is multiplied the next one comes
-// to registers and is split there; each of the three parts has a plane of its own in LDS: [line][32], 4 pieces of 16 bytes a line, piece p of line l at p ^ (l >> 1 & 3), so that the 16
-// lines of a fragment fall on distinct banks.  96 matrix instructions a wave and step stand against 24 fragments read and 32 values split a lane.
-//   rows operand     a lane loads 8 neighbours of the contraction; columns operand: 16 of one line, neighbouring lanes neighbouring lines
+// Tiles of LINES x LINES, 32 of the contraction a step.  128: two workgroups a compute unit, a wave multiplies 64 x 64 (96 matrix instructions a step against 24 fragments read and
+// 32 values split a lane); 64: up to four, a wave 32 x 32, for products that have few tiles.  While a step is multiplied the next one comes to registers and is split there; each
+// of the three parts has a plane of its own in LDS: [line][32], 4 pieces of 16 bytes a line, piece p of line l at p ^ (l >> 1 & 3), so that the 16 lines of a fragment
+// fall on distinct banks.
+//   rows operand     a lane loads 8 neighbours of the contraction at a time; columns operand: 16 or 8 of one line, neighbouring lanes neighbouring lines
 // A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
 constexpr int TILE = 128, BK = 32;
-constexpr int PLANE = TILE * BK;
 
 __device__ __forceinline__ short raw(bf16 v) { return __builtin_bit_cast(short, v); }
 __device__ __forceinline__ short raw(f16 v) { return __builtin_bit_cast(short, v); }
@@ -308,40 +312,45 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t (&part)[3]) {
 }
 __device__ __forceinline__ int piece_at(int line, int at) { return line * BK + (((at >> 3) ^ ((line >> 1) & 3)) * 8) + (at & 7); }
 
-template <bool COLS, bool GATE> struct Feed32 {
+template <bool COLS, bool GATE, int LINES> struct Feed32 {
+    static constexpr int THREADS = 256, PIECES = LINES * BK / THREADS / 8;          // of 8 neighbours, a lane and step
+    static constexpr int PLANE = LINES * BK;
     const float *p, *gate;
     int64_t ld, ldgate, line0, lines, c_end;
     bool whole;                    // every line of the tile is in the operand
-    // what is in flight: rows operands 2 pieces of 8 neighbours, of lines 64 apart; columns operands 16 neighbours of one line
-    struct Values { float v[16], d[GATE ? 16 : 1]; };
+    struct Values { float v[8 * PIECES], d[GATE ? 8 * PIECES : 1]; };          // in flight
+    struct Parts { u32x4 p[3][PIECES]; };
+    // the line and the first index of the lane's piece `h`
+    static __device__ __forceinline__ int line_of(int h) { return COLS ? threadIdx.x % LINES : h * (THREADS / 4) + (threadIdx.x >> 2); }
+    static __device__ __forceinline__ int at_of(int h) { return COLS ? (threadIdx.x / LINES * PIECES + h) * 8 : (threadIdx.x & 3) * 8; }
     __device__ __forceinline__ void fetch(int64_t c, Values& V) const {
         const bool all = whole && c + BK <= c_end;
         if constexpr (!COLS) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int64_t l = line0 + j * 64 + (threadIdx.x >> 2), at = c + (threadIdx.x & 3) * 8;
+            for (int h = 0; h < PIECES; ++h) {
+                const int64_t l = line0 + line_of(h), at = c + at_of(h);
                 const int64_t left = all ? 8 : l < lines ? c_end - at : 0;
 #pragma unroll
-                for (int h = 0; h < 8; h += 4) {
-                    load_some<float, 4>(p + l * ld + at + h, left - h, *(float(*)[4])(V.v + 8 * j + h));
-                    if constexpr (GATE) load_some<float, 4>(gate + l * ldgate + at + h, left - h, *(float(*)[4])(V.d + 8 * j + h));
+                for (int k = 0; k < 8; k += 4) {
+                    load_some<float, 4>(p + l * ld + at + k, left - k, *(float(*)[4])(V.v + 8 * h + k));
+                    if constexpr (GATE) load_some<float, 4>(gate + l * ldgate + at + k, left - k, *(float(*)[4])(V.d + 8 * h + k));
                 }
             }
         } else {
-            const int64_t at = c + (__builtin_amdgcn_readfirstlane(threadIdx.x >> 7)) * 16;          // the same for a wave
-            const uint32_t l = threadIdx.x & 127;
+            const int64_t at = c + __builtin_amdgcn_readfirstlane(at_of(0));          // the same for a wave
+            const uint32_t l = threadIdx.x % LINES;
             const float* q = p + at * ld + line0;
             const float* e = GATE ? gate + at * ldgate + line0 : nullptr;
             if (all) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
+                for (int k = 0; k < 8 * PIECES; ++k) {
                     V.v[k] = q[l];
                     q += ld;
                     if constexpr (GATE) V.d[k] = e[l], e += ldgate;
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
+                for (int k = 0; k < 8 * PIECES; ++k) {
                     const bool ok = line0 + l < lines && at + k < c_end;
                     V.v[k] = ok ? q[l] : 0.f;
                     q += ld;
@@ -350,58 +359,58 @@ template <bool COLS, bool GATE> struct Feed32 {
             }
         }
     }
-    struct Parts { uint32_t p[3][8]; };          // two neighbours a register
     // split; returns the sum of the values (of one line, for columns operands)
-    __device__ __forceinline__ float split(Values& V, Parts& S) const {
+    __device__ __forceinline__ float split(const Values& V, Parts& S) const {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float x = V.v[2 * k], y = V.v[2 * k + 1];
-            if constexpr (GATE) x *= V.d[2 * k], y *= V.d[2 * k + 1];
-            if constexpr (COLS) t += x + y;
-            uint32_t part[3];
-            split2(x, y, part);
+        for (int h = 0; h < PIECES; ++h)
 #pragma unroll
-            for (int q = 0; q < 3; ++q) S.p[q][k] = part[q];
-        }
+            for (int k = 0; k < 4; ++k) {
+                float x = V.v[8 * h + 2 * k], y = V.v[8 * h + 2 * k + 1];
+                if constexpr (GATE) x *= V.d[8 * h + 2 * k], y *= V.d[8 * h + 2 * k + 1];
+                if constexpr (COLS) t += x + y;
+                uint32_t part[3];
+                split2(x, y, part);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) S.p[q][h][k] = part[q];
+            }
         return t;
     }
     __device__ __forceinline__ void store(short* lds, const Parts& S) const {
 #pragma unroll
-        for (int q = 0; q < 3; ++q) {
+        for (int q = 0; q < 3; ++q)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int line = COLS ? threadIdx.x & 127 : h * 64 + (threadIdx.x >> 2), at = COLS ? (threadIdx.x >> 7) * 16 + 8 * h : (threadIdx.x & 3) * 8;
-                *(u32x4*)(lds + q * PLANE + piece_at(line, at)) = u32x4{S.p[q][4 * h], S.p[q][4 * h + 1], S.p[q][4 * h + 2], S.p[q][4 * h + 3]};
-            }
-        }
+            for (int h = 0; h < PIECES; ++h) *(u32x4*)(lds + q * PLANE + piece_at(line_of(h), at_of(h))) = S.p[q][h];
     }
 };
 
-template <bool ACOLS, bool BCOLS, bool GATE>
-__global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<float> E,
-                                                      float* column_sums /* [slices][M], or db itself where there is one slice */) {
+template <bool ACOLS, bool BCOLS, bool GATE, int LINES>
+__global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice,
+                                                                       Epilogue<float> E, float* column_sums /* [slices][M], or db itself where there is one slice */) {
+    constexpr int F = LINES / 32, PLANE = LINES * BK;          // fragments of a wave, either way
     __shared__ __attribute__((aligned(16))) union {
         struct { short a[3 * PLANE], b[3 * PLANE]; } in;
-        float out[4 * 64 * 64];
+        float out[LINES * LINES];
     } lds;
     uint32_t ti, tj;
-    tile_of(blockIdx.x, (uint32_t)((M + TILE - 1) / TILE), (uint32_t)((N + TILE - 1) / TILE), ti, tj);
-    const int64_t i0 = (int64_t)ti * TILE, j0 = (int64_t)tj * TILE;
+    tile_of(blockIdx.x, (uint32_t)((M + LINES - 1) / LINES), (uint32_t)((N + LINES - 1) / LINES), ti, tj);
+    const int64_t i0 = (int64_t)ti * LINES, j0 = (int64_t)tj * LINES;
     const int64_t c_begin = (int64_t)blockIdx.y * slice, c_end = c_begin + slice < K ? c_begin + slice : K;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
-    Feed32<ACOLS, GATE> fa;
-    Feed32<BCOLS, false> fb;
-    fa.p = A.p, fa.ld = A.ld, fa.gate = gate, fa.ldgate = ldgate, fa.line0 = i0, fa.lines = M, fa.c_end = c_end, fa.whole = i0 + TILE <= M;
-    fb.p = B.p, fb.ld = B.ld, fb.line0 = j0, fb.lines = N, fb.c_end = c_end, fb.whole = j0 + TILE <= N;
+    const int wi = (wave >> 1) * (LINES / 2), wj = (wave & 1) * (LINES / 2);
+    typedef Feed32<ACOLS, GATE, LINES> FA;
+    typedef Feed32<BCOLS, false, LINES> FB;
+    FA fa;
+    FB fb;
+    fa.p = A.p, fa.ld = A.ld, fa.gate = gate, fa.ldgate = ldgate, fa.line0 = i0, fa.lines = M, fa.c_end = c_end, fa.whole = i0 + LINES <= M;
+    fb.p = B.p, fb.ld = B.ld, fb.line0 = j0, fb.lines = N, fb.c_end = c_end, fb.whole = j0 + LINES <= N;
     const bool sums = ACOLS && column_sums && tj == 0;
     float total = 0.f;
-    f32x4 acc[4][4] = {};
-    typename Feed32<ACOLS, GATE>::Values ra;
-    typename Feed32<BCOLS, false>::Values rb;
-    typename Feed32<ACOLS, GATE>::Parts sa;
-    typename Feed32<BCOLS, false>::Parts sb;
+    f32x4 acc[F][F] = {};
+    typename FA::Values ra;
+    typename FB::Values rb;
+    typename FA::Parts sa;
+    typename FB::Parts sb;
     if (c_begin < c_end) {
         fa.fetch(c_begin, ra);
         fb.fetch(c_begin, rb);
@@ -416,13 +425,13 @@ __global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const fl
         // behind the end every value is outside and comes as zero
         fa.fetch(c + BK, ra);
         fb.fetch(c + BK, rb);
-        s16x8 vb[3][4];
+        s16x8 vb[3][F];
 #pragma unroll
         for (int q = 0; q < 3; ++q)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) vb[q][w] = *(const s16x8*)(lds.in.b + q * PLANE + piece_at(wj + w * 16 + (lane & 15), (lane >> 4) * 8));
+            for (int w = 0; w < F; ++w) vb[q][w] = *(const s16x8*)(lds.in.b + q * PLANE + piece_at(wj + w * 16 + (lane & 15), (lane >> 4) * 8));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < F; ++u) {
             s16x8 va[3];
 #pragma unroll
             for (int q = 0; q < 3; ++q) va[q] = *(const s16x8*)(lds.in.a + q * PLANE + piece_at(wi + u * 16 + (lane & 15), (lane >> 4) * 8));
@@ -431,31 +440,36 @@ __global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const fl
             for (int term = 0; term < 6; ++term) {
                 constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0};
 #pragma unroll
-                for (int w = 0; w < 4; ++w) acc[u][w] = mfma<bf16>(vb[PB[term]][w], va[PA[term]], acc[u][w]);
+                for (int w = 0; w < F; ++w) acc[u][w] = mfma<bf16>(vb[PB[term]][w], va[PA[term]], acc[u][w]);
             }
         }
-        // the next step is split in the shadow of the second half of the products
+        // the next step is split among the second half of the products
         total += fa.split(ra, sa);
         fb.split(rb, sb);
 #pragma unroll
-        for (int k = 0; k < 48; ++k) {
+        for (int k = 0; k < 3 * F * F; ++k) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         }
 #pragma unroll
-        for (int k = 0; k < 48; ++k) {
+        for (int k = 0; k < 3 * F * F; ++k) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 16 / F, 0);
         }
     }
     __syncthreads();
-    if (sums) {          // two lanes hold the halves of a line's sum
+    if (sums) {          // 256 / LINES lanes hold parts of a line's sum
         lds.out[threadIdx.x] = total;
         __syncthreads();
-        if (threadIdx.x < TILE && i0 + threadIdx.x < M) column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = lds.out[threadIdx.x] + lds.out[threadIdx.x + TILE];
+        if (threadIdx.x < LINES && i0 + threadIdx.x < M) {
+            float t = 0.f;
+#pragma unroll
+            for (int q = 0; q < 256 / LINES; ++q) t += lds.out[threadIdx.x + q * LINES];
+            column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = t;
+        }
         __syncthreads();
     }
-    store_wave<float, 4, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, [&](int64_t i, int64_t j, auto& z) {
+    const auto fix = [&](int64_t i, int64_t j, auto& z) {
         // a sum that is not finite is done again without the split, in fp32
 #pragma unroll 1
         for (int k = 0; k < 4; ++k)
@@ -468,7 +482,17 @@ __global__ void __launch_bounds__(256, 2) k_product32(Operand<float> A, const fl
                 }
                 z[k] = t;
             }
-    });
+    };
+    if constexpr (LINES == 128) {
+        store_wave<float, 4, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, fix);
+    } else {          // the four waves' sums side by side, then 16 lines each
+#pragma unroll
+        for (int u = 0; u < F; ++u)
+#pragma unroll
+            for (int w = 0; w < F; ++w) *(f32x4*)(lds.out + piece_of_sums(wi + u * 16 + (lane & 15), wj / 4 + w * 4 + (lane >> 4))) = acc[u][w];
+        __syncthreads();
+        drain_sums<float, 4>(E, lds.out, wave * 16, wave * 16 + 16, i0, j0, M, N, fix);
+    }
 }
 
 // ---- 16-bit products with tiles fed straight into LDS ---------------------------------------------------------------------------------------------------
@@ -916,32 +940,48 @@ struct Plan {
     int64_t tiles = 0, splits = 1, slice = 0;
     int64_t at_cols = 0, bytes = 0;          // the slices' sums come first, then their column sums
 };
-static Plan plan(int es, int64_t M, int64_t N, int64_t K, bool column_sums) {
+static Plan plan(int es, int columns /* operands that come by columns */, int64_t M, int64_t N, int64_t K, bool column_sums) {
     Plan p;
+    if (M == 0 || N == 0) return p;
     const auto tiles = [&](int64_t r, int64_t c) { return gs::cdiv(M, r) * gs::cdiv(N, c); };
-    p.tiles = tiles(TILE, TILE);
-    if (es == 2 && tiles(256, 256) >= 192) p.rows = p.cols = 256, p.tiles = tiles(256, 256);
-    if (es == 2 && p.rows == TILE && p.tiles <= CUS) {
-        // Tiles that do not fill the chip: rows of a tile and slices of the contraction by what they cost.  Measured: 0.5 us a step for 128 rows (2048 x 2048 x 2048:
-        // 23 us), 0.37 us for 64 (512 x 4096 x 4096: 28 us), 4 us for a second launch that reads and writes the slices' sums at 4 TB/s.
-        p.deep = true;
-        const int64_t steps = gs::cdiv(K, 64);
-        double best = 1e30;
+    // Tiles and slices by what they cost: rounds of the chip x (steps x us a step + the start and the end of a workgroup), and for slices a second launch that reads and
+    // writes their sums at 4 TB/s.  The us a step are measured, for one, two and four workgroups on a compute unit.
+    const auto join = [&](int64_t s) { return s > 1 ? 4.0 + 2.0 * s * M * N * 4 / 4e6 : 0.0; };
+    double best = 1e30;
+    const auto take = [&](int rows, int cols, int64_t t, int64_t s, double cost, bool deep) {
+        if (cost < best) best = cost, p.rows = rows, p.cols = cols, p.tiles = t, p.splits = s, p.deep = deep;
+    };
+    if (es == 4) {
+        // 128: 2.8 us a step with two a unit, 2.2 with one, 64: 1.4 with four, 1.1 with two, 0.85 with one -- times 1.2 where one operand comes a column at a time (dx), 1.5 where both do
+        // (dW).  131072 x 256 x 256: tiles of 128 / 64 130 / 134 us for y, 149 / 174 for dx, 125 / 208 for dW; 50000 x 256 x 295: 93 / 73 for y.
+        const int64_t steps = gs::cdiv(K, BK);
+        const double slow = columns == 0 ? 1.05 : columns == 1 ? 1.2 : 1.5;
         for (int r = 64; r <= TILE; r += 64) {
-            const int64_t t = tiles(r, TILE);
-            for (int64_t s = 1; s == 1 || (t * s <= CUS && s * 4 <= steps); s *= 2) {
-                if (t > CUS) break;
-                const double cost = gs::cdiv(steps, s) * (r == 64 ? 0.37 : 0.5) + (s > 1 ? 4.0 + 2.0 * s * M * N * 4 / 4e6 : 0.0);
-                if (cost < best) best = cost, p.rows = r, p.splits = s, p.tiles = t;
+            const int64_t t = tiles(r, r), most = r == 64 ? 4 : 2;
+            for (int64_t a_unit = 0; a_unit <= most; a_unit = a_unit ? 2 * a_unit : 1) {
+                int64_t s = a_unit ? a_unit * CUS / t : 1;          // as many slices as fill the chip with a_unit workgroups each, or one
+                if (a_unit && s > steps / 8) s = steps / 8;
+                if (s < 1 || s > 256) continue;
+                const int64_t wg = t * s, on = gs::cdiv(wg, CUS) < most ? gs::cdiv(wg, CUS) : most;
+                const double us = r == 64 ? (on == 1 ? 0.85 : on == 2 ? 1.1 : 1.4) * slow : (on == 1 ? 2.2 : 2.8);
+                take(r, r, t, s, gs::cdiv(wg, most * CUS) * (gs::cdiv(steps, s) * us + (r == 64 ? 5.0 : 12.0)) + join(s), false);
             }
         }
+    } else if (tiles(256, 256) >= 192) {
+        p.rows = p.cols = 256, p.tiles = tiles(256, 256);
+    } else if (tiles(TILE, TILE) > CUS) {
+        p.tiles = tiles(TILE, TILE);
+        if (p.tiles < 2 * CUS && K >= 1024) p.splits = 2 * CUS / p.tiles;
     } else {
-        const int64_t slots = p.rows == 256 ? CUS : 2 * CUS;
-        if (p.tiles < slots && K >= 512) {
-            p.splits = slots / p.tiles;
-            if (p.splits > K / 256) p.splits = K / 256;
-            if (p.splits > 256) p.splits = 256;
-            if (p.splits < 1) p.splits = 1;
+        // 0.5 us a step for 128 rows (2048 x 2048 x 2048: 22 us), 0.37 us for 64 (512 x 4096 x 4096: 27 us)
+        const int64_t steps = gs::cdiv(K, STEP);
+        for (int r = 64; r <= TILE; r += 64) {
+            const int64_t t = tiles(r, TILE);
+            if (t > CUS) continue;
+            int64_t full = CUS / t;
+            if (full > steps / 4) full = steps / 4;
+            for (const int64_t s : {(int64_t)1, full / 2, full})
+                if (s >= 1) take(r, TILE, t, s, gs::cdiv(steps, s) * (r == 64 ? 0.37 : 0.5) + join(s), true);
         }
     }
     p.slice = p.splits > 1 ? gs::cdiv(gs::cdiv(K, p.splits), 64) * 64 : K;
@@ -987,7 +1027,7 @@ template <typename T, bool ACOLS, bool BCOLS>
 int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilogue<T> E, char* ws, int64_t ws_bytes, hipStream_t stream, const float* gate, int64_t ldgate, T* db,
             Columns<T>& columns) {
     if (M == 0 || N == 0) return 0;
-    const Plan p = plan(sizeof(T), M, N, K, db != nullptr);
+    const Plan p = plan(sizeof(T), ACOLS + BCOLS, M, N, K, db != nullptr);
     GS_REQUIRE(ws_bytes >= p.bytes, "gs_linear: workspace too small");
     GS_REQUIRE(p.tiles + (int64_t)columns.blocks < (1ll << 31) && M * gs::cdiv(N, 4) < (31ll << 31), "gs_linear: too many tiles");
     Epilogue<T> first = E;
@@ -997,8 +1037,9 @@ int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilo
         const dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
         const Operand<float> A{(const float*)a.p, a.ld}, B{(const float*)b.p, b.ld};
         float* cols = db ? (p.splits > 1 ? (float*)(ws + p.at_cols) : db) : nullptr;
-        if (gate) hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, true>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
-        else hipLaunchKernelGGL((k_product32<ACOLS, BCOLS, false>), grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
+        const auto kernel = p.rows == 64 ? (gate ? k_product32<ACOLS, BCOLS, true, 64> : k_product32<ACOLS, BCOLS, false, 64>)
+                                         : (gate ? k_product32<ACOLS, BCOLS, true, 128> : k_product32<ACOLS, BCOLS, false, 128>);
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, A, gate, ldgate, B, M, N, K, p.slice, first, cols);
         if (db && p.splits > 1) beside = Columns<T>{cols, db, M, (int)p.splits, (uint32_t)gs::cdiv(M, 32)};
     } else {
         const dim3 grid((unsigned)(p.tiles + columns.blocks), (unsigned)p.splits);
@@ -1057,7 +1098,7 @@ int product_rows(const Line& x, const Line& w, int64_t M, int64_t N, int64_t K, 
 
 static int64_t forward_bytes(int es, const Line& x, const Line& w, int64_t M, int64_t N, int64_t K) {
     if (M <= FEW_ROWS) return rows_plan(M, N, K).bytes;
-    return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, M, N, K, false).bytes;
+    return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, 0, M, N, K, false).bytes;
 }
 
 template <typename T>
@@ -1097,9 +1138,9 @@ static BackwardPlan backward_plan(const Line& g, bool has_dact, const Line& x, c
     p.packs = p.cols + (p.pass && want_b ? align256(p.slabs * N * 4) : 0);
     p.prod = p.packs + (want_x ? packed_bytes(es, w, N) : 0) + (want_w ? packed_bytes(es, x, M) : 0);
     int64_t b = 0;
-    if (want_x) b = plan(es, M, K, N, false).bytes;
+    if (want_x) b = plan(es, 1, M, K, N, false).bytes;
     if (want_w) {
-        const int64_t c = plan(es, N, K, M, p.sums_with_w).bytes;
+        const int64_t c = plan(es, 2, N, K, M, p.sums_with_w).bytes;
         if (c > b) b = c;
     }
     p.total = p.prod + b;

@@ -128,3 +128,20 @@ def test_clip_c_entry_refuses_bad_arguments():
     for kw in (dict(ptr=None), dict(out=None), dict(numel=-1), dict(dtype=3), dict(dtype=-1), dict(kind=3), dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(norm=n), dict(ws=8)):
         assert call(**kw) != 0 and b"gs_grad_norm" in L.gs_last_error(), kw
     assert L.gs_grad_norm_workspace_bytes(c_int(-1)) == -1
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_linear_workspace_sizes(dtype):
+    """The plan of a call is made on the host: sizes from nothing to the largest, none negative, and for ordinary layers no more than a few times their operands."""
+    from gshell_amd import _lib
+    L = _lib.lib()
+    es = 4 if dtype == 0 else 2
+    for M in (0, 1, 2, 31, 32, 33, 64, 1000, 4096, 131072, (1 << 31) - 1):
+        for N in (0, 1, 7, 8, 64, 1000, 4096, 65536):
+            for K in (0, 1, 8, 295, 777, 4096, 65536):
+                for ld, at in ((K, 0), (K + 3, 2)):
+                    fwd = L.gs_linear_fwd_workspace_bytes(1024 + at, ld, 2048, K, M, N, K, dtype)
+                    bwd = L.gs_linear_bwd_workspace_bytes(4096, N, 1, 1024 + at, ld, 2048, K, M, N, K, dtype, 1, 1, 1)
+                    assert fwd >= 0 and bwd >= 0, (M, N, K)
+                    if max(M, N, K) < 5000:
+                        assert fwd <= 8 * es * (M * K + N * K + M * N) + (64 << 20) and bwd <= 8 * es * (M * K + N * K + M * N) + (160 << 20), (M, N, K, fwd, bwd)
