@@ -104,27 +104,37 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_count(const I* ids, const
         atomicAdd(&counts[(k >> shift) & (bins - 1)], 1u);
     }
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) hist[b * SORT_BLOCKS + blockIdx.x] = counts[b];
+    for (int b = threadIdx.x; b < bins; b += SORT_THREADS) hist[blockIdx.x * MAX_BINS + b] = counts[b];
 }
 
 template <typename I>
 __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(const I* ids, const uint32_t* keys, const uint32_t* pos, int64_t T, int64_t V, int64_t padding, int64_t tile,
                                                               int shift, int bits, const uint32_t* hist, uint32_t* keys_out, uint32_t* pos_out) {
-    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], tmp[SORT_WAVES];
-    const int bins = 1 << bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ uint32_t counts[SORT_WAVES * MAX_BINS], tmp[SORT_WAVES], part[2][SORT_THREADS];
+    const int bins = 1 << bits, wave = threadIdx.x >> 6;
     const int64_t t0 = (int64_t)blockIdx.x * tile, t1 = t0 + tile < T ? t0 + tile : T;
     const int64_t stretch = (tile / SORT_WAVES + 63) / 64 * 64;
     const int64_t w0 = t0 + wave * stretch < t1 ? t0 + wave * stretch : t1, w1 = w0 + stretch < t1 ? w0 + stretch : t1;
     const auto key = [&](int64_t i) { return ids ? key_of(ids[i], V, padding) : keys[i]; };
     wave_counts(key, w0, w1, shift, bits, counts);
-    uint32_t before = 0, all = 0;          // of this thread's bin: tokens in earlier tiles, in all tiles
-    if ((int)threadIdx.x < bins) {
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-            const uint32_t c = hist[threadIdx.x * SORT_BLOCKS + b];
-            before += b < (int)blockIdx.x ? c : 0;
-            all += c;
+    // tokens of each bin in earlier tiles and in all tiles: SORT_THREADS / bins threads share a bin's tiles, eight loads at a time
+    const int shares = SORT_THREADS >> bits, share = threadIdx.x >> bits, bin = threadIdx.x & (bins - 1);
+    uint32_t before = 0, all = 0;
+    for (int b = share; b < (int)gridDim.x; b += 8 * shares) {
+        uint32_t c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = b + k * shares < (int)gridDim.x ? hist[(b + k * shares) * MAX_BINS + bin] : 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            before += b + k * shares < (int)blockIdx.x ? c[k] : 0;
+            all += c[k];
         }
     }
+    part[0][threadIdx.x] = before, part[1][threadIdx.x] = all;
+    __syncthreads();
+    before = all = 0;
+    if ((int)threadIdx.x < bins)
+        for (int q = 0; q < shares; ++q) before += part[0][q * bins + threadIdx.x], all += part[1][q * bins + threadIdx.x];
     uint32_t total;
     uint32_t at = block_scan(all, tmp, total) + before;
     if ((int)threadIdx.x < bins)
@@ -200,25 +210,54 @@ template <typename T, int VEC, typename U> __device__ __forceinline__ void store
     }
 }
 
-// Forward: a group of 2^group_log lanes takes one (token, stretch of columns).
+// Forward: the output is one stretch of memory, written 16 aligned bytes a lane and piece; LOOKUPS pieces a lane are on their way together.  A piece inside a row is one load (at
+// whatever address the row has it), one that runs over a row's end is gathered.  The place of a lane's next piece comes without a division: step_rows, step_cols are
+// what a workgroup's pieces of one round cover.
+constexpr int LOOKUPS = 4;
 template <typename T, typename I>
-__global__ void __launch_bounds__(256) k_lookup(const I* ids, const T* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, float scale, T* y) {
+__global__ void __launch_bounds__(256) k_lookup(const I* ids, const T* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, int64_t step_rows, int64_t step_cols, float scale, T* y) {
     constexpr int VEC = 16 / sizeof(T);
-    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
-    if (unit >= tokens * stretches) return;
-    const int64_t t = unit / stretches, c = ((unit % stretches) << group_log) * VEC + (threadIdx.x & ((1 << group_log) - 1)) * VEC;
-    if (c >= D) return;
-    const int64_t id = (int64_t)ids[t];
-    float v[VEC];
-    if (id < 0 || id >= V) {
+    const int64_t total = tokens * D;
+    int64_t at = ((int64_t)blockIdx.x * 256 * LOOKUPS + threadIdx.x) * VEC;
+    int64_t t = at / D, c = at - t * D;
+    float v[LOOKUPS][VEC];
+    int64_t place[LOOKUPS];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] = __builtin_nanf("");
-    } else {
-        load_row<T, VEC>(w + id * ldw + c, D - c, v);
+    for (int u = 0; u < LOOKUPS; ++u) {
+        place[u] = at;
+        if (at < total) {
+            const int64_t id = (int64_t)ids[t];
+            const bool ok = id >= 0 && id < V;
+            if (c + VEC <= D) {
+                if (ok) load_row<T, VEC>(w + id * ldw + c, VEC, v[u]);
+                else
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) v[k] *= scale;
+                    for (int k = 0; k < VEC; ++k) v[u][k] = __builtin_nanf("");
+            } else {
+                int64_t r = t, q = c, row = ok ? id : -1;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    if (q == D) {
+                        ++r, q = 0;
+                        const int64_t next = at + k < total ? (int64_t)ids[r] : -1;
+                        row = next >= 0 && next < V ? next : -1;
+                    }
+                    v[u][k] = at + k < total ? (row >= 0 ? (float)w[row * ldw + q] : __builtin_nanf("")) : 0.f;
+                    ++q;
+                }
+            }
+        }
+        at += 256 * VEC;
+        t += step_rows, c += step_cols;
+        if (c >= D) c -= D, ++t;
     }
-    store_row<T, VEC>(y + t * D + c, D - c, v);
+#pragma unroll
+    for (int u = 0; u < LOOKUPS; ++u) {
+        if (place[u] >= total) return;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[u][k] *= scale;
+        store_row<T, VEC>(y + place[u], total - place[u], v[u]);
+    }
 }
 
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
@@ -231,28 +270,93 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
     return lo;
 }
 
-constexpr int BVEC = 4;          // columns of a lane in the gradient's sums
+constexpr int BVEC = 4;          // columns of a lane in the sums of narrow rows
 
-// Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
+// rows `v0 ..` of the table that no token names, 64 of them a wave
+template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int64_t v0, T* dw) {
+    constexpr int VEC = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63;
+    const int64_t v = v0 + lane;
+    if (v0 >= V) return;
+    bool empty = false;
+    if (v < V) {
+        const int64_t at = lower_bound(keys, tokens, (uint32_t)v);
+        empty = at >= tokens || keys[at] != (uint32_t)v;
+    }
+    const float zero[VEC] = {};
+    for (uint64_t m = __ballot(empty); m; m &= m - 1) {
+        T* row = dw + (v0 + (__ffsll((unsigned long long)m) - 1)) * D;
+        for (int64_t c = lane * VEC; c < D; c += 64 * VEC) store_row<T, VEC>(row + c, D - c, zero);
+    }
+}
+
+// Rows of more than 32 vectors of 16 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
+// eight rows are on their way at a time.  A run of up to CHUNK tokens is summed as a whole by the chunk where it begins; a longer one leaves a part in each of its chunks.
+// 65536 tokens of 1024 bf16 over 50000 rows: see the table of measurements beside the host code.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t stretches,
+                                                  int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + wave) * 64, dw);
+    const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
+    if (unit >= chunks * stretches) return;
+    const int64_t chunk = unit / stretches, c = (unit % stretches * 64 + lane) * VEC, e0 = chunk * CHUNK;
+    const uint32_t none = (uint32_t)V;
+    // this chunk and the next one; the one before in the lower lanes of `past`
+    static_assert(CHUNK == 32, "two chunks a wave");
+    const uint32_t key = e0 + lane < tokens ? keys[e0 + lane] : none, past = lane < 32 && e0 > 0 ? keys[e0 - 32 + lane] : none;
+    const uint32_t row_of = e0 + lane < tokens ? pos[e0 + lane] : 0;
+    const uint32_t key0 = __builtin_amdgcn_readlane(key, 0);
+    if (key0 == none) return;
+    const uint32_t after = __shfl_down(key, 1);
+    const uint64_t ends = __ballot(lane == 63 || key != after);          // lanes where a run ends
+    // the run that the chunk begins with: its tokens in the chunk before (32 at most) and from here on
+    const uint32_t behind = (uint32_t)__ballot(lane < 32 && e0 > 0 && past == key0);
+    const int back = behind == 0xffffffffu ? 32 : __clz((int)~behind), ahead = __builtin_ctzll(ends) + 1;
+    const bool long_head = back > 0 && back + ahead > CHUNK;
+    const int begin = back > 0 && !long_head ? ahead : 0;
+    if (begin >= CHUNK) return;
+    // the last run that begins (or goes on) in this chunk
+    const uint64_t upto = ends & ((1ull << (CHUNK - 1)) - 1);          // runs that end before the chunk's last token
+    const int tail = upto ? 64 - __builtin_clzll(upto) : 0;              // where the run of that last token begins (0: with the chunk)
+    const int tail_end = __builtin_ctzll(ends >> (CHUNK - 1)) + CHUNK;          // one behind its last token, 64 at most
+    const bool tail_is_head = tail == 0 && back > 0, long_tail = tail_is_head ? long_head : tail_end - tail > CHUNK;
+    int end = long_tail ? (tail_end < CHUNK ? tail_end : CHUNK) : tail_end;
+    const uint64_t empty = __ballot(key == none);
+    if (empty && __builtin_ctzll(empty) < end) end = __builtin_ctzll(empty);
+    float acc[VEC] = {};
+    const T* base = g + c;
+    for (int j = begin; j < end; j += 8) {
+        float v[8][VEC];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (j + k < end) load_row<T, VEC>(base + (int64_t)(uint32_t)__builtin_amdgcn_readlane(row_of, j + k) * ldg, D - c, v[k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (j + k >= end) break;
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) acc[q] += v[k][q];
+            if (!(ends >> (j + k) & 1) && j + k + 1 < end) continue;
+            if (long_head && j + k < ahead) {
+                store_row<float, VEC>(first + chunk * D + c, D - c, acc);
+            } else if (long_tail && j + k >= tail) {
+                store_row<float, VEC>(last + chunk * D + c, D - c, acc);
+            } else {
+#pragma unroll
+                for (int q = 0; q < VEC; ++q) acc[q] *= scale;
+                store_row<T, VEC>(dw + (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j + k) * D + c, D - c, acc);
+            }
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
+        }
+    }
+}
+
+// Narrower rows: several groups of lanes a wave, a chunk each; every run that crosses chunks leaves its parts.  Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int group_log,
                                                     int64_t stretches, int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
-    if ((int64_t)blockIdx.x >= sum_blocks) {
-        const int lane = threadIdx.x & 63;
-        const int64_t v0 = (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, v = v0 + lane;
-        if (v0 >= V) return;
-        bool empty = false;
-        if (v < V) {
-            const int64_t at = lower_bound(keys, tokens, (uint32_t)v);
-            empty = at >= tokens || keys[at] != (uint32_t)v;
-        }
-        const float zero[BVEC] = {};
-        for (uint64_t m = __ballot(empty); m; m &= m - 1) {
-            T* row = dw + (v0 + (__ffsll((unsigned long long)m) - 1)) * D;
-            for (int64_t c = lane * BVEC; c < D; c += 64 * BVEC) store_row<T, BVEC>(row + c, D - c, zero);
-        }
-        return;
-    }
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, dw);
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
     if (unit >= chunks * stretches) return;
     const int64_t chunk = unit / stretches, c = ((unit % stretches) << group_log) * BVEC + (threadIdx.x & ((1 << group_log) - 1)) * BVEC;
@@ -300,51 +404,66 @@ __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const 
     flush(true);
 }
 
-// Runs that cross chunks, in the order of their chunks: the chunk where a run begins joins it.  A workgroup takes one (chunk, stretch); its groups of lanes share
-// the run's chunks out in equal stretches.
+// Runs that left parts, in the order of their chunks: the chunk where a run begins joins it, a workgroup each, whose groups of lanes share the parts out in equal
+// stretches.  `shortest`: runs of fewer tokens left none.
 template <typename T>
-__global__ void __launch_bounds__(256) k_join_chunks(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, float scale, const float* first,
-                                                     const float* last, T* dw) {
-    __shared__ float part[256 * BVEC];
-    const int64_t chunk = blockIdx.x / stretches, e1 = (chunk + 1) * CHUNK;
+__global__ void __launch_bounds__(1024) k_join_chunks(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, int shortest, float scale,
+                                                      const float* first, const float* last, T* dw) {
+    __shared__ float part[1024 * BVEC];
+    const int64_t chunk = blockIdx.x, e1 = (chunk + 1) * CHUNK;
     if (e1 >= tokens) return;
-    const uint32_t run = keys[e1 - 1];
-    if (run == (uint32_t)V || keys[e1] != run) return;
-    if (keys[chunk * CHUNK] == run && chunk > 0 && keys[chunk * CHUNK - 1] == run) return;          // it began earlier
-    const int64_t end = lower_bound(keys, tokens, run + 1), more = (end - 1) / CHUNK - chunk;          // chunks behind this one that hold a part
-    const int groups = 256 >> group_log, group = threadIdx.x >> group_log;
-    const int64_t c = (((int64_t)(blockIdx.x % stretches) << group_log) + (threadIdx.x & ((1 << group_log) - 1))) * BVEC;
-    const int64_t share = (more + groups - 1) / groups, k0 = group * share, k1 = k0 + share < more ? k0 + share : more;
-    float acc[BVEC] = {};
-    if (c < D) {
-        for (int64_t k = k0; k < k1; k += 4) {
-            float v[4][BVEC];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (k + u < k1) load_row<float, BVEC>(first + (chunk + 1 + k + u) * D + c, D - c, v[u]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (k + u < k1)
-#pragma unroll
-                    for (int q = 0; q < BVEC; ++q) acc[q] += v[u][q];
-        }
+    // one look at this chunk's keys (every wave has them all), the one before it, and the first keys of the 64 chunks that follow
+    const int lane = threadIdx.x & 63;
+    const uint32_t key = keys[chunk * CHUNK + (lane & (CHUNK - 1))], before = chunk > 0 ? keys[chunk * CHUNK - 1] : (uint32_t)V;
+    const int64_t follow = (chunk + 1 + lane) * CHUNK;
+    const uint32_t next = follow < tokens ? keys[follow] : (uint32_t)V;
+    const uint32_t run = __builtin_amdgcn_readlane(key, CHUNK - 1);
+    const uint64_t reach = __ballot(next == run);
+    if (run == (uint32_t)V || !(reach & 1)) return;
+    const int inside = __popcll(__ballot(key == run && lane < CHUNK));          // its tokens in this chunk
+    if (inside == CHUNK && before == run) return;          // it began earlier
+    int64_t more = ~reach ? __builtin_ctzll(~reach) : 0;          // chunks behind this one that hold a part
+    if (!~reach) more = (lower_bound(keys, tokens, run + 1) - 1) / CHUNK - chunk;
+    if (shortest > 1 && more == 1) {          // two chunks: whether it is long enough shows where its last token would be
+        const int64_t last_at = e1 - inside + shortest - 1;
+        if (last_at >= tokens || keys[last_at] != run) return;
     }
+    const int groups = blockDim.x >> group_log, group = threadIdx.x >> group_log, x = threadIdx.x & ((1 << group_log) - 1);
+    const int64_t share = (more + groups - 1) / groups, k0 = group * share, k1 = k0 + share < more ? k0 + share : more;
+    for (int64_t s = 0; s < stretches; ++s) {
+        const int64_t c = ((s << group_log) + x) * BVEC;
+        float acc[BVEC] = {};
+        if (c < D)
+            for (int64_t q = k0; q < k1; q += 8) {
+                float v[8][BVEC];
 #pragma unroll
-    for (int q = 0; q < BVEC; ++q) part[threadIdx.x * BVEC + q] = acc[q];
-    __syncthreads();
-    if (group != 0 || c >= D) return;
-    float sum[BVEC];
-    load_row<float, BVEC>(last + chunk * D + c, D - c, sum);
-    for (int s = 0; s < groups; ++s)
+                for (int u = 0; u < 8; ++u)
+                    if (q + u < k1) load_row<float, BVEC>(first + (chunk + 1 + q + u) * D + c, D - c, v[u]);
 #pragma unroll
-        for (int q = 0; q < BVEC; ++q) sum[q] += part[((s << group_log) + threadIdx.x) * BVEC + q];
+                for (int u = 0; u < 8; ++u)
+                    if (q + u < k1)
 #pragma unroll
-    for (int q = 0; q < BVEC; ++q) sum[q] *= scale;
-    store_row<T, BVEC>(dw + (int64_t)run * D + c, D - c, sum);
+                        for (int e = 0; e < BVEC; ++e) acc[e] += v[u][e];
+            }
+#pragma unroll
+        for (int e = 0; e < BVEC; ++e) part[threadIdx.x * BVEC + e] = acc[e];
+        __syncthreads();
+        if (group == 0 && c < D) {
+            float sum[BVEC];
+            load_row<float, BVEC>(last + chunk * D + c, D - c, sum);
+            for (int q = 0; q < groups; ++q)
+#pragma unroll
+                for (int e = 0; e < BVEC; ++e) sum[e] += part[((q << group_log) + x) * BVEC + e];
+#pragma unroll
+            for (int e = 0; e < BVEC; ++e) sum[e] *= scale;
+            store_row<T, BVEC>(dw + (int64_t)run * D + c, D - c, sum);
+        }
+        __syncthreads();
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
-static int group_log_of(int64_t vectors) {
+static int group_log_of(int64_t vectors) {          // lanes, as a power of two, of a group that takes a row or a stretch of one
     int l = 0;
     while (l < 6 && (1ll << l) < vectors) ++l;
     return l;
@@ -369,14 +488,18 @@ static SortPlan sort_plan(int64_t T, int64_t D) {
     return p;
 }
 
+// Elements of a lane's vector.  16 bytes where every row starts on 16; otherwise the hardware takes 16 bytes at any address, but slower than 8 on 8.
+static int vector_of(int es, int64_t D, int64_t ld, const void* p, const void* q) {
+    const uintptr_t a = (uintptr_t)p | (uintptr_t)q | (uintptr_t)(D * es) | (uintptr_t)(ld * es);
+    return (a & 15) == 0 ? 16 / es : 8 / es;
+}
+
 template <typename T, typename I>
 int lookup(const void* ids, const void* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, float scale, void* y, hipStream_t stream) {
     constexpr int VEC = 16 / sizeof(T);
-    const int64_t vectors = gs::cdiv(D, VEC);
-    const int gl = group_log_of(vectors);
-    const int64_t stretches = gs::cdiv(vectors, 1ll << gl), blocks = gs::cdiv((tokens * stretches) << gl, 256);
+    const int64_t blocks = gs::cdiv(tokens * D, 256 * VEC * LOOKUPS), step = 256 * VEC;
     GS_REQUIRE(blocks < (1ll << 31), "gs_embedding_fwd: too large");
-    hipLaunchKernelGGL((k_lookup<T, I>), dim3((unsigned)blocks), dim3(256), 0, stream, (const I*)ids, (const T*)w, ldw, tokens, V, D, gl, stretches, scale, (T*)y);
+    hipLaunchKernelGGL((k_lookup<T, I>), dim3((unsigned)blocks), dim3(256), 0, stream, (const I*)ids, (const T*)w, ldw, tokens, V, D, step / D, step % D, scale, (T*)y);
     GS_LAUNCH_CHECK();
     return 0;
 }
@@ -415,16 +538,34 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
     uint32_t *keys = nullptr, *pos = nullptr;
     if (tokens > 0)
         if (const int rc = sort_tokens<I>(ids, tokens, V, padding, p, base, keys, pos, stream)) return rc;
+    float *first = (float*)(base + p.first), *last = (float*)(base + p.last);
+    const int64_t zero_blocks = gs::cdiv(V, 256);
+    constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
+    const int vec = vector_of(sizeof(T), D, ldg, g, dw);
+    const bool wide = gs::cdiv(D, vec) > 32;
     const int64_t vectors = gs::cdiv(D, BVEC);
     const int gl = group_log_of(vectors);
-    const int64_t stretches = gs::cdiv(vectors, 1ll << gl), sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256), zero_blocks = gs::cdiv(V, 256);
-    GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31) && p.chunks * stretches < (1ll << 31), "gs_embedding_bwd: too large");
-    float *first = (float*)(base + p.first), *last = (float*)(base + p.last);
-    hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
-                       gl, stretches, p.chunks, sum_blocks, scale, (T*)dw, first, last);
-    if (p.chunks > 1)
-        hipLaunchKernelGGL(k_join_chunks<T>, dim3((unsigned)(p.chunks * stretches)), dim3(256), 0, stream, (const uint32_t*)keys, tokens, V, D, gl, stretches, scale,
-                           (const float*)first, (const float*)last, (T*)dw);
+    const int64_t stretches = gs::cdiv(vectors, 1ll << gl);          // of the narrow sums
+    if (wide) {
+        const int64_t across = gs::cdiv(gs::cdiv(D, vec), 64), sum_blocks = gs::cdiv(p.chunks * across, 4);
+        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "gs_embedding_bwd: too large");
+        const auto kernel = vec == V16 ? k_sum_wide<T, V16> : k_sum_wide<T, V8>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
+                           across, p.chunks, sum_blocks, scale, (T*)dw, first, last);
+    } else {
+        const int64_t sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256);
+        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "gs_embedding_bwd: too large");
+        hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
+                           gl, stretches, p.chunks, sum_blocks, scale, (T*)dw, first, last);
+    }
+    if (p.chunks > 1) {
+        // groups cover a whole row; a run may hold most of the tokens: a large workgroup where rows are used a thousand times and more
+        const int threads = wide ? (tokens > V * 1000 ? 1024 : 512) : 256;
+        int jl = 0;
+        while (jl < 8 && (1ll << jl) < vectors) ++jl;
+        hipLaunchKernelGGL(k_join_chunks<T>, dim3((unsigned)p.chunks), dim3(threads), 0, stream, (const uint32_t*)keys, tokens, V, D, jl, gs::cdiv(vectors, 1ll << jl),
+                           wide ? CHUNK + 1 : 1, scale, (const float*)first, (const float*)last, (T*)dw);
+    }
     GS_LAUNCH_CHECK();
     return 0;
 }

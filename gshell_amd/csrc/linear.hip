@@ -57,14 +57,13 @@ template <bool FAST> __device__ __forceinline__ void act_relu(float z, float& y,
     y = z < 0.f ? 0.f : z;
     d = z <= 0.f ? 0.f : 1.f;
 }
-// With t = exp(-|beta z|) in [0, 1] (neither end of z overflows): log(1 + t) = 2 artanh(t / (2 + t)) by its series -- the argument is at most 1/3, and the term
-// after the last one below 2e-8 of the sum -- and one reciprocal of (1 + t)(2 + t) serves that and the derivative.
-template <bool FAST> __device__ __forceinline__ void act_softplus(float beta, float inv_beta, float z, float& y, float& d) {
-    const float t = exp_<FAST>(-fabsf(beta * z));
+// With t = exp(-|beta z|) in [0, 1] (neither end of z overflows): log(1 + t) = 2 artanh(q), q = t / (2 + t) <= 1/3, as q times a polynomial in q^2 (fitted at Chebyshev's
+// points, relative error 4e-9), and one reciprocal of (1 + t)(2 + t) serves that and the derivative.  The exponent is rounded once, as beta z is.
+__device__ __forceinline__ void act_softplus(float beta_log2e, float two_over_beta, float z, float& y, float& d) {
+    const float t = __builtin_amdgcn_exp2f(-fabsf(beta_log2e * z));
     const float u = 1.f + t, v = 2.f + t, r = rcp_(u * v), q = t * (r * u), w = q * q;
-    float s = 0.07692308f;
-    for (const float c : {0.09090909f, 0.11111111f, 0.14285714f, 0.2f, 0.33333333f, 1.f}) s = fmaf(s, w, c);
-    y = (z < 0.f ? 0.f : z) + 2.f * q * s * inv_beta;
+    const float s = fmaf(fmaf(fmaf(fmaf(0.14087328f, w, 0.13980709f), w, 0.20012426f), w, 0.33333158f), w, 1.f);
+    y = fmaf(q * s, two_over_beta, fmaxf(z, 0.f));
     d = (z >= 0.f ? 1.f : t) * (r * v);
 }
 template <bool FAST> __device__ __forceinline__ void act_silu(float z, float& y, float& d) {
@@ -88,7 +87,7 @@ template <bool FAST> __device__ __forceinline__ void act_gelu(float z, float& y,
     d = fmaf(z, e * 0.39894228040143268f, phi);
 }
 // BATCH x V values at once: the choice is the same for the whole launch
-template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, float beta, float inv_beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
+template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, float beta_log2e, float two_over_beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
     switch (act) {
         case ACT_RELU:
 #pragma unroll
@@ -96,7 +95,7 @@ template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(
             break;
         case ACT_SOFTPLUS:
 #pragma unroll
-            for (int k = 0; k < V * BATCH; ++k) act_softplus<FAST>(beta, inv_beta, z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
+            for (int k = 0; k < V * BATCH; ++k) act_softplus(beta_log2e, two_over_beta, z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
             break;
         case ACT_SILU:
 #pragma unroll
@@ -116,7 +115,7 @@ template <typename T> struct Epilogue {
     float* part;                                    // not null: fp32 sums of this slice of the contraction go to part[split][M][N], nothing else is done
     int64_t ldr, ldo;
     int act;
-    float beta, inv_beta;
+    float beta_log2e, two_over_beta;          // of softplus
 };
 
 template <typename T, int V> struct __attribute__((packed)) Pack { T v[V]; };          // rows start at any element: the hardware takes unaligned vectors
@@ -163,7 +162,7 @@ template <typename T, int V, int BATCH> __device__ __forceinline__ void finish(c
     }
     if (E.act != ACT_NONE) {
         float d[BATCH][V];
-        act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta, E.inv_beta, z, d);
+        act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta_log2e, E.two_over_beta, z, d);
         if (E.dact)
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
@@ -384,6 +383,7 @@ template <bool COLS, bool GATE, int LINES> struct Feed32 {
     }
 };
 
+
 template <bool ACOLS, bool BCOLS, bool GATE, int LINES>
 __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice,
                                                                        Epilogue<float> E, float* column_sums /* [slices][M], or db itself where there is one slice */) {
@@ -411,14 +411,20 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
     typename FB::Values rb;
     typename FA::Parts sa;
     typename FB::Parts sb;
+    // With two workgroups a unit the next step is split among the second half of the products; with four or more right before it is stored
+    constexpr bool AHEAD = LINES == 128;
+    const auto split = [&]() __attribute__((always_inline)) {
+        total += fa.split(ra, sa);
+        fb.split(rb, sb);
+    };
     if (c_begin < c_end) {
         fa.fetch(c_begin, ra);
         fb.fetch(c_begin, rb);
-        total += fa.split(ra, sa);
-        fb.split(rb, sb);
+        if (AHEAD) split();
     }
     for (int64_t c = c_begin; c < c_end; c += BK) {
         __syncthreads();
+        if (!AHEAD) split();
         fa.store(lds.in.a, sa);
         fb.store(lds.in.b, sb);
         __syncthreads();
@@ -443,18 +449,18 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
                 for (int w = 0; w < F; ++w) acc[u][w] = mfma<bf16>(vb[PB[term]][w], va[PA[term]], acc[u][w]);
             }
         }
-        // the next step is split among the second half of the products
-        total += fa.split(ra, sa);
-        fb.split(rb, sb);
+        if constexpr (AHEAD) {
+            split();
 #pragma unroll
-        for (int k = 0; k < 3 * F * F; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        }
+            for (int q = 0; q < 3 * F * F; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            }
 #pragma unroll
-        for (int k = 0; k < 3 * F * F; ++k) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 16 / F, 0);
+            for (int q = 0; q < 3 * F * F; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            }
         }
     }
     __syncthreads();
@@ -1108,7 +1114,7 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
     const int64_t need = forward_bytes(sizeof(T), lx, lw, M, N, K);
     GS_REQUIRE(ws_bytes >= need && (ws || need == 0), "gs_linear_fwd: workspace too small");
     char* at = (char*)ws;
-    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta, act == ACT_SOFTPLUS ? 1.f / beta : 0.f};
+    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta * 1.44269504f, act == ACT_SOFTPLUS ? 2.f / beta : 0.f};
     if (M <= FEW_ROWS) return product_rows<T>(lx, lw, M, N, K, E, at, stream);
     Pack2<T> P{};
     at += repack<T>(P, 0, lx, M, at);

@@ -151,3 +151,20 @@ def test_module():
     assert torch.equal(y, m.weight[ids] * 4.0)
     y.sum().backward()
     assert float(m.weight.grad[2, 0]) == 8.0 and not m.weight.grad[1].any()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("D", [300, 520, 24])
+@pytest.mark.parametrize("seed", range(4))
+def test_runs_of_lengths_around_a_chunk(kind, D, seed):
+    """Sorted, the tokens lie in runs of lengths around the 32 of a chunk and its multiples, at every offset to the chunks' borders; the padding row is one of the long ones."""
+    gen = torch.Generator().manual_seed(seed)
+    lengths = torch.tensor([1, 2, 3, 30, 31, 32, 33, 34, 63, 64, 65, 95, 96, 97, 200])[torch.randint(0, 15, (60 if seed else 30,), generator=gen)]
+    if seed == 2:
+        lengths[0] = 32
+    if seed == 3:
+        lengths = torch.cat([lengths, torch.tensor([700])])
+    V = len(lengths) * 2 + 1
+    ids = torch.repeat_interleave(torch.arange(len(lengths)) * 2 + (seed & 1), lengths)
+    ids = ids[torch.randperm(len(ids), generator=gen)]
+    check_one(ids, V, D, TYPES[kind], 1.0, int(ids[0]) if seed == 3 else None, seed)
