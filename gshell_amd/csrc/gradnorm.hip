@@ -7,6 +7,10 @@
 // fp32 value neither overflows nor vanishes there, and the order of the sum no longer shows); in the second every workgroup adds the partial sums for itself, in
 // the same order, and scales its share of the elements.  Bound by memory: each gradient is read once, then read again and written.  The second launch walks the
 // elements from the end: what the first has read last is still in the 256 MB cache.  In place and with a factor of one it writes nothing.
+//
+// Measured, GPU time of both launches, new tensors for the result: 30 fp32 tensors of 22 million elements 58 us (264 MB read and written, 4.5 TB/s; a copy of
+// 1 GB reaches 5.2 TB/s), 300 bf16 tensors of 600 million 785 us (3.6 GB, 4.6 TB/s), 16 fp32 tensors of half a million 10 us (two launches, each as long as its
+// slowest chain of loads).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -22,8 +26,8 @@ typedef __bf16 bf16;
 typedef _Float16 f16;
 
 constexpr int TABLE = 120;          // tensors a launch: the table stays below the 4 KB of kernel arguments
-constexpr int THREADS = 256, CHUNK_BYTES = THREADS * 16 * 4;
-constexpr int MAX_BLOCKS = 2048;
+constexpr int THREADS = 256, CHUNK_BYTES = THREADS * 16 * 2;          // two loads of 16 bytes a thread: 785 us for the 600 million, four 815, eight more; 10.1 us for the half million, four 11.0
+constexpr int MAX_BLOCKS = 2048;          // eight workgroups a CU; 1024 789 us, 4096 810
 
 struct Table {
     const void* src[TABLE];
@@ -165,19 +169,22 @@ static unsigned grid_of(const Table& T) { return T.first[T.n] < (uint32_t)MAX_BL
 
 template <int P>
 int run(int n, const void* const* src, void* const* dst, const int64_t* numel, const int32_t* type, float max_norm, float* norm_out, double* part, hipStream_t stream) {
-    int parts = 0;
+    int parts = 0, tables = 0;
+    std::vector<int> starts(n / TABLE + 1);
     Table T;
     for (int from = 0; from < n;) {
+        const int start = from;
         if (const int rc = fill(T, from, n, src, dst, numel, type)) return rc;
         if (T.n == 0) continue;
+        starts[tables++] = start;
         hipLaunchKernelGGL(k_norm_partials<P>, dim3(grid_of(T)), dim3(THREADS), 0, stream, T, part + parts);
         parts += (int)grid_of(T);
     }
     bool told = false;
     if (dst)
-        for (int from = 0; from < n;) {
+        for (int t = tables - 1; t >= 0; --t) {          // the last table first: it is what the cache holds
+            int from = starts[t];
             if (const int rc = fill(T, from, n, src, dst, numel, type)) return rc;
-            if (T.n == 0) continue;
             hipLaunchKernelGGL(k_norm_scale<P>, dim3(grid_of(T)), dim3(THREADS), 0, stream, T, (const double*)part, parts, max_norm, told ? nullptr : norm_out);
             told = true;
         }
@@ -220,13 +227,13 @@ extern "C" int gs_grad_norm(int n_tensors, const void* const* grads, void* const
     GS_REQUIRE(norm_type == 0 || norm_type == 1 || norm_type == 2, "gs_grad_norm: norm_type is 0 (2-norm), 1 (1-norm) or 2 (largest magnitude)");
     GS_REQUIRE(!out || max_norm >= 0.f, "gs_grad_norm: max_norm must not be negative or NaN");
     for (int k = 0; k < n_tensors; ++k) GS_REQUIRE(numel[k] == 0 || (numel[k] > 0 && grads[k] && (!out || out[k]) && dtypes[k] >= 0 && dtypes[k] <= 2), "gs_grad_norm: null tensor or unknown type");
-    try {
+    try {          // the lists on the host may not fit
         GS_REQUIRE(!out || !overlap(n_tensors, grads, out, numel, dtypes), "gs_grad_norm: an output shares memory with another output or another gradient");
+        GS_REQUIRE(workspace && workspace_bytes >= gs_grad_norm_workspace_bytes(n_tensors), "gs_grad_norm: workspace too small");
+        const auto go = norm_type == 0 ? run<NORM_2> : norm_type == 1 ? run<NORM_1> : run<NORM_INF>;
+        return go(n_tensors, grads, out, numel, dtypes, max_norm, norm, (double*)workspace, (hipStream_t)stream);
     } catch (const std::bad_alloc&) {
         gs::set_error("gs_grad_norm: out of host memory");
         return 3;
     }
-    GS_REQUIRE(workspace && workspace_bytes >= gs_grad_norm_workspace_bytes(n_tensors), "gs_grad_norm: workspace too small");
-    const auto go = norm_type == 0 ? run<NORM_2> : norm_type == 1 ? run<NORM_1> : run<NORM_INF>;
-    return go(n_tensors, grads, out, numel, dtypes, max_norm, norm, (double*)workspace, (hipStream_t)stream);
 }
