@@ -410,7 +410,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) k_join_chunks(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int group_log, int64_t stretches, int shortest, float scale,
                                                       const float* first, const float* last, T* dw) {
     __shared__ float part[1024 * BVEC];
-    const int64_t chunk = blockIdx.x, e1 = (chunk + 1) * CHUNK;
+    const int64_t chunk = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, e1 = (chunk + 1) * CHUNK;
     if (e1 >= tokens) return;
     // one look at this chunk's keys (every wave has them all), the one before it, and the first keys of the 64 chunks that follow
     const int lane = threadIdx.x & 63;
@@ -498,7 +498,7 @@ template <typename T, typename I>
 int lookup(const void* ids, const void* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, float scale, void* y, hipStream_t stream) {
     constexpr int VEC = 16 / sizeof(T);
     const int64_t blocks = gs::cdiv(tokens * D, 256 * VEC * LOOKUPS), step = 256 * VEC;
-    GS_REQUIRE(blocks < (1ll << 31), "gs_embedding_fwd: too large");
+    GS_REQUIRE(blocks < (1ll << 24), "gs_embedding_fwd: too large for one launch");
     hipLaunchKernelGGL((k_lookup<T, I>), dim3((unsigned)blocks), dim3(256), 0, stream, (const I*)ids, (const T*)w, ldw, tokens, V, D, step / D, step % D, scale, (T*)y);
     GS_LAUNCH_CHECK();
     return 0;
@@ -548,13 +548,13 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
     const int64_t stretches = gs::cdiv(vectors, 1ll << gl);          // of the narrow sums
     if (wide) {
         const int64_t across = gs::cdiv(gs::cdiv(D, vec), 64), sum_blocks = gs::cdiv(p.chunks * across, 4);
-        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "gs_embedding_bwd: too large");
+        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         const auto kernel = vec == V16 ? k_sum_wide<T, V16> : k_sum_wide<T, V8>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
                            across, p.chunks, sum_blocks, scale, (T*)dw, first, last);
     } else {
         const int64_t sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256);
-        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 31), "gs_embedding_bwd: too large");
+        GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
                            gl, stretches, p.chunks, sum_blocks, scale, (T*)dw, first, last);
     }
@@ -563,7 +563,8 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
         const int threads = wide ? (tokens > V * 1000 ? 1024 : 512) : 256;
         int jl = 0;
         while (jl < 8 && (1ll << jl) < vectors) ++jl;
-        hipLaunchKernelGGL(k_join_chunks<T>, dim3((unsigned)p.chunks), dim3(threads), 0, stream, (const uint32_t*)keys, tokens, V, D, jl, gs::cdiv(vectors, 1ll << jl),
+        const int64_t gx = p.chunks < (1 << 20) ? p.chunks : 1 << 20;          // a launch has fewer than 2^32 lanes either way of its grid
+        hipLaunchKernelGGL(k_join_chunks<T>, dim3((unsigned)gx, (unsigned)gs::cdiv(p.chunks, gx)), dim3(threads), 0, stream, (const uint32_t*)keys, tokens, V, D, jl, gs::cdiv(vectors, 1ll << jl),
                            wide ? CHUNK + 1 : 1, scale, (const float*)first, (const float*)last, (T*)dw);
     }
     GS_LAUNCH_CHECK();
@@ -596,6 +597,7 @@ extern "C" int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64
     if (V == 0 || D == 0) return 0;
     GS_REQUIRE(dw && (T == 0 || (ids && g && ldg >= 0)), "gs_embedding_bwd: null argument");
     GS_REQUIRE(workspace && workspace_bytes >= sort_plan(T, D).total, "gs_embedding_bwd: workspace too small");
+    GS_REQUIRE(((uintptr_t)workspace & 15) == 0, "gs_embedding_bwd: the workspace must start on 16 bytes");
     const auto run = dtype == 0 ? (ids64 ? gradient<float, int64_t> : gradient<float, int32_t>) : dtype == 1 ? (ids64 ? gradient<bf16, int64_t> : gradient<bf16, int32_t>)
                                                                                              : (ids64 ? gradient<f16, int64_t> : gradient<f16, int32_t>);
     return run(ids, g, ldg, T, V, D, padding_idx, scale, dw, (char*)workspace, (hipStream_t)stream);

@@ -230,6 +230,7 @@ extern "C" int gs_grad_norm(int n_tensors, const void* const* grads, void* const
     try {          // the lists on the host may not fit
         GS_REQUIRE(!out || !overlap(n_tensors, grads, out, numel, dtypes), "gs_grad_norm: an output shares memory with another output or another gradient");
         GS_REQUIRE(workspace && workspace_bytes >= gs_grad_norm_workspace_bytes(n_tensors), "gs_grad_norm: workspace too small");
+        GS_REQUIRE(((uintptr_t)workspace & 7) == 0, "gs_grad_norm: the workspace must start on 8 bytes");
         const auto go = norm_type == 0 ? run<NORM_2> : norm_type == 1 ? run<NORM_1> : run<NORM_INF>;
         return go(n_tensors, grads, out, numel, dtypes, max_norm, norm, (double*)workspace, (hipStream_t)stream);
     } catch (const std::bad_alloc&) {

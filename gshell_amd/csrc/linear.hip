@@ -40,6 +40,9 @@ template <> __device__ __forceinline__ f32x4 mfma<f16>(s16x8 a, s16x8 b, f32x4 c
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// g act'(z).  Where the derivative is exactly zero nothing passes, an infinity or NaN neither.
+__device__ __forceinline__ float gated(float g, float d) { return d == 0.f ? 0.f : g * d; }
+
 // Value and derivative of the activation, on the hardware's exp2, log2 and reciprocal (1 ulp each).  For 16-bit layers (FAST) the exponent's product is rounded, and
 // erfc is Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7): far below the rounding of the result.  For fp32 the product's rounding error goes into the
 // exponential as a factor, and erfc is the library's.
@@ -471,19 +474,23 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
             float t = 0.f;
 #pragma unroll
             for (int q = 0; q < 256 / LINES; ++q) t += lds.out[threadIdx.x + q * LINES];
+            if (GATE && !(fabsf(t) < __builtin_inff())) {          // again, as gated() has it
+                t = 0.f;
+                for (int64_t c = c_begin; c < c_end; ++c) t += gated(A.p[c * A.ld + i0 + threadIdx.x], gate[c * ldgate + i0 + threadIdx.x]);
+            }
             column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = t;
         }
         __syncthreads();
     }
     const auto fix = [&](int64_t i, int64_t j, auto& z) {
-        // a sum that is not finite is done again without the split, in fp32
+        // a sum that is not finite is done again without the split, in fp32, and with gated()
 #pragma unroll 1
         for (int k = 0; k < 4; ++k)
             if (!(fabsf(z[k]) < __builtin_inff()) && j + k < N) {
                 float t = 0.f;
                 for (int64_t c = c_begin; c < c_end; ++c) {
                     float a = ACOLS ? A.p[c * A.ld + i] : A.p[i * A.ld + c];
-                    if (GATE) a *= ACOLS ? gate[c * ldgate + i] : gate[i * ldgate + c];
+                    if (GATE) a = gated(a, ACOLS ? gate[c * ldgate + i] : gate[i * ldgate + c]);
                     t = fmaf(a, BCOLS ? B.p[c * B.ld + j + k] : B.p[(j + k) * B.ld + c], t);
                 }
                 z[k] = t;
@@ -910,7 +917,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_prepare(Gz<T> G, 
             if (G.dact) {
                 load_some<typename dact_type<T>::type, V>(G.dact + m * G.N + j, in_row, d);
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[k] *= d[k];
+                for (int k = 0; k < V; ++k) v[k] = gated(v[k], d[k]);
             }
             if (G.gz) store_some<T, V>(G.gz + m * G.ldgz + j, V, v);
 #pragma unroll
@@ -936,6 +943,7 @@ template <typename T> __global__ void __launch_bounds__(1024) k_join_columns(Col
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
 constexpr int CUS = 256;
+constexpr int64_t MAX_TILES = (1ll << 32) / 256 - 1;          // a launch has fewer than 2^32 lanes
 static int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
@@ -964,6 +972,7 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
         const double slow = columns == 0 ? 1.05 : columns == 1 ? 1.2 : 1.5;
         for (int r = 64; r <= TILE; r += 64) {
             const int64_t t = tiles(r, r), most = r == 64 ? 4 : 2;
+            if (r == 64 && t >= MAX_TILES) continue;
             for (int64_t a_unit = 0; a_unit <= most; a_unit = a_unit ? 2 * a_unit : 1) {
                 int64_t s = a_unit ? a_unit * CUS / t : 1;          // as many slices as fill the chip with a_unit workgroups each, or one
                 if (a_unit && s > steps / 8) s = steps / 8;
@@ -1018,7 +1027,7 @@ template <typename T> int64_t repack(Pack2<T>& P, int q, Line& a, int64_t rows, 
 }
 template <typename T> int prepare(const Gz<T>& G, const Pack2<T>& P, hipStream_t stream) {
     const uint64_t blocks = (uint64_t)G.blocks + P.blocks[0] + P.blocks[1];
-    GS_REQUIRE(blocks < (1ull << 31), "gs_linear: operands too large for one launch");
+    GS_REQUIRE(blocks <= (uint64_t)MAX_TILES, "gs_linear: operands too large for one launch");
     if (blocks) hipLaunchKernelGGL(k_prepare<T>, dim3((unsigned)blocks), dim3(256), 0, stream, G, P);
     return 0;
 }
@@ -1035,7 +1044,7 @@ int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilo
     if (M == 0 || N == 0) return 0;
     const Plan p = plan(sizeof(T), ACOLS + BCOLS, M, N, K, db != nullptr);
     GS_REQUIRE(ws_bytes >= p.bytes, "gs_linear: workspace too small");
-    GS_REQUIRE(p.tiles + (int64_t)columns.blocks < (1ll << 31) && M * gs::cdiv(N, 4) < (31ll << 31), "gs_linear: too many tiles");
+    GS_REQUIRE(p.tiles + (int64_t)columns.blocks <= (p.rows == 256 || p.deep ? MAX_TILES / 2 : MAX_TILES), "gs_linear: too many tiles for one launch");
     Epilogue<T> first = E;
     first.part = p.splits > 1 ? (float*)ws : nullptr;
     Columns<T> none{}, beside = none;
@@ -1071,7 +1080,7 @@ int product(const Line& a, const Line& b, int64_t M, int64_t N, int64_t K, Epilo
 }
 
 // k_rows: at most 32 rows, and where its workgroups of 16 columns do not fill the chip slices of the contraction, each of one round of the waves or more
-constexpr int64_t FEW_ROWS = 32;
+static bool few_rows(int64_t M, int64_t N) { return M <= 32 && N <= MAX_TILES * 8; }
 static Plan rows_plan(int64_t M, int64_t N, int64_t K) {
     Plan p;
     p.cols = gs::cdiv(N, 32) >= CUS ? 32 : 16;          // x is read by every workgroup: twice the columns where that leaves a workgroup for each compute unit
@@ -1103,7 +1112,7 @@ int product_rows(const Line& x, const Line& w, int64_t M, int64_t N, int64_t K, 
 }
 
 static int64_t forward_bytes(int es, const Line& x, const Line& w, int64_t M, int64_t N, int64_t K) {
-    if (M <= FEW_ROWS) return rows_plan(M, N, K).bytes;
+    if (few_rows(M, N)) return rows_plan(M, N, K).bytes;
     return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, 0, M, N, K, false).bytes;
 }
 
@@ -1113,9 +1122,10 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
     Line lx{x, ldx, K, false}, lw{w, ldw, K, false};
     const int64_t need = forward_bytes(sizeof(T), lx, lw, M, N, K);
     GS_REQUIRE(ws_bytes >= need && (ws || need == 0), "gs_linear_fwd: workspace too small");
+    GS_REQUIRE(((uintptr_t)ws & 15) == 0, "gs_linear_fwd: the workspace must start on 16 bytes");
     char* at = (char*)ws;
     Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta * 1.44269504f, act == ACT_SOFTPLUS ? 2.f / beta : 0.f};
-    if (M <= FEW_ROWS) return product_rows<T>(lx, lw, M, N, K, E, at, stream);
+    if (few_rows(M, N)) return product_rows<T>(lx, lw, M, N, K, E, at, stream);
     Pack2<T> P{};
     at += repack<T>(P, 0, lx, M, at);
     at += repack<T>(P, 1, lw, N, at);
@@ -1159,6 +1169,7 @@ int linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, int6
     Line gz{g, ldg, N, false}, lx{x, ldx, K, false}, lw{w, ldw, K, false};
     const BackwardPlan p = backward_plan(gz, dact != nullptr, lx, lw, M, N, K, sizeof(T), dx != nullptr, dw != nullptr, db != nullptr);
     GS_REQUIRE(ws_bytes >= p.total && (ws || p.total == 0), "gs_linear_bwd: workspace too small");
+    GS_REQUIRE(((uintptr_t)ws & 15) == 0, "gs_linear_bwd: the workspace must start on 16 bytes");
     if (N == 0 && K == 0) return 0;
     char* base = (char*)ws;
     Gz<T> G{};
@@ -1213,7 +1224,7 @@ extern "C" int gs_linear_fwd(const void* x, int64_t ldx, const void* weight, int
     GS_REQUIRE(act != ACT_SOFTPLUS || (beta > 0.f && beta < 1e30f), "gs_linear_fwd: softplus needs a positive finite beta");
     if (M == 0 || N == 0) return 0;
     GS_REQUIRE(y && ldy >= N && (!residual || ldr >= 0), "gs_linear_fwd: null output or row stride smaller than a row");
-    GS_REQUIRE(K == 0 || (x && weight && ldx >= 0 && ldw >= 0), "gs_linear_fwd: null operand");
+    GS_REQUIRE(K == 0 || (x && weight && ldx >= 0 && ldw >= 0), "gs_linear_fwd: null operand or negative row stride");
     const auto run = dtype == DT_F32 ? linear_fwd<float> : dtype == DT_BF16 ? linear_fwd<bf16> : linear_fwd<f16>;
     return run(x, ldx, weight, ldw, bias, residual, ldr, M, N, K, act, beta, y, ldy, dact, workspace, workspace_bytes, (hipStream_t)stream);
 }
@@ -1229,7 +1240,7 @@ extern "C" int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const
     GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_linear_bwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     GS_REQUIRE(sizes_ok(M, N, K, dtype), "gs_linear_bwd: sizes are 0 .. 2^31 - 1, of 16-bit rows 0 .. 2^21 - 1");
     GS_REQUIRE(M == 0 || N == 0 || (g && ldg >= 0), "gs_linear_bwd: null gradient");
-    GS_REQUIRE(M == 0 || N == 0 || K == 0 || ((!dx || weight) && (!dw || x)), "gs_linear_bwd: null operand");
+    GS_REQUIRE(M == 0 || N == 0 || K == 0 || ((!dx || (weight && ldw >= 0)) && (!dw || (x && ldx >= 0))), "gs_linear_bwd: null operand or negative row stride");
     const auto run = dtype == DT_F32 ? linear_bwd<float> : dtype == DT_BF16 ? linear_bwd<bf16> : linear_bwd<f16>;
     return run(g, ldg, dact, x, ldx, weight, ldw, M, N, K, dx, dw, db, workspace, workspace_bytes, (hipStream_t)stream);
 }

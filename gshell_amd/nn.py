@@ -157,7 +157,7 @@ def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
     activation: None, "relu", "softplus" (log(1 + exp(beta z)) / beta), "silu" or "gelu" (erf form).  The residual is added behind the activation and has the
     output's shape (an expanded view may stand for it).  All operands have one type (float32, bfloat16, float16) and one device; x, weight and residual may be views whose rows are
     any stride apart.  fp32 operands keep fp32's accuracy.  Where the gradient is taken of an activation, act'(z) is kept for the backward pass: 2 bytes an output
-    for bf16, 4 for the others."""
+    for bf16, 4 for the others; where it is exactly zero (relu of z <= 0) nothing passes, an infinite gradient neither."""
     act = ACTIVATIONS.get(activation)
     beta = float(beta)
     dtype, device, xs, ws = x.dtype, x.get_device(), x.shape, weight.shape
@@ -287,5 +287,17 @@ class Embedding(torch.nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, device=device, dtype=dtype)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, embeddings, freeze=True, padding_idx=None, scale=1.0):
+        """A table with the rows of `embeddings` [V, D], which it shares; frozen unless told otherwise."""
+        if embeddings.dim() != 2:
+            raise GShellHipError(f"Embedding: rows [V, D] are wanted, got {tuple(embeddings.shape)}")
+        table = cls(*embeddings.shape, padding_idx=padding_idx, scale=scale, device="meta", dtype=embeddings.dtype)
+        table.weight = torch.nn.Parameter(embeddings, requires_grad=not freeze)
+        return table
+
     def forward(self, ids):
         return embedding(ids, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", scale={self.scale}"

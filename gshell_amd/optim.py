@@ -154,7 +154,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)) -> norm, one fp32 value on the device.  Without `out`, in place.
 
     `out`: tensors of the gradients' shapes and types; one may be its gradient's own place, otherwise no output shares memory with a gradient or another output (such a
-    call is refused).  A norm that is NaN makes every output NaN, one that is infinite makes finite elements zero."""
+    call is refused; of outputs that are not contiguous the same one twice).  A norm that is NaN makes every output NaN, one that is infinite makes finite elements zero."""
     code = _norm_code(norm_type, "clip_grads")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -174,6 +174,9 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         _check_grads(out, "clip_grads")
         if out[0].get_device() != grads[0].get_device():
             raise _lib.GShellHipError(f"clip_grads: gradients are on {grads[0].device}, outputs on {out[0].device}")
+    apart = [o.data_ptr() for o in out if not o.is_contiguous()]          # written from copies, one after the other
+    if len(set(apart)) != len(apart):
+        raise _lib.GShellHipError("clip_grads: the same output twice")
     src = [g if g.is_contiguous() else g.contiguous() for g in grads]
     dst = src if out is grads else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in out]
     norm = _launch_norm(src, dst, types, max_norm, code)

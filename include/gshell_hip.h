@@ -862,8 +862,8 @@ int gs_flexi_cut_bwd(const int64_t* pa, const int64_t* pb, int64_t n, const floa
  *   log(1 + exp(beta z)) / beta, 3 silu, 4 gelu (erf form).  bias, residual may be null.
  *   dact [M,N] (contiguous; fp16 for bf16 layers, fp32 otherwise; null = not wanted) receives act'(z) for gs_linear_bwd.
  *   gs_linear_bwd: gz = g act'(z) -> dx = gz W [M,K], dW = gz^T x [N,K], db = column sums of gz; any of the three may be null.
- *   dact null = no activation.  M, N, K < 2^31; N, K < 2^21 for 16-bit layers.  Sums are taken in a fixed order: the same bits every time.
- *   The workspaces are the caller's and hold nothing between calls; their sizes go by the addresses and strides too (16-bit operands
+ *   dact null = no activation; where act'(z) is exactly zero nothing passes, whatever g is.  M, N, K < 2^31; N, K < 2^21 for 16-bit layers.  Sums are taken in a fixed order: the same bits every time.
+ *   The workspaces are the caller's, start on 16 bytes and hold nothing between calls; their sizes go by the addresses and strides too (16-bit operands
  *   whose rows do not start on 16 bytes are repacked first).
  * ---------------------------------------------------------------------------------- */
 int64_t gs_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* weight, int64_t ldw, int64_t M, int64_t N, int64_t K,
@@ -882,7 +882,7 @@ int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, i
  *   fwd: y [T,D] = scale * weight[ids], weight [V,D] with rows ldw elements apart; ids int64 (ids64 = 1) or int32.
  *   bwd: dw [V,D] (written whole, unnamed rows zero) = scale * sum of g's rows (ldg apart) by id, in the order of the tokens, in 32 bits: the same
  *        bits every time.  padding_idx: a row without gradient (-1: none).  An id outside [0, V) gives a NaN row and no gradient.
- *   dtype as for gs_linear_fwd.
+ *   dtype as for gs_linear_fwd; the workspace starts on 16 bytes.
  * ---------------------------------------------------------------------------------- */
 int gs_embedding_fwd(const void* ids, int ids64, const void* weight, int64_t ldw, int64_t T, int64_t V, int64_t D, int dtype,
                      float scale, void* y, gs_stream_t stream);
