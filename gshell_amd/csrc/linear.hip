@@ -328,16 +328,19 @@ template <bool COLS, bool GATE, int LINES> struct Feed32 {
     __device__ __forceinline__ void fetch(int64_t c, Values& V) const {
         const bool all = whole && c + BK <= c_end;
         if constexpr (!COLS) {
+            const auto some = [&](auto left_of) __attribute__((always_inline)) {
 #pragma unroll
-            for (int h = 0; h < PIECES; ++h) {
-                const int64_t l = line0 + line_of(h), at = c + at_of(h);
-                const int64_t left = all ? 8 : l < lines ? c_end - at : 0;
+                for (int h = 0; h < PIECES; ++h) {
+                    const int64_t l = line0 + line_of(h), at = c + at_of(h), left = left_of(l, at);
 #pragma unroll
-                for (int k = 0; k < 8; k += 4) {
-                    load_some<float, 4>(p + l * ld + at + k, left - k, *(float(*)[4])(V.v + 8 * h + k));
-                    if constexpr (GATE) load_some<float, 4>(gate + l * ldgate + at + k, left - k, *(float(*)[4])(V.d + 8 * h + k));
+                    for (int k = 0; k < 8; k += 4) {
+                        load_some<float, 4>(p + l * ld + at + k, left - k, *(float(*)[4])(V.v + 8 * h + k));
+                        if constexpr (GATE) load_some<float, 4>(gate + l * ldgate + at + k, left - k, *(float(*)[4])(V.d + 8 * h + k));
+                    }
                 }
-            }
+            };
+            if (all) some([](int64_t, int64_t) { return (int64_t)8; });
+            else some([&](int64_t l, int64_t at) { return l < lines ? c_end - at : 0; });
         } else {
             const int64_t at = c + __builtin_amdgcn_readfirstlane(at_of(0));          // the same for a wave
             const uint32_t l = threadIdx.x % LINES;
