@@ -3,7 +3,8 @@
 //
 //     y_t = s W[id_t]                      dW_v = s sum_{t: id_t = v} g_t   (rows that no id names: zero)
 //
-// The gradient's sums run over the tokens of a row in their order, in 32 bits, and do not depend on how the launch is scheduled: the tokens are sorted by row
+// The gradient's sums are 32-bit, in an order that does not depend on how the launch is scheduled.  Tables of few, narrow rows: partial tables in LDS, added up in their order
+// (k_sum_few).  Others: the tokens are sorted by row
 // (a stable radix sort of our own), then every CHUNK neighbours of the sorted list are summed by one group of lanes.  A run of equal rows inside a chunk is written at once;
 // one that crosses chunks leaves a part in each and is joined in a second launch, so that a row that holds most of the tokens is spread over the chip as well.
 // No atomics, no pass over the table but the one that writes it.
@@ -213,7 +214,9 @@ template <typename T, int VEC, typename U> __device__ __forceinline__ void store
 // Forward: the output is one stretch of memory, written 16 aligned bytes a lane and piece; LOOKUPS pieces a lane are on their way together.  A piece inside a row is one load (at
 // whatever address the row has it), one that runs over a row's end is gathered.  The place of a lane's next piece comes without a division: step_rows, step_cols are
 // what a workgroup's pieces of one round cover.
-constexpr int LOOKUPS = 4;
+// Bound by memory: 65536 rows of 1024 bf16 out of 50000 44 us (134 MB written, 32 MB of different rows read), 262144 of 32 fp32 10 us; 8 rows of 4096 3.2 us, a launch.  One piece a
+// lane 47, 9.8 and 2.7 us, four 46, 9.9 and 3.4, eight 57, 10.7 and 5.0.
+constexpr int LOOKUPS = 2;
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) k_lookup(const I* ids, const T* w, int64_t ldw, int64_t tokens, int64_t V, int64_t D, int64_t step_rows, int64_t step_cols, float scale, T* y) {
     constexpr int VEC = 16 / sizeof(T);
@@ -292,7 +295,8 @@ template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t*
 
 // Rows of more than 32 vectors of 16 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
 // eight rows are on their way at a time.  A run of up to CHUNK tokens is summed as a whole by the chunk where it begins; a longer one leaves a part in each of its chunks.
-// 65536 tokens of 1024 bf16 over 50000 rows: see the table of measurements beside the host code.
+// Bound by memory: 65536 tokens of 1024 bf16, their numbers spread like 1 / n over 50000 rows: 67 us for 134 MB of gradient, 102 MB of table and the long runs' parts
+// (3.5 TB/s), evenly spread 59 us.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t stretches,
                                                   int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const ui
     }
 }
 
-// Narrower rows: several groups of lanes a wave, a chunk each; every run that crosses chunks leaves its parts.  Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
+// Narrower rows: several groups of lanes a wave, a chunk each, 25 us for 262144 tokens of 64 bf16 over 160 rows; every run that crosses chunks leaves its parts.  Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int group_log,
                                                     int64_t stretches, int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
@@ -462,11 +466,85 @@ __global__ void __launch_bounds__(1024) k_join_chunks(const uint32_t* keys, int6
     }
 }
 
+// Tables of few and narrow rows: no sort.  Each group of lanes (as many as a row has columns) keeps a table of its own in LDS and adds every groups-th token of the workgroup's
+// stretch to it, a lane a column; tokens without a row go to one more behind the last.  A place belongs to one lane, which reads, adds and writes it in the tokens' order: the
+// sums are the same every time (LDS's float atomics need twice the time of these).  The tables are added up in their order, the workgroups' sums in a second launch
+// (`part`; null: there is one workgroup, which writes dw).  Bound by the chain through LDS, a token at a time for each of a compute unit's 16 .. 512 groups.
+constexpr int FEW_FLOATS = 40960, FEW_AHEAD = 8;          // all of a compute unit's LDS; tokens of a group that are on their way together
+template <typename T, typename I>
+__global__ void __launch_bounds__(512) k_sum_few(const I* ids, const T* g, int64_t ldg, int64_t tokens, int64_t per, int V, int D, int64_t padding, int group_log, float scale, T* dw, float* part) {
+    __shared__ float tables[FEW_FLOATS];
+    const int size = V * D, whole = size + D, groups = blockDim.x >> group_log, group = threadIdx.x >> group_log, lane = threadIdx.x & ((1 << group_log) - 1);
+    for (int e = threadIdx.x; e < whole * groups; e += blockDim.x) tables[e] = 0.f;
+    __syncthreads();
+    const int64_t t0 = (int64_t)blockIdx.x * per, t1 = t0 + per < tokens ? t0 + per : tokens;
+    if (lane < D) {
+        float* mine = tables + group * whole + lane;
+        const T* column = g + lane;
+        int64_t t = t0 + group;
+        for (; t + (FEW_AHEAD - 1) * groups < t1; t += FEW_AHEAD * groups) {
+            I id[FEW_AHEAD];
+            T v[FEW_AHEAD];
+#pragma unroll
+            for (int k = 0; k < FEW_AHEAD; ++k) id[k] = ids[t + k * groups], v[k] = column[(t + k * groups) * ldg];
+#pragma unroll
+            for (int k = 0; k < FEW_AHEAD; ++k) mine[(int)key_of(id[k], V, padding) * D] += (float)v[k];
+        }
+        for (; t < t1; t += groups) mine[(int)key_of(ids[t], V, padding) * D] += (float)column[t * ldg];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < size; e += blockDim.x) {
+        float s = 0.f;
+        for (int q = 0; q < groups; ++q) s += tables[q * whole + e];
+        if (part) part[(int64_t)blockIdx.x * size + e] = s;
+        else dw[e] = (T)(s * scale);
+    }
+}
+// 32 elements a workgroup, the parts in eight stretches side by side
+template <typename T> __global__ void __launch_bounds__(256) k_join_few(const float* part, int parts, int size, float scale, T* dw) {
+    __shared__ float sums[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, e = blockIdx.x * 32 + x, share = (parts + 7) / 8, k0 = y * share, k1 = k0 + share < parts ? k0 + share : parts;
+    float s = 0.f;
+    if (e < size)
+        for (int k = k0; k < k1; k += 8) {
+            float q[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) q[u] = k + u < k1 ? part[(int64_t)(k + u) * size + e] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += q[u];
+        }
+    sums[y][x] = s;
+    __syncthreads();
+    if (y > 0 || e >= size) return;
+    for (int q = 1; q < 8; ++q) s += sums[q][x];
+    dw[e] = (T)(s * scale);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------------------------------
 static int group_log_of(int64_t vectors) {          // lanes, as a power of two, of a group that takes a row or a stretch of one
     int l = 0;
     while (l < 6 && (1ll << l) < vectors) ++l;
     return l;
+}
+
+// Whether a table counts as one of few, narrow rows: at most 64 columns, and the tables of 256 lanes' groups fit in LDS; then twice the lanes where theirs do, and workgroups for
+// the chip.  fp32, lookup and gradient: 262144 tokens over 72 x 32 26 us, sorted 54; over 140 x 64 54, sorted 59; 2 million over 150 x 8 49, sorted 181; 256 over 72 x 32 13,
+// sorted 25.  With more than 64 columns, in stretches of 64: 262144 over 14 x 200 117, sorted 153, but over 70 x 130 132, sorted 116, and over 9 x 1024 689, sorted 584.
+struct FewPlan {
+    int threads = 0, group_log = 0;          // no threads: it does not
+    int64_t blocks = 0, per = 0, bytes = 0;
+};
+static FewPlan few_plan(int64_t T, int64_t V, int64_t D) {
+    FewPlan p;
+    if (T == 0 || V > FEW_FLOATS || D > 64) return p;
+    p.group_log = group_log_of(D);
+    if ((V + 1) * D * (256 >> p.group_log) > FEW_FLOATS) return p;
+    p.threads = (V + 1) * D * (512 >> p.group_log) > FEW_FLOATS ? 256 : 512;
+    const int64_t round = (int64_t)(p.threads >> p.group_log) * FEW_AHEAD, rounds = gs::cdiv(T, round);
+    p.per = gs::cdiv(rounds, rounds < 256 ? rounds : 256) * round;
+    p.blocks = gs::cdiv(T, p.per);
+    p.bytes = p.blocks > 1 ? p.blocks * V * D * 4 : 0;
+    return p;
 }
 
 struct SortPlan {
@@ -534,6 +612,13 @@ template <typename I> int sort_tokens(const void* ids, int64_t T, int64_t V, int
 
 template <typename T, typename I>
 int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t padding, float scale, void* dw, char* base, hipStream_t stream) {
+    if (const FewPlan f = few_plan(tokens, V, D); f.threads) {
+        float* part = f.blocks > 1 ? (float*)base : nullptr;
+        hipLaunchKernelGGL((k_sum_few<T, I>), dim3((unsigned)f.blocks), dim3(f.threads), 0, stream, (const I*)ids, (const T*)g, ldg, tokens, f.per, (int)V, (int)D, padding, f.group_log, scale, (T*)dw, part);
+        if (part) hipLaunchKernelGGL(k_join_few<T>, dim3((unsigned)gs::cdiv(V * D, 32)), dim3(256), 0, stream, (const float*)part, (int)f.blocks, (int)(V * D), scale, (T*)dw);
+        GS_LAUNCH_CHECK();
+        return 0;
+    }
     const SortPlan p = sort_plan(tokens, D);
     uint32_t *keys = nullptr, *pos = nullptr;
     if (tokens > 0)
@@ -576,6 +661,11 @@ static bool sizes_ok(int64_t T, int64_t V, int64_t D) {
     return T >= 0 && V >= 0 && D >= 0 && T < top && V < top && D < top;
 }
 
+static int64_t bytes_of(int64_t T, int64_t V, int64_t D) {
+    const FewPlan f = few_plan(T, V, D);
+    return f.threads ? (f.bytes > 16 ? f.bytes : 16) : sort_plan(T, D).total;
+}
+
 }  // namespace
 
 extern "C" int gs_embedding_fwd(const void* ids, int ids64, const void* weight, int64_t ldw, int64_t T, int64_t V, int64_t D, int dtype, float scale, void* y, gs_stream_t stream) {
@@ -588,7 +678,7 @@ extern "C" int gs_embedding_fwd(const void* ids, int ids64, const void* weight, 
     return run(ids, weight, ldw, T, V, D, scale, y, (hipStream_t)stream);
 }
 
-extern "C" int64_t gs_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) { return sizes_ok(T, V, D) ? sort_plan(T, D).total : -1; }
+extern "C" int64_t gs_embedding_bwd_workspace_bytes(int64_t T, int64_t V, int64_t D) { return sizes_ok(T, V, D) ? bytes_of(T, V, D) : -1; }
 
 extern "C" int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64_t ldg, int64_t T, int64_t V, int64_t D, int64_t padding_idx, int dtype, float scale, void* dw,
                                 void* workspace, int64_t workspace_bytes, gs_stream_t stream) {
@@ -596,7 +686,7 @@ extern "C" int gs_embedding_bwd(const void* ids, int ids64, const void* g, int64
     GS_REQUIRE(dtype >= 0 && dtype <= 2, "gs_embedding_bwd: dtype is 0 (fp32), 1 (bf16) or 2 (fp16)");
     if (V == 0 || D == 0) return 0;
     GS_REQUIRE(dw && (T == 0 || (ids && g && ldg >= 0)), "gs_embedding_bwd: null argument");
-    GS_REQUIRE(workspace && workspace_bytes >= sort_plan(T, D).total, "gs_embedding_bwd: workspace too small");
+    GS_REQUIRE(workspace && workspace_bytes >= bytes_of(T, V, D), "gs_embedding_bwd: workspace too small");
     GS_REQUIRE(((uintptr_t)workspace & 15) == 0, "gs_embedding_bwd: the workspace must start on 16 bytes");
     const auto run = dtype == 0 ? (ids64 ? gradient<float, int64_t> : gradient<float, int32_t>) : dtype == 1 ? (ids64 ? gradient<bf16, int64_t> : gradient<bf16, int32_t>)
                                                                                              : (ids64 ? gradient<f16, int64_t> : gradient<f16, int32_t>);

@@ -53,6 +53,25 @@ def test_runs(kind, T, what):
     check_one(ids, V, D, TYPES[kind], 2.0, None, T)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T", [40, 2000, 5000])
+@pytest.mark.parametrize("what", ["one row", "two rows", "ends of chunks", "sorted", "reversed", "last row"])
+@pytest.mark.parametrize("V,D", [(1500, 20), (1500, 270)])
+def test_runs_in_larger_tables(kind, T, what, V, D):
+    at = torch.arange(T)
+    ids = {"one row": torch.full((T,), 17), "two rows": at % 2, "ends of chunks": torch.clamp(at // 32, max=V - 1), "sorted": (at * V) // T, "reversed": V - 1 - (at * V) // T,
+           "last row": torch.full((T,), V - 1)}[what]
+    check_one(ids, V, D, TYPES[kind], 2.0, None, T)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T,V,D", [(1, 1, 1), (9, 160, 1), (5000, 160, 1), (5000, 161, 1), (700, 80, 32), (700, 160, 32), (700, 161, 32), (9000, 160, 64), (9000, 10, 1024), (300, 5, 2048), (40, 1, 9000),
+                                   (100000, 2, 3), (131072, 72, 33)])
+def test_around_what_counts_as_few_rows(kind, T, V, D):
+    gen = torch.Generator().manual_seed(T + V)
+    check_one(torch.randint(-1, V + 1, (T,), generator=gen).clamp_(0, V - 1), V, D, TYPES[kind], 0.5, V // 2 if V > 2 else None, T)
+
+
 def test_shapes_types_of_ids_and_repeatability():
     from gshell_amd import nn
     gen = torch.Generator().manual_seed(1)
