@@ -663,7 +663,7 @@ static bool sizes_ok(int64_t T, int64_t V, int64_t D) {
 
 static int64_t bytes_of(int64_t T, int64_t V, int64_t D) {
     const FewPlan f = few_plan(T, V, D);
-    return f.threads ? (f.bytes > 16 ? f.bytes : 16) : sort_plan(T, D).total;
+    return f.threads ? align256(f.bytes + 1) : sort_plan(T, D).total;
 }
 
 }  // namespace

@@ -8,8 +8,9 @@
 // ("columns"): y = (x rows, W rows), dx = (gz rows, W columns), dW = (gz columns, x columns).  Products run on the matrix cores with 32-bit sums.
 // fp32 operands are split into three bf16 parts, x = x1 + x2 + x3 (each part the rounding of what the ones before left: 24 bits and more in all,
 // and bf16 has fp32's exponents), and six products are summed, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1; the three left out are below
-// 2^-25 |x y| each.  That is 6 / 16 of the bf16 rate, where the fp32 matrix instruction has 1 / 16.  An infinity has no such split (inf * 0): a sum
-// that comes out non-finite is done again with fp32 multiply-adds.
+// 2^-25 |x y| each.  That is 1 / 6 of the bf16 rate, where the fp32 matrix instruction has 1 / 16.  An infinity has no such split (inf * 0): a sum
+// that comes out non-finite is done again with fp32 multiply-adds (131072 x 256 x 256 of nothing but NaN: 15 ms).  The matrix cores take parts below 2^-126 as zero: operands
+// below 2^-112 keep fewer bits, 2^-17 at 2^-118.
 #include <hip/hip_runtime.h>
 
 #include "../../include/gshell_hip.h"
@@ -293,6 +294,10 @@ template <typename T> __device__ __forceinline__ void join_columns(const Columns
 // fall on distinct banks.
 //   rows operand     a lane loads 8 neighbours of the contraction at a time; columns operand: 16 or 8 of one line, neighbouring lanes neighbouring lines
 // A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
+// 131072 x 256 x 256: y 119 us (144 Tflop/s; the library's fp32 product 155), with softplus and act' kept 171; dx 122 (145), with a gate 168; dW 107 (319), with a gate and db 134.
+// 4096 x 4096 x 4096: 790, 650, 690 us (1040).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (55 us of dx, 80 of y with
+// softplus, by leaving it out) share a compute unit and overlap in part.  Tried and left: the weight's parts made once by a launch of their own and loaded straight into LDS, 165
+// + 5 us of 184 for dx and 180 + 5 of 184 for y; workgroups that start a quarter of a tile apart, no change.
 constexpr int TILE = 128, BK = 32;
 
 __device__ __forceinline__ short raw(bf16 v) { return __builtin_bit_cast(short, v); }
@@ -518,6 +523,9 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
 //   columns operand  LDS holds [64][line]; fragments come out transposed by ds_read_b64_tr_b16 (4 contraction rows x 16 lines a 16-lane group); the 32-byte
 //                    piece q of row k sits at q ^ h(k), with h different for the 16 rows that one instruction reads
 // Lines and contraction beyond the operand are loaded as zero (an offset outside of the buffer's range).
+// 16384 x 4096 x 4096 bf16 with 256 x 256 tiles: y 511 us (1.08 Pflop/s; the library 448), with gelu, residual and act' kept 540; dx 500 (522), dW 442 .. 484 (577).  Four tiles a
+// compute unit: what is left is their starts and ends, 15 us each, in which the matrix cores wait; the clock falls with them busy, so less waiting gains less than it
+// takes away.  The next lines' residual loaded ahead in the epilogue: 588 us for 577.  4096 x 2048 x 2048 with 128 x 128 tiles: 39, 40, 41 us (36, 38, 50).
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int STEP = 64;
 constexpr uint32_t OUTSIDE = 0x80000000u;          // every buffer's range: an offset of this size is outside, a tile's own offsets are below
@@ -663,6 +671,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Opera
 
 // The same product where the tiles do not fill the chip and latency is what counts: one workgroup a compute unit, tiles of BM x 128, four buffers, so that three steps are
 // on their way while one is multiplied, and twice the waves: each 64 x 64 of the tile is done by two of them, one for either half of a step, whose sums are added in the end.
+// 2048 x 2048 x 2048 bf16: y 20.5 us, dx 23, dW 24 (the library 23, 27, 30); 1000 x 1000 x 1000 fp16 10, 11, 11 (21, 20, 22); 512 x 4096 x 4096 27, 37, 24 (27, 35, 27).
 // Every step loads and reads ahead, behind the end too (nothing but zeros comes from there): without branches the compiler sees which loads a read waits for.
 template <typename T, bool ACOLS, bool BCOLS, int BM>
 __global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand<T> B, int64_t M, int64_t N, int64_t lines_a, int64_t lines_b, int64_t K, int64_t slice, Epilogue<T> E, Columns<T> C) {
@@ -757,6 +766,7 @@ __global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand
 // CHUNK, and fragments come straight from memory: each matrix instruction takes 16 bytes a lane of 16 rows of W, so W is read once, with nothing staged, and the loads of the
 // next stretch are on their way while one is multiplied.  16-bit: one instruction a load; fp32: the fp32 matrix instruction four times (its rate does not matter here, and it
 // rounds like a chain of fused multiply-adds).  The waves' sums meet in LDS.
+// 1 x 4096 x 4096 bf16 9.7 us, 24 rows of 8192 -> 2048 fp16 with bias and silu 10.2: 33.6 MB, 6.5 us of a large copy's rate, and a launch; all of W is asked for at once.
 constexpr int ROWS_THREADS = 512, ROWS_WAVES = ROWS_THREADS / 64;
 template <typename T, int MT, int NT>
 __global__ void __launch_bounds__(ROWS_THREADS) k_rows(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<T> E) {
@@ -877,7 +887,7 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
 }
 
 // What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type, in rows that start on 16 bytes with zeros behind their ends, and its
-// column sums (of the unrounded values) by slabs of rows.  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
+// column sums (of the unrounded values) by slabs of rows: 16384 x 4096 bf16 73 us, 402 MB at 5.5 TB/s.  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
 constexpr int GZ_LANES = 32, GZ_LINES = 8;
 template <typename T> struct Gz {
     const T* g;
