@@ -86,6 +86,7 @@ class HipAdam(torch.optim.Adam):
 
 
 _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_group_tensors = torch._C._group_tensors_by_device_and_dtype
 _NORM_TYPES = {2.0: 0, 1.0: 1, float("inf"): 2}
 
 
@@ -107,13 +108,29 @@ def _refuse_grads(tensors, what):
             raise _lib.GShellHipError(f"{what}: tensors are on {tensors[0].device} and on {t.device}")
 
 
-def _check_grads(tensors, what):
-    """Type codes of `tensors`: dense, on one device, of known types -- on the host, before anything is launched."""
+def _check_grads(tensors, what, out=None):
+    """Type codes of `tensors` (and of `out`): dense, on one device, of known types -- on the host, before anything is launched."""
+    # Where all are alike one call a list tells (as torch's own optimisers sort their tensors).  A call for both lists would not: it lets the second one's lie on the CPU.
+    kinds = list(_group_tensors([tensors], False))
+    if len(kinds) == 1 and kinds[0][1] in _GRAD_TYPES and kinds[0][0].type == "cuda" and (out is None or list(_group_tensors([out], False)) == kinds):
+        return [_GRAD_TYPES[kinds[0][1]]] * len(tensors)
     types = [_GRAD_TYPES.get(t.dtype) for t in tensors]
-    devices = {t.get_device() for t in tensors if t.layout is torch.strided and t.is_cuda}
-    if None in types or len(devices) != 1 or not all([t.layout is torch.strided and t.is_cuda for t in tensors]):
-        _refuse_grads(tensors, what)
+    every = tensors if out is None else tensors + out
+    devices = {t.get_device() for t in every if t.layout is torch.strided and t.is_cuda}
+    if None in types or len(devices) != 1 or not all([t.layout is torch.strided and t.is_cuda for t in every]):
+        _refuse_grads(every, what)
     return types
+
+
+def _dense(tensors, what):
+    """Whether each of `tensors` is contiguous; refuses sparse ones."""
+    try:
+        whole = [t.is_contiguous() for t in tensors]
+    except RuntimeError:          # compressed layouts have no such thing
+        whole = [False]
+    if not all(whole) and any(t.layout is not torch.strided for t in tensors):
+        _refuse_grads(tensors, what)
+    return whole
 
 
 def _launch_norm(src, dst, types, max_norm, code):
@@ -146,7 +163,7 @@ def grad_norm(tensors, norm_type=2.0):
     if not tensors:
         return torch.zeros(())
     types = _check_grads(tensors, "grad_norm")
-    return _launch_norm([t if t.is_contiguous() else t.contiguous() for t in tensors], None, types, 0.0, code)
+    return _launch_norm([t if c else t.contiguous() for t, c in zip(tensors, _dense(tensors, "grad_norm"))], None, types, 0.0, code)
 
 
 @torch.no_grad()
@@ -165,24 +182,26 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         if len(out) != len(grads):
             raise _lib.GShellHipError(f"clip_grads: {len(grads)} gradients and {len(out)} outputs")
         for g, o in zip(grads, out):
-            if o.shape != g.shape or o.dtype != g.dtype:
+            if o.dtype != g.dtype or not o.is_same_size(g):
                 raise _lib.GShellHipError(f"clip_grads: an output is {tuple(o.shape)} {o.dtype}, its gradient {tuple(g.shape)} {g.dtype}")
     if not grads:
         return torch.zeros(())
-    types = _check_grads(grads, "clip_grads")
+    types = _check_grads(grads, "clip_grads", None if out is grads else out)
+    whole = _dense(grads, "clip_grads")
+    src = grads if all(whole) else [g if c else g.contiguous() for g, c in zip(grads, whole)]
     if out is not grads:
-        _check_grads(out, "clip_grads")
-        if out[0].get_device() != grads[0].get_device():
-            raise _lib.GShellHipError(f"clip_grads: gradients are on {grads[0].device}, outputs on {out[0].device}")
-    apart = [o.data_ptr() for o in out if not o.is_contiguous()]          # written from copies, one after the other
-    if len(set(apart)) != len(apart):
-        raise _lib.GShellHipError("clip_grads: the same output twice")
-    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    dst = src if out is grads else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in out]
-    norm = _launch_norm(src, dst, types, max_norm, code)
-    for o, d in zip(out, dst):
-        if d is not o:
-            o.copy_(d)
+        whole = _dense(out, "clip_grads")
+    if all(whole):
+        norm = _launch_norm(src, src if out is grads else out, types, max_norm, code)
+    else:          # outputs that are not contiguous are written from copies, one after the other
+        apart = [o.data_ptr() for o, c in zip(out, whole) if not c]
+        if len(set(apart)) != len(apart):
+            raise _lib.GShellHipError("clip_grads: the same output twice")
+        dst = src if out is grads else [o if c else torch.empty_like(o, memory_format=torch.contiguous_format) for o, c in zip(out, whole)]
+        norm = _launch_norm(src, dst, types, max_norm, code)
+        for o, d in zip(out, dst):
+            if d is not o:
+                o.copy_(d)
     torch.autograd.graph.increment_version(out)
     return norm
 

@@ -148,3 +148,32 @@ def test_a_captured_clip_replays():
         held = [norm.clone()] + [o.clone() for o in out]
         want = [torch.empty_like(g) for g in gs]
         assert torch.equal(held[0], optim.clip_grads(gs, 1.0, out=want)) and all(torch.equal(a, b) for a, b in zip(held[1:], want))
+
+
+def test_refusals_on_the_device():
+    from gshell_amd import optim
+    from gshell_amd._lib import GShellHipError
+    g = torch.randn(6, 4, device=DEV)
+    for bad in (g.to_sparse(), g.to_sparse_csr()):
+        for call in (lambda: optim.grad_norm([g, bad]), lambda: optim.clip_grads([g, bad], 1.0)):      # noqa: B023
+            with pytest.raises(GShellHipError, match="dense float32"):
+                call()
+    t = torch.empty(4, 6, device=DEV).t()
+    a = torch.empty(12, 2, device=DEV)
+    for grads, out, what in (([g, g.clone()], [t, t], "same output twice"), ([t, t], None, "same output twice"), ([g], [g.half()], "an output is"), ([g], [g.cpu()], "HBM"),
+                             ([g], [torch.empty(4, 6, device=DEV)], "an output is"), ([g, g], None, "shares memory"), ([a[:, 0], a[:, 0]], None, "same output twice")):
+        before = g.clone()
+        with pytest.raises(GShellHipError, match=what):
+            optim.clip_grads(grads, 1.0, out=out)
+        assert torch.equal(g, before)
+
+
+def test_views_of_one_tensor_clip_apart():
+    """Columns of one matrix: not contiguous, each written from a copy; whole numbers over a power of two are exact."""
+    from gshell_amd import optim
+    a = torch.zeros(16, 3, device=DEV)
+    a[:, 0], a[:, 2] = 3.0, 4.0
+    n = optim.clip_grads([a[:, 0], a[:, 2]], 10.0)          # 4 * 5
+    assert float(n) == 20.0
+    want = torch.tensor([1.5, 0.0, 2.0], device=DEV).expand(16, 3)
+    assert torch.allclose(a, want, rtol=4 * 2.0 ** -24, atol=0)

@@ -145,3 +145,22 @@ def test_linear_workspace_sizes(dtype):
                     assert fwd >= 0 and bwd >= 0, (M, N, K)
                     if max(M, N, K) < 5000:
                         assert fwd <= 8 * es * (M * K + N * K + M * N) + (64 << 20) and bwd <= 8 * es * (M * K + N * K + M * N) + (160 << 20), (M, N, K, fwd, bwd)
+
+
+def test_linear_backward_c_entry_refuses_bad_arguments():
+    from gshell_amd import _lib
+    L, p = _lib.lib(), 256
+
+    def bwd(g=p, ldg=4, x=p, ldx=4, w=p, ldw=4, M=4, N=4, K=4, dtype=0, dx=p, dw=p, db=p, ws=p, ws_bytes=1 << 30):
+        return L.gs_linear_bwd(g, ldg, 0, x, ldx, w, ldw, M, N, K, dtype, dx, dw, db, ws, ws_bytes, 0)
+    for kw in (dict(g=0), dict(ldg=-1), dict(x=0), dict(ldx=-4), dict(w=0), dict(ldw=-4), dict(M=-1), dict(K=1 << 31), dict(dtype=1, N=1 << 21), dict(dtype=3), dict(ws_bytes=0, dtype=1), dict(ws=257)):
+        assert bwd(**kw) != 0 and b"gs_linear_bwd" in L.gs_last_error(), kw
+
+
+def test_modules_say_what_they_are_and_a_table_can_be_given():
+    rows = torch.arange(12.0).view(3, 4)
+    table = nn.Embedding.from_pretrained(rows, padding_idx=-1, scale=0.5)
+    assert table.weight.data_ptr() == rows.data_ptr() and not table.weight.requires_grad and table.padding_idx == 2 and table.scale == 0.5 and torch.equal(rows, torch.arange(12.0).view(3, 4))
+    assert nn.Embedding.from_pretrained(rows, freeze=False).weight.requires_grad and "scale=0.5" in repr(table) and "activation=gelu" in repr(nn.Linear(2, 3, activation="gelu"))
+    with pytest.raises(GShellHipError, match="rows"):
+        nn.Embedding.from_pretrained(rows[0])
