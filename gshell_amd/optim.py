@@ -86,7 +86,7 @@ class HipAdam(torch.optim.Adam):
 
 
 _GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_group_tensors = torch._C._group_tensors_by_device_and_dtype
+_stream_of, _group_tensors = torch._C._cuda_getCurrentRawStream, torch._C._group_tensors_by_device_and_dtype
 _NORM_TYPES = {2.0: 0, 1.0: 1, float("inf"): 2}
 
 
@@ -144,7 +144,7 @@ def _launch_norm(src, dst, types, max_norm, code):
     at, numel, kinds = array("q", [t.data_ptr() for t in src]), array("q", [t.numel() for t in src]), array("i", types)
     to = None if dst is None else at if dst is src else array("q", [t.data_ptr() for t in dst])
     args = (n, at.buffer_info()[0], None if to is None else to.buffer_info()[0], numel.buffer_info()[0], kinds.buffer_info()[0], code, max_norm, norm.data_ptr(), ws.data_ptr(),
-            need, torch.cuda.current_stream(dev).cuda_stream)
+            need, _stream_of(dev))
     if torch.cuda.current_device() == dev:
         rc = L.gs_grad_norm(*args)
     else:
@@ -155,7 +155,6 @@ def _launch_norm(src, dst, types, max_norm, code):
     return norm
 
 
-@torch.no_grad()
 def grad_norm(tensors, norm_type=2.0):
     """The norm (2, 1 or inf) of all elements of `tensors` together, one fp32 value on their device; summed in 64 bits."""
     code = _norm_code(norm_type, "grad_norm")
@@ -163,10 +162,9 @@ def grad_norm(tensors, norm_type=2.0):
     if not tensors:
         return torch.zeros(())
     types = _check_grads(tensors, "grad_norm")
-    return _launch_norm([t if c else t.contiguous() for t, c in zip(tensors, _dense(tensors, "grad_norm"))], None, types, 0.0, code)
+    return _launch_norm([t if c else t.detach().contiguous() for t, c in zip(tensors, _dense(tensors, "grad_norm"))], None, types, 0.0, code)
 
 
-@torch.no_grad()
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)) -> norm, one fp32 value on the device.  Without `out`, in place.
 
@@ -188,7 +186,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         return torch.zeros(())
     types = _check_grads(grads, "clip_grads", None if out is grads else out)
     whole = _dense(grads, "clip_grads")
-    src = grads if all(whole) else [g if c else g.contiguous() for g, c in zip(grads, whole)]
+    src = grads if all(whole) else [g if c else g.detach().contiguous() for g, c in zip(grads, whole)]
     if out is not grads:
         whole = _dense(out, "clip_grads")
     if all(whole):
@@ -201,7 +199,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         norm = _launch_norm(src, dst, types, max_norm, code)
         for o, d in zip(out, dst):
             if d is not o:
-                o.copy_(d)
+                o.detach().copy_(d)
     torch.autograd.graph.increment_version(out)
     return norm
 
