@@ -20,7 +20,7 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "softplus": 2, "silu": 3, "gelu": 
 # The calls below are short next to what Python spends around them, and a backward pass runs in a thread of its own, where every Python object comes from another core's
 # cache: plain numbers and addresses go to the C functions (_lib.PLAIN_CALLS), what a backward pass needs is worked out in the forward pass, and the current device is changed
 # only where it is another one.
-_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+_stream_of, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _at(t):
@@ -66,7 +66,7 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
 
 def _linear_backward(ctx, g):
     x, weight, dact = ctx.saved_tensors
-    M, K, N, code, want_x, want_w, want_b, want_r = ctx.rest
+    M, K, N, code, want_x, want_w, want_b, want_r, L = ctx.rest
     dx = dw = db = None
     if want_x or want_w or want_b:
         gr, ldg = _rows(g)
@@ -84,7 +84,6 @@ def _linear_backward(ctx, g):
         if want_b:
             db = gr.new_empty(N)
             bo = db.data_ptr()
-        L = _lib.lib()
         gp, dp = gr.data_ptr(), _at(dact)
         need = L.gs_linear_bwd_workspace_bytes(gp, ldg, dact is not None, xp, ldx, wp, ldw, M, N, K, code, want_x, want_w, want_b)
         if need < 0:
@@ -108,7 +107,7 @@ class _LinearFn(torch.autograd.Function):
         want_x, want_w, want_b, want_r, _, _ = ctx.needs_input_grad
         y, dact = _linear_forward(x, weight, bias, residual, act, beta, want_x or want_w or want_b)
         ctx.save_for_backward(x if want_w else None, weight if want_x else None, dact)
-        ctx.rest = (*x.shape, weight.shape[0], _DTYPES[x.dtype], want_x, want_w, want_b, want_r)
+        ctx.rest = (*x.shape, weight.shape[0], _DTYPES[x.dtype], want_x, want_w, want_b, want_r, _lib.lib())
         return y
 
     @staticmethod
@@ -222,17 +221,17 @@ def _lookup(ids, weight, scale):
 
 def _embedding_backward(ctx, g):
     ids, = ctx.saved_tensors
-    kind, T, V, D, padding_idx, code, scale, need = ctx.rest
+    kind, T, V, D, padding_idx, code, scale, need, call = ctx.rest
     g, ldg = _rows(g)
     dw = g.new_empty((V, D))
     ws = g.new_empty(need, dtype=torch.uint8)
     device = g.get_device()
     args = (ids.data_ptr(), kind, g.data_ptr(), ldg, T, V, D, padding_idx, code, scale, dw.data_ptr(), ws.data_ptr(), need, _stream_of(device))
     if _current_device() == device:
-        rc = _lib.lib().gs_embedding_bwd(*args)
+        rc = call(*args)
     else:
         with torch.cuda.device(device):
-            rc = _lib.lib().gs_embedding_bwd(*args)
+            rc = call(*args)
     if rc:
         check(rc, "gs_embedding_bwd")
     return None, dw, None, None
@@ -242,8 +241,8 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
-        T, (V, D) = ids.numel(), weight.shape
-        ctx.rest = (_ID_TYPES[ids.dtype], T, V, D, padding_idx, _DTYPES[weight.dtype], scale, _lib.lib().gs_embedding_bwd_workspace_bytes(T, V, D))
+        T, (V, D), L = ids.numel(), weight.shape, _lib.lib()
+        ctx.rest = (_ID_TYPES[ids.dtype], T, V, D, padding_idx, _DTYPES[weight.dtype], scale, L.gs_embedding_bwd_workspace_bytes(T, V, D), L.gs_embedding_bwd)
         return _lookup(ids, weight, scale)
 
     @staticmethod

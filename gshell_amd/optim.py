@@ -145,7 +145,7 @@ def _launch_norm(src, dst, types, max_norm, code):
     to = None if dst is None else at if dst is src else array("q", [t.data_ptr() for t in dst])
     args = (n, at.buffer_info()[0], None if to is None else to.buffer_info()[0], numel.buffer_info()[0], kinds.buffer_info()[0], code, max_norm, norm.data_ptr(), ws.data_ptr(),
             need, _stream_of(dev))
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:
         rc = L.gs_grad_norm(*args)
     else:
         with torch.cuda.device(dev):
