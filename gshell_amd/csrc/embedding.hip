@@ -193,9 +193,15 @@ template <typename T, int VEC, typename U> __device__ __forceinline__ void load_
         const Pack<T, VEC> q = *(const Pack<T, VEC>*)p;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) out[k] = (U)q.v[k];
+    } else if (left > 0) {          // what is behind the row's end repeats its last value in the load: one branch and one wait
+        const int n = (int)left;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out[k] = (U)p[k < n ? k : n - 1];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) out[k] = k < n ? out[k] : (U)0.f;
     } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) out[k] = k < left ? (U)p[k] : (U)0.f;
+        for (int k = 0; k < VEC; ++k) out[k] = (U)0.f;
     }
 }
 template <typename T, int VEC, typename U> __device__ __forceinline__ void store_row(T* p, int64_t left, const U (&in)[VEC]) {
@@ -236,6 +242,18 @@ __global__ void __launch_bounds__(256) k_lookup(const I* ids, const T* w, int64_
                 else
 #pragma unroll
                     for (int k = 0; k < VEC; ++k) v[u][k] = __builtin_nanf("");
+            } else if (D >= VEC && V > 0) {          // two rows; what has no value to read reads the table's first
+                const int64_t next = t + 1 < tokens ? (int64_t)ids[t + 1] : -1;
+                const bool ok1 = next >= 0 && next < V;
+                const T *a = ok ? w + id * ldw + c : w, *b = ok1 ? w + next * ldw : w;
+                const int here = (int)(D - c), da = ok ? 1 : 0, db = ok1 ? 1 : 0;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) v[u][k] = (float)a[(k < here ? k : 0) * da];
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) {
+                    const float q = (float)b[k < here ? 0 : (k - here) * db];
+                    v[u][k] = k < here ? (ok ? v[u][k] : __builtin_nanf("")) : ok1 ? q : __builtin_nanf("");
+                }
             } else {
                 int64_t r = t, q = c, row = ok ? id : -1;
 #pragma unroll
