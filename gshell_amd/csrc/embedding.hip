@@ -293,23 +293,26 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
 
 constexpr int BVEC = 4;          // columns of a lane in the sums of narrow rows
 
-// rows `v0 ..` of the table that no token names, 64 of them a wave
-template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int64_t v0, T* dw) {
+// Rows of the table that no token names: `rows` of them a wave from v0 on, 64 at most, 2^group_log lanes a row
+// (6 tokens of 3389 fp32 over 1801 rows: 15 us with one row a wave, 80 with 64)
+template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int64_t v0, int rows, int group_log, T* dw) {
     constexpr int VEC = 16 / sizeof(T);
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, group = 1 << group_log;
     const int64_t v = v0 + lane;
     if (v0 >= V) return;
     bool empty = false;
-    if (v < V) {
+    if (lane < rows && v < V) {
         const int64_t at = lower_bound(keys, tokens, (uint32_t)v);
         empty = at >= tokens || keys[at] != (uint32_t)v;
     }
+    const uint64_t which = __ballot(empty);
     const float zero[VEC] = {};
-    for (uint64_t m = __ballot(empty); m; m &= m - 1) {
-        T* row = dw + (v0 + (__ffsll((unsigned long long)m) - 1)) * D;
-        for (int64_t c = lane * VEC; c < D; c += 64 * VEC) store_row<T, VEC>(row + c, D - c, zero);
-    }
+    for (int r = lane >> group_log; r < rows; r += 64 >> group_log)
+        if (which >> r & 1)
+            for (int64_t c = (lane & (group - 1)) * VEC; c < D; c += group * VEC) store_row<T, VEC>(dw + (v0 + r) * D + c, D - c, zero);
 }
+// 64 rows a wave, fewer where the waves would be fewer than those of four workgroups a compute unit
+static int rows_a_wave(int64_t V) { return V >= 64 * 4096 ? 64 : V >= 16 * 4096 ? 16 : V >= 4 * 4096 ? 4 : 1; }
 
 // Rows of more than 32 vectors of 16 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
 // eight rows are on their way at a time.  A run of up to CHUNK tokens is summed as a whole by the chunk where it begins; a longer one leaves a part in each of its chunks.
@@ -317,9 +320,9 @@ template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t*
 // (3.5 TB/s), evenly spread 59 us.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t stretches,
-                                                  int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
+                                                  int64_t chunks, int64_t sum_blocks, int rows, int clear_log, float scale, T* dw, float* first, float* last) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + wave) * 64, dw);
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + wave) * rows, rows, clear_log, dw);
     const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
     if (unit >= chunks * stretches) return;
     const int64_t chunk = unit / stretches, c = (unit % stretches * 64 + lane) * VEC, e0 = chunk * CHUNK;
@@ -377,8 +380,8 @@ __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const ui
 // Narrower rows: several groups of lanes a wave, a chunk each, 25 us for 262144 tokens of 64 bf16 over 160 rows; every run that crosses chunks leaves its parts.  Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int group_log,
-                                                    int64_t stretches, int64_t chunks, int64_t sum_blocks, float scale, T* dw, float* first, float* last) {
-    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * 64, dw);
+                                                    int64_t stretches, int64_t chunks, int64_t sum_blocks, int rows, int clear_log, float scale, T* dw, float* first, float* last) {
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * rows, rows, clear_log, dw);
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
     if (unit >= chunks * stretches) return;
     const int64_t chunk = unit / stretches, c = ((unit % stretches) << group_log) * BVEC + (threadIdx.x & ((1 << group_log) - 1)) * BVEC;
@@ -400,15 +403,25 @@ __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const 
             store_row<T, BVEC>(dw + (int64_t)run * D + c, D - c, out);
         }
     };
+    // the next tokens' rows and numbers are on their way while these are summed; what is behind the end repeats the last one
+    uint32_t next[8], place[8];
+    const auto fetch = [&](int64_t e) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t at = e + k < e1 ? e + k : e1 - 1;
+            next[k] = keys[at], place[k] = pos[at];
+        }
+    };
+    fetch(e0);
     for (int64_t e = e0; e < e1; e += 8) {
         uint32_t key[8];
         float v[8][BVEC];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) key[k] = e + k < e1 ? keys[e + k] : none;
-#pragma unroll
         for (int k = 0; k < 8; ++k) {
-            if (key[k] != none) load_row<T, BVEC>(g + (int64_t)pos[e + k] * ldg + c, D - c, v[k]);
+            key[k] = e + k < e1 ? next[k] : none;
+            if (key[k] != none) load_row<T, BVEC>(g + (int64_t)place[k] * ldg + c, D - c, v[k]);
         }
+        if (e + 8 < e1) fetch(e + 8);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (e + k >= e1) break;
@@ -642,7 +655,8 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
     if (tokens > 0)
         if (const int rc = sort_tokens<I>(ids, tokens, V, padding, p, base, keys, pos, stream)) return rc;
     float *first = (float*)(base + p.first), *last = (float*)(base + p.last);
-    const int64_t zero_blocks = gs::cdiv(V, 256);
+    const int rows = rows_a_wave(V), clear_log = group_log_of(gs::cdiv(D, 16 / sizeof(T)));
+    const int64_t zero_blocks = gs::cdiv(V, 4 * rows);
     constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
     const int vec = vector_of(sizeof(T), D, ldg, g, dw);
     const bool wide = gs::cdiv(D, vec) > 32;
@@ -654,12 +668,12 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
         GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         const auto kernel = vec == V16 ? k_sum_wide<T, V16> : k_sum_wide<T, V8>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
-                           across, p.chunks, sum_blocks, scale, (T*)dw, first, last);
+                           across, p.chunks, sum_blocks, rows, clear_log, scale, (T*)dw, first, last);
     } else {
         const int64_t sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256);
         GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
-                           gl, stretches, p.chunks, sum_blocks, scale, (T*)dw, first, last);
+                           gl, stretches, p.chunks, sum_blocks, rows, clear_log, scale, (T*)dw, first, last);
     }
     if (p.chunks > 1) {
         // groups cover a whole row; a run may hold most of the tokens: a large workgroup where rows are used a thousand times and more
