@@ -905,8 +905,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
 }
 
 // What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type, in rows that start on 16 bytes with zeros behind their ends, and its
-// column sums (of the unrounded values) by slabs of rows: 16384 x 4096 bf16 73 us, 402 MB at 5.5 TB/s.  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
-constexpr int GZ_LANES = 32, GZ_LINES = 8;
+// column sums (of the unrounded values) by slabs of rows: 16384 x 4096 bf16 73 us, 402 MB at 5.5 TB/s; 28432 x 6528 260 us, 1.1 GB (one line of a lane at a time 300, four 354).  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
+constexpr int GZ_LANES = 32, GZ_LINES = 8, GZ_ROUND = 2 * GZ_LINES;
 template <typename T> struct Gz {
     const T* g;
     const typename dact_type<T>::type* dact;
@@ -942,17 +942,25 @@ template <typename T> __global__ void __launch_bounds__(256) k_prepare(Gz<T> G, 
     const int64_t m0 = by * G.slab, m1 = m0 + G.slab < G.M ? m0 + G.slab : G.M;
     float s[V] = {};
     if (in_row > 0)
-        for (int64_t m = m0 + y; m < m1; m += GZ_LINES) {
-            float v[V], d[V];
-            load_some<T, V>(G.g + m * G.ldg + j, in_row, v);
-            if (G.dact) {
-                load_some<typename dact_type<T>::type, V>(G.dact + m * G.N + j, in_row, d);
+        for (int64_t m = m0 + y; m < m1; m += GZ_ROUND) {
+            // GZ_ROUND / GZ_LINES lines of a lane are on their way together
+            float v[GZ_ROUND / GZ_LINES][V], d[GZ_ROUND / GZ_LINES][V];
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[k] = gated(v[k], d[k]);
+            for (int q = 0; q < GZ_ROUND / GZ_LINES; ++q) {
+                const int64_t l = m + q * GZ_LINES, some = l < m1 ? in_row : 0;
+                load_some<T, V>(G.g + l * G.ldg + j, some, v[q]);
+                if (G.dact) load_some<typename dact_type<T>::type, V>(G.dact + l * G.N + j, some, d[q]);
             }
-            if (G.gz) store_some<T, V>(G.gz + m * G.ldgz + j, V, v);
 #pragma unroll
-            for (int k = 0; k < V; ++k) s[k] += v[k];
+            for (int q = 0; q < GZ_ROUND / GZ_LINES; ++q) {
+                const int64_t l = m + q * GZ_LINES;
+                if (G.dact)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) v[q][k] = gated(v[q][k], d[q][k]);
+                if (G.gz && l < m1) store_some<T, V>(G.gz + l * G.ldgz + j, V, v[q]);
+#pragma unroll
+                for (int k = 0; k < V; ++k) s[k] += v[q][k];
+            }
         }
     if (!G.part) return;
 #pragma unroll
