@@ -2,7 +2,7 @@
 
   linear(x, weight, bias, residual, activation)   y = act(x W^T + b) + r with its backward pass   (csrc/linear.hip)
   Linear                                          torch.nn.Linear with that epilogue; same parameter names, same initialisation
-  embedding(ids, weight, scale, padding_idx)      y_t = scale W[id_t], gradient by sorted ids             (csrc/embedding.hip)
+  embedding(ids, weight, scale, padding_idx)      y_t = scale W[id_t], gradient without atomics           (csrc/embedding.hip)
   Embedding                                       torch.nn.Embedding's parameters and initialisation, with the scale
 
 bf16, fp16 and fp32; every sum is 32-bit; a call's sums are taken in a fixed order, so the same inputs give the same bits.  All operands live in HBM: there is no CPU
@@ -253,7 +253,7 @@ class _EmbeddingFn(torch.autograd.Function):
 def embedding(ids, weight, scale=1.0, padding_idx=None):
     """scale * weight[ids]: ids int64 or int32 of any shape, weight [V, D] (float32, bfloat16, float16) -> ids.shape + [D].
 
-    The gradient sums a row's tokens in their order in 32 bits: the same bits every time.  The row `padding_idx` gets none.  Ids are not looked at on the host: one outside
+    The gradient sums a row's tokens in 32 bits, in an order that the sizes and the ids alone decide: the same bits every time.  The row `padding_idx` gets none.  Ids are not looked at on the host: one outside
     of [0, V) gives a row of NaN and has no gradient (negative ids do not count from the end)."""
     if weight.dim() != 2 or weight.dtype not in _DTYPES:
         raise GShellHipError(f"embedding: a weight [V, D] of float32, bfloat16 or float16 is wanted, got {tuple(weight.shape)} {weight.dtype}")

@@ -878,10 +878,10 @@ int gs_linear_bwd(const void* g, int64_t ldg, const void* dact, const void* x, i
                   int64_t workspace_bytes, gs_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
- * Table lookup with scaling, and its gradient by sorted row numbers
+ * Table lookup with scaling, and its gradient without atomics
  *   fwd: y [T,D] = scale * weight[ids], weight [V,D] with rows ldw elements apart; ids int64 (ids64 = 1) or int32.
- *   bwd: dw [V,D] (written whole, unnamed rows zero) = scale * sum of g's rows (ldg apart) by id, in the order of the tokens, in 32 bits: the same
- *        bits every time.  padding_idx: a row without gradient (-1: none).  An id outside [0, V) gives a NaN row and no gradient.
+ *   bwd: dw [V,D] (written whole, unnamed rows zero) = scale * sum of g's rows (ldg apart) by id, in 32 bits, in an order that the sizes and ids decide: the
+ *        same bits every time.  padding_idx: a row without gradient (-1: none).  An id outside [0, V) gives a NaN row and no gradient.
  *   dtype as for gs_linear_fwd; the workspace starts on 16 bytes.
  * ---------------------------------------------------------------------------------- */
 int gs_embedding_fwd(const void* ids, int ids64, const void* weight, int64_t ldw, int64_t T, int64_t V, int64_t D, int dtype,

@@ -72,6 +72,13 @@ def test_around_what_counts_as_few_rows(kind, T, V, D):
     check_one(torch.randint(-1, V + 1, (T,), generator=gen).clamp_(0, V - 1), V, D, TYPES[kind], 0.5, V // 2 if V > 2 else None, T)
 
 
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("T,V,D", [(3000, 70001, 520), (3000, 9000, 4100), (5000, 4200000, 4)])
+def test_large_tables(kind, T, V, D):
+    gen = torch.Generator().manual_seed(T)
+    check_one(torch.randint(0, V // 3, (T,), generator=gen) * 3, V, D, TYPES[kind], 2.0, 0, T)
+
+
 def test_shapes_types_of_ids_and_repeatability():
     from gshell_amd import nn
     gen = torch.Generator().manual_seed(1)
