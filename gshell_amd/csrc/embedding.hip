@@ -574,6 +574,7 @@ static int group_log_of(int64_t vectors) {          // lanes, as a power of two,
 // Whether a table counts as one of few, narrow rows: at most 64 columns, and the tables of 256 lanes' groups fit in LDS; then twice the lanes where theirs do, and workgroups for
 // the chip.  fp32, lookup and gradient: 262144 tokens over 72 x 32 26 us, sorted 54; over 140 x 64 54, sorted 59; 2 million over 150 x 8 49, sorted 181; 256 over 72 x 32 13,
 // sorted 25.  With more than 64 columns, in stretches of 64: 262144 over 14 x 200 117, sorted 153, but over 70 x 130 132, sorted 116, and over 9 x 1024 689, sorted 584.
+constexpr int ONE_BLOCK = 8;
 struct FewPlan {
     int threads = 0, group_log = 0;          // no threads: it does not
     int64_t blocks = 0, per = 0, bytes = 0;
@@ -585,7 +586,9 @@ static FewPlan few_plan(int64_t T, int64_t V, int64_t D) {
     if ((V + 1) * D * (256 >> p.group_log) > FEW_FLOATS) return p;
     p.threads = (V + 1) * D * (512 >> p.group_log) > FEW_FLOATS ? 256 : 512;
     const int64_t round = (int64_t)(p.threads >> p.group_log) * FEW_AHEAD, rounds = gs::cdiv(T, round);
-    p.per = gs::cdiv(rounds, rounds < 256 ? rounds : 256) * round;
+    // A few rounds by one workgroup, without the second launch: 1000 tokens over 72 x 32 fp32 13 us of GPU time with the lookup, as by 8 workgroups, and 35 us of the host's for 39;
+    // 2000 would take 17 us for 13.
+    p.per = gs::cdiv(rounds, rounds <= ONE_BLOCK ? 1 : rounds < 256 ? rounds : 256) * round;
     p.blocks = gs::cdiv(T, p.per);
     p.bytes = p.blocks > 1 ? p.blocks * V * D * 4 : 0;
     return p;

@@ -7,10 +7,11 @@
 
 bf16, fp16 and fp32; every sum is 32-bit; a call's sums are taken in a fixed order, so the same inputs give the same bits.  All operands live in HBM: there is no CPU
 fallback.  A call launches on the current stream of its operands' device and keeps nothing between calls.  Gradients can be taken once
-(a second differentiation raises).  Under torch.autocast the operators run in their operands' own type.
+(a second differentiation, forward-mode differentiation and torch.func's transforms raise).  Under torch.autocast the operators run in their operands' own type.
 
 A backward pass that is captured into a graph must be the only live graph of its leaves: drop the outputs of eager passes over the same parameters first."""
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import GShellHipError, check
@@ -64,7 +65,14 @@ def _linear_forward(x, weight, bias, residual, act, beta, want_dact):
     return y, dact
 
 
+_once_differentiable = torch.autograd.function.once_differentiable
+# Function.apply without what it does for torch.func's transforms, which these layers do not take part in: where one is active the usual apply is called, and says so.
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
 def _linear_backward(ctx, g):
+    if torch.is_grad_enabled():          # create_graph: the results carry a node that says that they cannot be differentiated again
+        return _once_differentiable(_linear_backward)(ctx, g)
     x, weight, dact = ctx.saved_tensors
     M, K, N, code, want_x, want_w, want_b, want_r, L = ctx.rest
     dx = dw = db = None
@@ -110,17 +118,10 @@ class _LinearFn(torch.autograd.Function):
         ctx.rest = (*x.shape, weight.shape[0], _DTYPES[x.dtype], want_x, want_w, want_b, want_r, _lib.lib())
         return y
 
-    @staticmethod
-    def backward(ctx, g):
-        return _once(_linear_backward, ctx, g)
+    backward = staticmethod(_linear_backward)
 
 
-_once_differentiable = torch.autograd.function.once_differentiable
-
-
-def _once(body, ctx, g):
-    """A backward pass that cannot be differentiated again: where that is asked for (create_graph), its results carry a node that says so."""
-    return _once_differentiable(body)(ctx, g) if torch.is_grad_enabled() else body(ctx, g)
+_linear_apply = super(torch.autograd.Function, _LinearFn).apply
 
 
 def _linear_refuse(x, weight, bias, residual, activation, beta):
@@ -176,8 +177,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
         rows = xs[:-1].numel()
         x = x.reshape(rows, ws[1])
         residual = None if residual is None else residual.reshape(rows, ws[0])
-    if grad and torch.is_grad_enabled():
-        y = _LinearFn.apply(x, weight, bias, residual, act, beta)
+    if grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:          # (forward-mode differentiation is refused there)
+        y = (_LinearFn.apply if _transforms_active() else _linear_apply)(x, weight, bias, residual, act, beta)
     else:
         y = _linear_forward(x, weight, bias, residual, act, beta, False)[0]
     return y if flat else y.reshape(xs[:-1] + ws[:1])
@@ -220,6 +221,8 @@ def _lookup(ids, weight, scale):
 
 
 def _embedding_backward(ctx, g):
+    if torch.is_grad_enabled():
+        return _once_differentiable(_embedding_backward)(ctx, g)
     ids, = ctx.saved_tensors
     kind, T, V, D, padding_idx, code, scale, need, call = ctx.rest
     g, ldg = _rows(g)
@@ -245,9 +248,10 @@ class _EmbeddingFn(torch.autograd.Function):
         ctx.rest = (_ID_TYPES[ids.dtype], T, V, D, padding_idx, _DTYPES[weight.dtype], scale, L.gs_embedding_bwd_workspace_bytes(T, V, D), L.gs_embedding_bwd)
         return _lookup(ids, weight, scale)
 
-    @staticmethod
-    def backward(ctx, g):
-        return _once(_embedding_backward, ctx, g)
+    backward = staticmethod(_embedding_backward)
+
+
+_embedding_apply = super(torch.autograd.Function, _EmbeddingFn).apply
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None):
@@ -272,8 +276,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
                 raise GShellHipError(f"embedding: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
         raise GShellHipError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
     flat = ids if ids.is_contiguous() else ids.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
-        y = _EmbeddingFn.apply(flat, weight, float(scale), int(padding_idx))
+    if weight.requires_grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:
+        y = (_EmbeddingFn.apply if _transforms_active() else _embedding_apply)(flat, weight, float(scale), int(padding_idx))
     else:
         y = _lookup(flat, weight, float(scale))
     return y if ids.dim() == 1 else y.view(ids.shape + (D,))

@@ -311,3 +311,29 @@ def test_the_trainer_clips_by_the_joint_norm(monkeypatch):
     assert len(grads) > 3
     for a, b in grads:
         assert ((a - b).abs() <= 1024 * W * b.abs()).all()
+
+
+def test_torch_func_says_that_it_is_not_taken_part_in():
+    from gshell_amd import nn
+    x, w = torch.randn(5, 8, device=DEV), torch.randn(4, 8, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda q: nn.linear(q, w).sum())(x)
+    ids, table = torch.arange(4, device=DEV), torch.randn(6, 3, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: nn.embedding(ids, t).sum())(table)
+
+
+def test_forward_mode_and_vmap_raise():
+    import torch.autograd.forward_ad as fa
+    from gshell_amd import nn
+    x, w = torch.randn(5, 8, device=DEV), torch.randn(4, 8, device=DEV)
+    with fa.dual_level():
+        with pytest.raises(NotImplementedError):
+            nn.linear(fa.make_dual(x, torch.ones_like(x)), w)
+        with pytest.raises(NotImplementedError):
+            nn.embedding(torch.arange(3, device=DEV), fa.make_dual(w, torch.ones_like(w)))
+        assert torch.equal(nn.linear(x, w), nn.linear(x, w))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda q: nn.linear(q, w))(x[:, None])
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda q: nn.embedding(torch.arange(3, device=DEV), q))(w[None])
