@@ -127,15 +127,12 @@ template <typename T, int V> struct __attribute__((packed)) Pack { T v[V]; };   
 template <typename T> constexpr int width() { return 16 / (int)sizeof(T); }
 
 // V neighbouring values, of which the first `in_row` are in the row.  Others repeat the row's last one in the load, so that a row's end costs one branch and one wait
-// (83195 x 62 -> 103 bf16 with gelu and residual, a step: 134 us for 163) -- or, FEW, are not loaded, a branch each: for tiles of 256, whose accumulators leave no registers for more.
-template <typename T, int V, bool FEW = false> __device__ __forceinline__ void load_some(const T* p, int64_t in_row, float (&v)[V]) {
+// (83195 x 62 -> 103 bf16 with gelu and residual, a step: 134 us for 163).
+template <typename T, int V> __device__ __forceinline__ void load_some(const T* p, int64_t in_row, float (&v)[V]) {
     if (in_row >= V) {
         const Pack<T, V> q = *(const Pack<T, V>*)p;
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] = (float)q.v[k];
-    } else if (FEW) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = k < in_row ? (float)p[k] : 0.f;
     } else if (in_row > 0) {
         const int n = (int)in_row;
 #pragma unroll
@@ -159,35 +156,39 @@ template <typename T, int V> __device__ __forceinline__ void store_some(T* p, in
             if (k < in_row) p[k] = (T)v[k];
     }
 }
-// BATCH x V outputs of the lines i[0 .. BATCH-1] (those below M), columns j ..
-template <typename T, int V, int BATCH> __device__ __forceinline__ void finish(const Epilogue<T>& E, const int64_t (&i)[BATCH], int64_t j, int64_t M, int64_t N, float (&z)[BATCH][V]) {
-    const int64_t in_row = N - j;
+// BATCH x V outputs of the lines i, i + step, .. (those below M), columns j ..; q: their columns' bias.  ALL: every one of them is in the output.
+template <typename T, int V, int BATCH, bool ALL = false>
+__device__ __forceinline__ void finish(const Epilogue<T>& E, int64_t i, int64_t step, int64_t j, int64_t M, int64_t N, float (&z)[BATCH][V], const float (&q)[V]) {
+    const int64_t in_row = ALL ? V : N - j;
+    const auto in = [&](int b) __attribute__((always_inline)) { return ALL || i + b * step < M; };
     float r[BATCH][V];
-    if (E.res)
+    if (E.res) {
+        const T* p = E.res + i * E.ldr + j;
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) load_some<T, V, BATCH == 2>(E.res + i[b] * E.ldr + j, i[b] < M ? in_row : 0, r[b]);
-    if (E.bias) {
-        float q[V];
-        load_some<T, V, BATCH == 2>(E.bias + j, in_row, q);
+        for (int b = 0; b < BATCH; ++b) load_some<T, V>(p + b * (step * E.ldr), in(b) ? in_row : 0, r[b]);
+    }
+    if (E.bias)
 #pragma unroll
         for (int b = 0; b < BATCH; ++b)
 #pragma unroll
             for (int k = 0; k < V; ++k) z[b][k] += q[k];
-    }
     if (E.act != ACT_NONE) {
         float d[BATCH][V];
         act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta_log2e, E.two_over_beta, z, d);
-        if (E.dact)
+        if (E.dact) {
+            auto* p = E.dact + i * N + j;
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
-                if (i[b] < M) store_some<typename dact_type<T>::type, V>(E.dact + i[b] * N + j, in_row, d[b]);
+                if (in(b)) store_some<typename dact_type<T>::type, V>(p + b * (step * N), in_row, d[b]);
+        }
     }
+    T* p = E.out + i * E.ldo + j;
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
         if (E.res)
 #pragma unroll
             for (int k = 0; k < V; ++k) z[b][k] += r[b][k];
-        if (i[b] < M) store_some<T, V>(E.out + i[b] * E.ldo + j, in_row, z[b]);
+        if (in(b)) store_some<T, V>(p + b * (step * E.ldo), in_row, z[b]);
     }
 }
 
@@ -216,37 +217,46 @@ template <int TM> __device__ __forceinline__ void put_sums(const f32x4 (&acc)[TM
 #pragma unroll
         for (int w = 0; w < 4; ++w) *(f32x4*)(lds + piece_of_sums(u * 16 + (lane & 15), w * 4 + (lane >> 4))) = acc[first + u][w];
 }
-// Lines l_begin .. l_end of them, BATCH lines a lane side by side, as many as the registers hold: what they read of the residual is in flight together.
+// Lines l_begin .. l_end of them, BATCH lines a lane side by side, as many as the registers hold (one with tiles of 256): what they read of the residual is in flight together.
+// A stretch inside of the output goes without checks (131072 x 256 x 256 fp32: y with softplus 164 us for 170, dx 156 for 165, dW 131 for 134).
 // fix(i, j, z): what a sum is replaced by.
-template <typename T, int BATCH, typename F>
-__device__ __forceinline__ void drain_sums(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
+template <typename T, int BATCH, bool ALL, typename F>
+__device__ __forceinline__ void drain_lines(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j, int64_t M, int64_t N, const float (&q)[width<T>()], F& fix) {
     constexpr int V = width<T>(), LANES = 64 / V, LINES = 64 / LANES;
     const int lane = threadIdx.x & 63, c = lane % LANES * V;
-    const int64_t j = j0 + c;
 #pragma unroll 1
     for (int l0 = l_begin; l0 < l_end; l0 += LINES * BATCH) {
-        int64_t i[BATCH];
         float z[BATCH][V];
+        const int64_t i = i0 + l0 + lane / LANES;
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
             const int l = l0 + b * LINES + lane / LANES;
-            i[b] = i0 + l;
 #pragma unroll
             for (int k = 0; k < V; k += 4) {
-                const f32x4 q = *(const f32x4*)(lds + piece_of_sums(l, (c + k) >> 2));
+                const f32x4 s = *(const f32x4*)(lds + piece_of_sums(l, (c + k) >> 2));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[b][k + e] = q[e];
+                for (int e = 0; e < 4; ++e) z[b][k + e] = s[e];
             }
-            if (i[b] < M && j < N) fix(i[b], j, z[b]);
+            if (ALL || i + b * LINES < M) fix(i + b * LINES, j, z[b]);
         }
         if (E.part) {
 #pragma unroll
             for (int b = 0; b < BATCH; ++b)
-                if (i[b] < M && j < N) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i[b]) * N + j, N - j, z[b]);
-        } else if (j < N) {
-            finish<T, V, BATCH>(E, i, j, M, N, z);
+                if (ALL || i + b * LINES < M) store_some<float, V>(E.part + ((int64_t)blockIdx.y * M + i + b * LINES) * N + j, ALL ? V : N - j, z[b]);
+        } else {
+            finish<T, V, BATCH, ALL>(E, i, LINES, j, M, N, z, q);
         }
     }
+}
+template <typename T, int BATCH, typename F>
+__device__ __forceinline__ void drain_sums(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
+    constexpr int V = width<T>(), LANES = 64 / V;
+    const int64_t j = j0 + (threadIdx.x & 63) % LANES * V;
+    float q[V] = {};
+    if (j >= N) return;
+    if (E.bias && !E.part) load_some<T, V>(E.bias + j, N - j, q);
+    if (i0 + l_end <= M && j0 + 64 <= N) drain_lines<T, BATCH, true>(E, lds, l_begin, l_end, i0, j, M, N, q, fix);
+    else drain_lines<T, BATCH, false>(E, lds, l_begin, l_end, i0, j, M, N, q, fix);
 }
 template <typename T, int TM, int BATCH, typename F>
 __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&acc)[TM][4], float* lds, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
@@ -304,8 +314,8 @@ template <typename T> __device__ __forceinline__ void join_columns(const Columns
 // fall on distinct banks.
 //   rows operand     a lane loads 8 neighbours of the contraction at a time; columns operand: 16 or 8 of one line, neighbouring lanes neighbouring lines
 // A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
-// 131072 x 256 x 256: y 119 us (144 Tflop/s; the library's fp32 product 155), with softplus and act' kept 171; dx 122 (145), with a gate 168; dW 107 (319), with a gate and db 134.
-// 4096 x 4096 x 4096: 790, 650, 690 us (1040).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (55 us of dx, 80 of y with
+// 131072 x 256 x 256: y 117 us (147 Tflop/s; the library's fp32 product 155), with softplus and act' kept 164; dx 114 (154), with a gate 156; dW 107 (319), with a gate and db 131.
+// 4096 x 4096 x 4096: 780, 660, 680 us (1040); 512 x 512 x 512 11, 12, 12 (20).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (45 us of dx, 65 of y with
 // softplus, by leaving it out) share a compute unit and overlap in part.  Tried and left: the weight's parts made once by a launch of their own and loaded straight into LDS, 165
 // + 5 us of 184 for dx and 180 + 5 of 184 for y; workgroups that start a quarter of a tile apart, no change.
 constexpr int TILE = 128, BK = 32;
@@ -510,6 +520,7 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
     }
     const auto fix = [&](int64_t i, int64_t j, auto& z) {
         // a sum that is not finite is done again without the split, in fp32, and with gated()
+        if (fabsf(z[0]) + fabsf(z[1]) + fabsf(z[2]) + fabsf(z[3]) < __builtin_inff()) return;
 #pragma unroll 1
         for (int k = 0; k < 4; ++k)
             if (!(fabsf(z[k]) < __builtin_inff()) && j + k < N) {
@@ -541,7 +552,7 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
 //   columns operand  LDS holds [64][line]; fragments come out transposed by ds_read_b64_tr_b16 (4 contraction rows x 16 lines a 16-lane group); the 32-byte
 //                    piece q of row k sits at q ^ h(k), with h different for the 16 rows that one instruction reads
 // Lines and contraction beyond the operand are loaded as zero (an offset outside of the buffer's range).
-// 16384 x 4096 x 4096 bf16 with 256 x 256 tiles: y 511 us (1.08 Pflop/s; the library 448), with gelu, residual and act' kept 540; dx 500 (522), dW 442 .. 484 (577).  Four tiles a
+// 16384 x 4096 x 4096 bf16 with 256 x 256 tiles: y 511 us (1.08 Pflop/s; the library 448), with gelu, residual and act' kept 535; dx 500 (522), dW 442 .. 484 (577).  Four tiles a
 // compute unit: what is left is their starts and ends, 15 us each, in which the matrix cores wait; the clock falls with them busy, so less waiting gains less than it
 // takes away.  The next lines' residual loaded ahead in the epilogue: 588 us for 577.  4096 x 2048 x 2048 with 128 x 128 tiles: 39, 40, 41 us (36, 38, 50).
 typedef __attribute__((address_space(3))) void lds_void;
@@ -683,7 +694,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Opera
     static_assert(WN == 64 && BUFFER * 2 * 2 == THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
     constexpr int SHARE = THREADS / 64 / 2;
     short* mine = wave < SHARE ? s0 : s1;
-    store_wave<T, TM, (TM > 4 ? 2 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+    store_wave<T, TM, (TM > 4 ? 1 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
 #endif
 }
 
@@ -865,9 +876,11 @@ __global__ void __launch_bounds__(ROWS_THREADS) k_rows(const T* x, int64_t ldx, 
         float z[1][1] = {{0.f}};
 #pragma unroll
         for (int s = 0; s < ROWS_WAVES; ++s) z[0][0] += sums[s][n * MT + (m16 >> 4)][m16 & 15][k & 15];
-        const int64_t row[1] = {m};
         if (E.part) E.part[((int64_t)blockIdx.y * M + m) * N + j] = z[0][0];
-        else finish<T, 1, 1>(E, row, j, M, N, z);
+        else {
+            const float q[1] = {E.bias ? (float)E.bias[j] : 0.f};
+            finish<T, 1, 1>(E, m, 0, j, M, N, z, q);
+        }
     }
 }
 
@@ -900,8 +913,10 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
 #pragma unroll
             for (int e = 0; e < V; ++e) z[0][e] += sums[g * each + x][e];
     }
-    const int64_t line[1] = {i};
-    if (ok) finish<T, V, 1>(E, line, j, M, N, z);
+    if (!ok) return;
+    float q[V] = {};
+    if (E.bias) load_some<T, V>(E.bias + j, N - j, q);
+    finish<T, V, 1>(E, i, 0, j, M, N, z, q);
 }
 
 // What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type, in rows that start on 16 bytes with zeros behind their ends, and its
