@@ -314,7 +314,7 @@ template <typename T> __device__ __forceinline__ void join_columns(const Columns
 // fall on distinct banks.
 //   rows operand     a lane loads 8 neighbours of the contraction at a time; columns operand: 16 or 8 of one line, neighbouring lanes neighbouring lines
 // A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
-// 131072 x 256 x 256: y 117 us (147 Tflop/s; the library's fp32 product 155), with softplus and act' kept 164; dx 114 (154), with a gate 156; dW 107 (319), with a gate and db 131.
+// 131072 x 256 x 256: y 107 us (161 Tflop/s; the library's fp32 product 155), with softplus and act' kept 158; dx 114 (154), with a gate 156; dW 107 (319), with a gate and db 131.
 // 4096 x 4096 x 4096: 780, 660, 680 us (1040); 512 x 512 x 512 11, 12, 12 (20).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (45 us of dx, 65 of y with
 // softplus, by leaving it out) share a compute unit and overlap in part.  Tried and left: the weight's parts made once by a launch of their own and loaded straight into LDS, 165
 // + 5 us of 184 for dx and 180 + 5 of 184 for y; workgroups that start a quarter of a tile apart, no change.
@@ -1021,7 +1021,8 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
     };
     if (es == 4) {
         // 128: 2.8 us a step with two a unit, 2.2 with one, 64: 1.4 with four, 1.1 with two, 0.85 with one -- times 1.2 where one operand comes a column at a time (dx), 1.5 where both do
-        // (dW).  131072 x 256 x 256: tiles of 128 / 64 130 / 134 us for y, 149 / 174 for dx, 125 / 208 for dW; 50000 x 256 x 295: 93 / 73 for y.
+        // (dW).  131072 x 256 x 256: tiles of 128 / 64 107 / 122 us for y, 113 / 127 for dx, 107 / 147 for dW; 50000 x 256 x 295 with softplus: 82 / 73 for y; 52549 x 4927 x 671
+        // 2220 / 2580; 31273 x 418 x 40 45 / 32.
         const int64_t steps = gs::cdiv(K, BK);
         const double slow = columns == 0 ? 1.05 : columns == 1 ? 1.2 : 1.5;
         for (int r = 64; r <= TILE; r += 64) {
@@ -1031,9 +1032,12 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
                 int64_t s = a_unit ? a_unit * CUS / t : 1;          // as many slices as fill the chip with a_unit workgroups each, or one
                 if (a_unit && s > steps / 2) s = steps / 2;          // (steps / 4 costs small training steps 2 %, steps / 8 7 %)
                 if (s < 1 || s > 256) continue;
-                const int64_t wg = t * s, on = gs::cdiv(wg, CUS) < most ? gs::cdiv(wg, CUS) : most;
-                const double us = r == 64 ? (on == 1 ? 0.85 : on == 2 ? 1.1 : 1.4) * slow : (on == 1 ? 2.2 : 2.8);
-                take(r, r, t, s, gs::cdiv(wg, most * CUS) * (gs::cdiv(steps, s) * us + (r == 64 ? 5.0 : 12.0)) + join(s), false);
+                const auto round = [&](int64_t wg) {          // of as many workgroups
+                    const int64_t on = gs::cdiv(wg, CUS);
+                    return wg == 0 ? 0.0 : gs::cdiv(steps, s) * (r == 64 ? (on == 1 ? 0.85 : on == 2 ? 1.1 : 1.4) * slow : (on == 1 ? 2.2 : 2.8)) + (r == 64 ? 5.0 : 11.0);
+                };
+                const int64_t wg = t * s, full = most * CUS;
+                take(r, r, t, s, (wg / full) * round(full) + round(wg % full) + join(s), false);
             }
         }
     } else if (tiles(256, 256) >= 192) {
