@@ -3,7 +3,7 @@
 //
 //     y_t = s W[id_t]                      dW_v = s sum_{t: id_t = v} g_t   (rows that no id names: zero)
 //
-// The gradient's sums are 32-bit, in an order that does not depend on how the launch is scheduled.  Tables of few, narrow rows: partial tables in LDS, added up in their order
+// The gradient's sums are 32-bit, in an order that does not depend on how the launch is scheduled, nor on where g lies.  Tables of few, narrow rows: partial tables in LDS, added up in their order
 // (k_sum_few).  Others: the tokens are sorted by row
 // (a stable radix sort of our own), then every CHUNK neighbours of the sorted list are summed by one group of lanes.  A run of equal rows inside a chunk is written at once;
 // one that crosses chunks leaves a part in each and is joined in a second launch, so that a row that holds most of the tokens is spread over the chip as well.
@@ -327,7 +327,7 @@ template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t*
 // 64 rows a wave, fewer where the waves would be fewer than those of four workgroups a compute unit
 static int rows_a_wave(int64_t V) { return V >= 64 * 4096 ? 64 : V >= 16 * 4096 ? 16 : V >= 4 * 4096 ? 4 : 1; }
 
-// Rows of more than 32 vectors of 16 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
+// Rows of more than 256 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
 // eight rows are on their way at a time.  A run of up to CHUNK tokens is summed as a whole by the chunk where it begins; a longer one leaves a part in each of its chunks.
 // Bound by memory: 65536 tokens of 1024 bf16, their numbers spread like 1 / n over 50000 rows: 61 us for 134 MB of gradient, 102 MB of table and the long runs' parts
 // (3.9 TB/s).
@@ -677,8 +677,11 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
     const int rows = rows_a_wave(V), clear_log = group_log_of(gs::cdiv(D, 16 / sizeof(T)));
     const int64_t zero_blocks = gs::cdiv(V, 4 * rows);
     constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
-    const int vec = vector_of(sizeof(T), D, ldg, g, dw);
-    const bool wide = gs::cdiv(D, vec) > 32;
+    // Which sums: by the row's size alone, not by where g lies (they add the tokens of a long run in different orders).  Rows of 256 .. 512 bytes, 65536 tokens of 128 fp32 over 50000
+    // rows: k_sum_wide with 8 bytes a lane 46 us, k_sum_chunks 49; 262144 of 256 bf16 89 and 102.
+    const int64_t row = D * (int64_t)sizeof(T);
+    const bool wide = row > 256;
+    const int vec = row <= 512 ? V8 : vector_of(sizeof(T), D, ldg, g, dw);
     const int64_t vectors = gs::cdiv(D, BVEC);
     const int gl = group_log_of(vectors);
     const int64_t stretches = gs::cdiv(vectors, 1ll << gl);          // of the narrow sums
