@@ -66,3 +66,23 @@ def test_an_infinite_gradient_passes_where_the_derivative_is_not_zero():
         g[3, 5] = float("inf")
         dx, db = torch.autograd.grad(y, [x, b], g)
         assert (dx[3] == float("-inf")).all() and db[5] == float("inf") and not db[:5].any() and not db[6:].any()
+
+
+@pytest.mark.parametrize("M", [5, 130])
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+def test_gelu_of_16_bit_layers_is_relative_in_its_tail(kind, M):
+    """Phi(z) is 2^-14 of itself there and the exponential 4 w z^2 / 2; the result is rounded once, fp16's below 2^-14 by half of 2^-24."""
+    from gshell_amd import nn
+    dtype = TYPES[kind]
+    u = torch.finfo(dtype).eps / 2
+    z = column_inputs(-8.0, -3.0, dtype, N=512)
+    w = torch.zeros(512, 8, dtype=dtype)
+    w[:, 0] = z
+    x = torch.zeros(M, 8, dtype=dtype)
+    x[:, 0] = 1
+    got = nn.linear(x.to(DEV), w.to(DEV), activation="gelu").cpu().double()
+    ref, _ = tail("gelu", z.double(), 1.0)
+    # the approximation shows where the rounding to the layer's type does not hide it: it moves a result by one step at most, and only next to a border between two
+    err = (got - ref).abs()
+    bar = (u + 2.0 ** -14 + 2 * W * z.double() ** 2 + 16 * W) * ref.abs() + (2.0 ** -25 if kind == "fp16" else 0)
+    assert (err <= bar).all(), float((err / bar).max())
