@@ -74,14 +74,23 @@ template <bool FAST> __device__ __forceinline__ void act_relu(float z, float& y,
     y = z < 0.f ? 0.f : z;
     d = z <= 0.f ? 0.f : 1.f;
 }
+// softplus's constants: log2(e) beta in two parts (48 bits), 2 / beta
+struct Beta {
+    float log2e, low, two_over;
+};
 // With t = exp(-|beta z|) in [0, 1] (neither end of z overflows): log(1 + t) = 2 artanh(q), q = t / (2 + t) <= 1/3, as q times a polynomial in q^2 (fitted at Chebyshev's
-// points, relative error 4e-9), and one reciprocal of (1 + t)(2 + t) serves that and the derivative.  The exponent is rounded once, as beta z is.
-__device__ __forceinline__ void act_softplus(float beta_log2e, float two_over_beta, float z, float& y, float& d) {
-    const float t = __builtin_amdgcn_exp2f(-fabsf(beta_log2e * z));
-    const float u = 1.f + t, v = 2.f + t, r = rcp_(u * v), q = t * (r * u), w = q * q;
+// points, relative error 8e-9), and one reciprocal of (1 + t)(2 + t) serves that and the derivative.  Where p is infinite r is nonsense, but t is zero.
+template <bool FAST> __device__ __forceinline__ void act_softplus(const Beta& beta, float z, float& y, float& d) {
+    const float a = fabsf(z), p = beta.log2e * a;
+    float t = __builtin_amdgcn_exp2f(-p);
+    if (!FAST) {
+        const float r = __builtin_fmaf(a, beta.low, __builtin_fmaf(a, beta.log2e, -p));
+        t = __builtin_fmaf(t, __builtin_amdgcn_fmed3f(r * -0.69314718f, -1.f, 1.f), t);
+    }
+    const float u = 1.f + t, v = 2.f + t, k = rcp_(u * v), q = t * (k * u), w = q * q;
     const float s = fmaf(fmaf(fmaf(fmaf(0.14087328f, w, 0.13980709f), w, 0.20012426f), w, 0.33333158f), w, 1.f);
-    y = fmaf(q * s, two_over_beta, fmaxf(z, 0.f));
-    d = (z >= 0.f ? 1.f : t) * (r * v);
+    y = fmaf(q * s, beta.two_over, fmaxf(z, 0.f));
+    d = (z >= 0.f ? 1.f : t) * (k * v);
 }
 template <bool FAST> __device__ __forceinline__ void act_silu(float z, float& y, float& d) {
     const float s = rcp_(1.f + exp_<FAST>(-z));
@@ -106,7 +115,7 @@ template <bool FAST> __device__ __forceinline__ void act_gelu(float z, float& y,
     d = fmaf(z, e * 0.39894228040143268f, phi);
 }
 // BATCH x V values at once: the choice is the same for the whole launch
-template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, float beta_log2e, float two_over_beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
+template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(int act, const Beta& beta, float (&z)[BATCH][V], float (&d)[BATCH][V]) {
     switch (act) {
         case ACT_RELU:
 #pragma unroll
@@ -114,7 +123,7 @@ template <bool FAST, int V, int BATCH> __device__ __forceinline__ void act_eval(
             break;
         case ACT_SOFTPLUS:
 #pragma unroll
-            for (int k = 0; k < V * BATCH; ++k) act_softplus(beta_log2e, two_over_beta, z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
+            for (int k = 0; k < V * BATCH; ++k) act_softplus<FAST>(beta, z[k / V][k % V], z[k / V][k % V], d[k / V][k % V]);
             break;
         case ACT_SILU:
 #pragma unroll
@@ -134,7 +143,7 @@ template <typename T> struct Epilogue {
     float* part;                                    // not null: fp32 sums of this slice of the contraction go to part[split][M][N], nothing else is done
     int64_t ldr, ldo;
     int act;
-    float beta_log2e, two_over_beta;          // of softplus
+    Beta beta;          // of softplus
 };
 
 template <typename T, int V> struct __attribute__((packed)) Pack { T v[V]; };          // rows start at any element: the hardware takes unaligned vectors
@@ -189,7 +198,7 @@ __device__ __forceinline__ void finish(const Epilogue<T>& E, int64_t i, int64_t 
             for (int k = 0; k < V; ++k) z[b][k] += q[k];
     if (E.act != ACT_NONE) {
         float d[BATCH][V];
-        act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta_log2e, E.two_over_beta, z, d);
+        act_eval<sizeof(T) == 2, V, BATCH>(E.act, E.beta, z, d);
         if (E.dact) {
             auto* p = E.dact + i * N + j;
 #pragma unroll
@@ -1189,6 +1198,11 @@ static int64_t forward_bytes(int es, const Line& x, const Line& w, int64_t M, in
     return packed_bytes(es, x, M) + packed_bytes(es, w, N) + plan(es, 0, M, N, K, false).bytes;
 }
 
+static Beta beta_of(float beta) {
+    const double c = (double)beta * 1.4426950408889634;
+    return {(float)c, (float)(c - (double)(float)c), 2.f / beta};
+}
+
 template <typename T>
 int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* res, int64_t ldr, int64_t M, int64_t N, int64_t K, int act,
                float beta, void* y, int64_t ldy, void* dact, void* ws, int64_t ws_bytes, hipStream_t stream) {
@@ -1197,7 +1211,7 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const voi
     GS_REQUIRE(ws_bytes >= need && (ws || need == 0), "gs_linear_fwd: workspace too small");
     GS_REQUIRE(((uintptr_t)ws & 15) == 0, "gs_linear_fwd: the workspace must start on 16 bytes");
     char* at = (char*)ws;
-    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta * 1.44269504f, act == ACT_SOFTPLUS ? 2.f / beta : 0.f};
+    Epilogue<T> E{(const T*)bias, (const T*)res, (T*)y, (typename dact_type<T>::type*)dact, nullptr, ldr, ldy, act, beta_of(act == ACT_SOFTPLUS ? beta : 1.f)};
     if (few_rows(M, N)) return product_rows<T>(lx, lw, M, N, K, E, at, stream);
     Pack2<T> P{};
     at += repack<T>(P, 0, lx, M, at);

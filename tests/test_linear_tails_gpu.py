@@ -30,7 +30,7 @@ def column_inputs(lo, hi, dtype, N=96, scale=1.0):
 
 @pytest.mark.parametrize("M", [24, 200])
 @pytest.mark.parametrize("act,beta,lo,hi", [("softplus", 1.0, -22.0, -12.0), ("softplus", 1.0, -85.0, -20.0), ("softplus", 100.0, -0.85, -0.12), ("silu", 1.0, -85.0, -9.0), ("gelu", 1.0, -12.5, -4.0)])
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
 def test_gradients_of_saturated_columns(kind, act, beta, lo, hi, M):
     """act' reaches the backward pass with half a step of the layer's type (fp32: as it is) and is off by itself by the exponent's roundings, 4 w |exponent|, and 32 w (exponential,
     reciprocal, polynomial: some ten roundings).  16-bit gelu's Phi, 4e-5 of itself, is at most a tenth of z pdf here.  dW takes gz rounded once more, db does not."""
@@ -50,8 +50,10 @@ def test_gradients_of_saturated_columns(kind, act, beta, lo, hi, M):
     exponent = (z.double() ** 2 / 2) if act == "gelu" else (beta * z.double()).abs()
     ref = g.double().sum(0) * d
     kept = (u if kind == "bf16" else 0) + 4 * W * exponent + 32 * W + 1e-5 * (act == "gelu" and kind == "bf16")
-    for got, extra in ((db, 0), (dw[:, 0], u)):
-        bar = (kept + extra + u + M * W) * 1.01 * ref.abs()
+    # fp32 products: a value's three bf16 parts count where they are 2^-126 or more, so a term lacks at most two parts of less than that
+    lost = M * 2.0 ** -125 if kind == "fp32" else 0
+    for got, extra, low in ((db, 0, 0), (dw[:, 0], u, lost)):
+        bar = (kept + extra + u + M * W) * 1.01 * ref.abs() + low
         assert ((got - ref).abs() <= bar).all(), float(((got - ref).abs() / ref.abs()).max())
 
 
@@ -86,3 +88,34 @@ def test_gelu_of_16_bit_layers_is_relative_in_its_tail(kind, M):
     err = (got - ref).abs()
     bar = (u + 2.0 ** -14 + 2 * W * z.double() ** 2 + 16 * W) * ref.abs() + (2.0 ** -25 if kind == "fp16" else 0)
     assert (err <= bar).all(), float((err / bar).max())
+
+
+@pytest.mark.parametrize("M", [5, 130])
+@pytest.mark.parametrize("beta", [1.0, 3.0, 100.0])
+def test_fp32_softplus_is_relative_in_its_tail(beta, M):
+    """exp2, the reciprocal (one step each), the polynomial (2^-26) and some ten roundings: 24 w of the result, wherever the exponent is; results below
+    2^-126 are multiples of 2^-149."""
+    from gshell_amd import nn
+    z = column_inputs(-85.0, -2.0, torch.float32, N=768, scale=1 / beta)
+    w = torch.zeros(768, 8)
+    w[:, 0] = z
+    x = torch.zeros(M, 8)
+    x[:, 0] = 1
+    got = nn.linear(x.to(DEV), w.to(DEV), activation="softplus", beta=beta).cpu().double()
+    ref, _ = tail("softplus", z.double(), beta)
+    assert ((got - ref).abs() <= 24 * W * ref + 2.0 ** -149).all(), float(((got - ref).abs() / ref).max() / W)
+
+
+def test_softplus_ends():
+    from gshell_amd import nn
+    inf = float("inf")
+    z = torch.tensor([inf, -inf, float("nan"), 3e38, -3e38, 0.0, 1e-30, -1e-30], device=DEV)
+    for beta in (1.0, 100.0, 1e-3):
+        w = torch.ones(1, 1, device=DEV)
+        x = z[:, None].clone().requires_grad_(True)
+        y = nn.linear(x, w, activation="softplus", beta=beta)
+        dx, = torch.autograd.grad(y.sum(), x)
+        y, dx = y[:, 0].detach().cpu().double(), dx[:, 0].cpu().double()
+        ref, d = torch.logaddexp(torch.zeros(8, dtype=torch.float64), z.cpu().double() * beta) / beta, torch.sigmoid(z.cpu().double() * beta)
+        assert torch.allclose(y, ref, rtol=1e-5, equal_nan=True), (beta, y, ref)
+        assert torch.allclose(dx, d, rtol=1e-5, equal_nan=True), (beta, dx, d)
