@@ -9,7 +9,8 @@
 // fp32 operands are split into three bf16 parts, x = x1 + x2 + x3 (each part the rounding of what the ones before left: 24 bits and more in all,
 // and bf16 has fp32's exponents), and six products are summed, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1; the three left out are below
 // 2^-25 |x y| each.  That is 1 / 6 of the bf16 rate, where the fp32 matrix instruction has 1 / 16.  An infinity has no such split (inf * 0): a sum
-// that comes out non-finite is done again with fp32 multiply-adds (131072 x 256 x 256 of nothing but NaN: 15 ms).  The matrix cores take parts below 2^-126 as zero: operands
+// that comes out non-finite is done again with the fp32 matrix instruction (nothing but NaN takes 4 .. 10 times an ordinary product: y of 131072 x 256 x 256 0.6 ms, of
+// 8192 x 4096 x 4096 8.3 ms; a sum a lane took 100 times).  The matrix cores take parts below 2^-126 as zero: operands
 // below 2^-112 keep fewer bits, 2^-17 at 2^-118.
 #include <hip/hip_runtime.h>
 
@@ -243,9 +244,8 @@ template <int TM> __device__ __forceinline__ void put_sums(const f32x4 (&acc)[TM
 }
 // Lines l_begin .. l_end of them, BATCH lines a lane side by side, as many as the registers hold (one with tiles of 256): what they read of the residual is in flight together.
 // A stretch inside of the output goes without checks (131072 x 256 x 256 fp32: y with softplus 164 us for 170, dx 156 for 165, dW 131 for 134).
-// fix(i, j, z): what a sum is replaced by.
-template <typename T, int BATCH, bool ALL, typename F>
-__device__ __forceinline__ void drain_lines(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j, int64_t M, int64_t N, const float (&q)[width<T>()], F& fix) {
+template <typename T, int BATCH, bool ALL>
+__device__ __forceinline__ void drain_lines(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j, int64_t M, int64_t N, const float (&q)[width<T>()]) {
     constexpr int V = width<T>(), LANES = 64 / V, LINES = 64 / LANES;
     const int lane = threadIdx.x & 63, c = lane % LANES * V;
 #pragma unroll 1
@@ -261,7 +261,6 @@ __device__ __forceinline__ void drain_lines(const Epilogue<T>& E, const float* l
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[b][k + e] = s[e];
             }
-            if (ALL || i + b * LINES < M) fix(i + b * LINES, j, z[b]);
         }
         if (E.part) {
 #pragma unroll
@@ -272,18 +271,18 @@ __device__ __forceinline__ void drain_lines(const Epilogue<T>& E, const float* l
         }
     }
 }
-template <typename T, int BATCH, typename F>
-__device__ __forceinline__ void drain_sums(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
+template <typename T, int BATCH>
+__device__ __forceinline__ void drain_sums(const Epilogue<T>& E, const float* lds, int l_begin, int l_end, int64_t i0, int64_t j0, int64_t M, int64_t N) {
     constexpr int V = width<T>(), LANES = 64 / V;
     const int64_t j = j0 + (threadIdx.x & 63) % LANES * V;
     float q[V] = {};
     if (j >= N) return;
     if (E.bias && !E.part) load_some<T, V>(E.bias + j, N - j, q);
-    if (i0 + l_end <= M && j0 + 64 <= N) drain_lines<T, BATCH, true>(E, lds, l_begin, l_end, i0, j, M, N, q, fix);
-    else drain_lines<T, BATCH, false>(E, lds, l_begin, l_end, i0, j, M, N, q, fix);
+    if (i0 + l_end <= M && j0 + 64 <= N) drain_lines<T, BATCH, true>(E, lds, l_begin, l_end, i0, j, M, N, q);
+    else drain_lines<T, BATCH, false>(E, lds, l_begin, l_end, i0, j, M, N, q);
 }
-template <typename T, int TM, int BATCH, typename F>
-__device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&acc)[TM][4], float* lds, int64_t i0, int64_t j0, int64_t M, int64_t N, F fix) {
+template <typename T, int TM, int BATCH>
+__device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&acc)[TM][4], float* lds, int64_t i0, int64_t j0, int64_t M, int64_t N) {
 #pragma unroll 1
     for (int part = 0; part < TM / 4; ++part) {
 #pragma unroll
@@ -291,7 +290,7 @@ __device__ __forceinline__ void store_wave(const Epilogue<T>& E, const f32x4 (&a
             if (p == part) put_sums<TM>(acc, 4 * p, lds);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        drain_sums<T, BATCH>(E, lds, 0, 64, i0 + part * 64, j0, M, N, fix);
+        drain_sums<T, BATCH>(E, lds, 0, 64, i0 + part * 64, j0, M, N);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -446,6 +445,41 @@ template <bool COLS, bool GATE, int LINES> struct Feed32 {
     }
 };
 
+// The sums of 16 x 16 outputs (i, j ..) by the fp32 matrix instruction, straight from memory, 64 of the contraction on their way at a time; what is outside counts as zero.  A
+// function of its own, called where there are infinities or NaN: its registers are not the products'.
+template <bool COLS> __device__ __forceinline__ void load_line(const float* p, int64_t ld, int64_t line, int64_t lines, int64_t c, int64_t c_end, float (&v)[4]) {
+    if constexpr (!COLS) {
+        load_some<float, 4>(p + line * ld + c, line < lines ? c_end - c : 0, v);
+    } else {          // what is outside repeats the last of the contraction or the last line in the load
+        const float* q = p + (line < lines ? line : lines - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = q[(c + e < c_end ? c + e : c_end - 1) * ld];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = line < lines && c + e < c_end ? v[e] : 0.f;
+    }
+}
+template <bool ACOLS, bool BCOLS, bool GATE>
+__device__ __noinline__ f32x4 plain_sums(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t i, int64_t j, int64_t M, int64_t N, int64_t c_begin, int64_t c_end) {
+    constexpr int U = 4;
+    const int lane = threadIdx.x & 63;
+    i += lane & 15, j += lane & 15;
+    f32x4 sum = {};
+    for (int64_t c = c_begin; c < c_end; c += 16 * U) {
+        float a[U][4], b[U][4], d[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t k = c + u * 16 + (lane >> 4) * 4;
+            load_line<ACOLS>(A.p, A.ld, i, M, k, c_end, a[u]);
+            if (GATE) load_line<ACOLS>(gate, ldgate, i, M, k, c_end, d[u]);
+            load_line<BCOLS>(B.p, B.ld, j, N, k, c_end, b[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(b[u][e], GATE ? gated(a[u][e], d[u][e]) : a[u][e], sum, 0, 0, 0);
+    }
+    return sum;
+}
 
 template <bool ACOLS, bool BCOLS, bool GATE, int LINES>
 __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<float> A, const float* gate, int64_t ldgate, Operand<float> B, int64_t M, int64_t N, int64_t K, int64_t slice,
@@ -536,36 +570,52 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
             for (int q = 0; q < 256 / LINES; ++q) t += lds.out[threadIdx.x + q * LINES];
             if (GATE && !(fabsf(t) < __builtin_inff())) {          // again, as gated() has it
                 t = 0.f;
-                for (int64_t c = c_begin; c < c_end; ++c) t += gated(A.p[c * A.ld + i0 + threadIdx.x], gate[c * ldgate + i0 + threadIdx.x]);
+                const float *p = A.p + i0 + threadIdx.x, *d = gate + i0 + threadIdx.x;
+                for (int64_t c = c_begin; c < c_end; c += 8) {
+                    float v[8], e[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const int64_t k = c + q < c_end ? c + q : c_end - 1;
+                        v[q] = p[k * A.ld], e[q] = d[k * ldgate];
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) t += c + q < c_end ? gated(v[q], e[q]) : 0.f;
+                }
             }
             column_sums[(int64_t)blockIdx.y * M + i0 + threadIdx.x] = t;
         }
         __syncthreads();
     }
-    const auto fix = [&](int64_t i, int64_t j, auto& z) {
-        // a sum that is not finite is done again without the split, in fp32, and with gated()
-        if (fabsf(z[0]) + fabsf(z[1]) + fabsf(z[2]) + fabsf(z[3]) < __builtin_inff()) return;
-#pragma unroll 1
-        for (int k = 0; k < 4; ++k)
-            if (!(fabsf(z[k]) < __builtin_inff()) && j + k < N) {
-                float t = 0.f;
-                for (int64_t c = c_begin; c < c_end; ++c) {
-                    float a = ACOLS ? A.p[c * A.ld + i] : A.p[i * A.ld + c];
-                    if (GATE) a = gated(a, ACOLS ? gate[c * ldgate + i] : gate[i * ldgate + c]);
-                    t = fmaf(a, BCOLS ? B.p[c * B.ld + j + k] : B.p[(j + k) * B.ld + c], t);
-                }
-                z[k] = t;
+    // sums that are not finite are done again without the split, 16 x 16 of them a time, and with gated()
+    float all = 0.f;
+#pragma unroll
+    for (int u = 0; u < F; ++u)
+#pragma unroll
+        for (int w = 0; w < F; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) all = __builtin_fmaf(acc[u][w][e], 0.f, all);          // zero, or NaN
+    if (__ballot(all != 0.f))
+#pragma unroll
+        for (int u = 0; u < F; ++u)
+#pragma unroll
+            for (int w = 0; w < F; ++w) {
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= !(fabsf(acc[u][w][e]) < __builtin_inff());
+                if (!__ballot(bad)) continue;
+                const f32x4 again = plain_sums<ACOLS, BCOLS, GATE>(A, gate, ldgate, B, i0 + wi + u * 16, j0 + wj + w * 16, M, N, c_begin, c_end);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][w][e] = fabsf(acc[u][w][e]) < __builtin_inff() ? acc[u][w][e] : again[e];
             }
-    };
     if constexpr (LINES == 128) {
-        store_wave<float, 4, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N, fix);
+        store_wave<float, 4, 4>(E, acc, lds.out + wave * 64 * 64, i0 + wi, j0 + wj, M, N);
     } else {          // the four waves' sums side by side, then 16 lines each
 #pragma unroll
         for (int u = 0; u < F; ++u)
 #pragma unroll
             for (int w = 0; w < F; ++w) *(f32x4*)(lds.out + piece_of_sums(wi + u * 16 + (lane & 15), wj / 4 + w * 4 + (lane >> 4))) = acc[u][w];
         __syncthreads();
-        drain_sums<float, 4>(E, lds.out, wave * 16, wave * 16 + 16, i0, j0, M, N, fix);
+        drain_sums<float, 4>(E, lds.out, wave * 16, wave * 16 + 16, i0, j0, M, N);
     }
 }
 
@@ -718,7 +768,7 @@ __global__ void __launch_bounds__(BM / WM * (BN / WN) * 64, 2) k_product16(Opera
     static_assert(WN == 64 && BUFFER * 2 * 2 == THREADS / 64 * 64 * 64 * 4, "LDS for the sums");
     constexpr int SHARE = THREADS / 64 / 2;
     short* mine = wave < SHARE ? s0 : s1;
-    store_wave<T, TM, (TM > 4 ? 1 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+    store_wave<T, TM, (TM > 4 ? 1 : 4)>(E, acc, (float*)mine + wave % SHARE * 64 * 64, i0 + wi, j0 + wj, M, N);
 #endif
 }
 
@@ -810,7 +860,7 @@ __global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand
             }
     }
     __syncthreads();
-    drain_sums<T, 4>(E, sums, half * 32, half * 32 + 32, i0 + wi, j0 + wj, M, N, [](int64_t, int64_t, auto&) {});
+    drain_sums<T, 4>(E, sums, half * 32, half * 32 + 32, i0 + wi, j0 + wj, M, N);
 #endif
 }
 
