@@ -1118,7 +1118,6 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
         p.rows = p.cols = 256, p.tiles = tiles(256, 256);
     } else if (tiles(TILE, TILE) > CUS) {
         p.tiles = tiles(TILE, TILE);
-        if (p.tiles < 2 * CUS && K >= 1024) p.splits = 2 * CUS / p.tiles;
     } else {
         // 0.5 us a step for 128 rows (2048 x 2048 x 2048: 22 us), 0.37 us for 64 (512 x 4096 x 4096: 27 us)
         const int64_t steps = gs::cdiv(K, STEP);
