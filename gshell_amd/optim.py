@@ -97,6 +97,12 @@ def _norm_code(norm_type, what):
     return code
 
 
+def takes(tensors):
+    """Whether the calls below take these gradients: dense float32, bfloat16 or float16, in HBM and on one device, none of them twice."""
+    return len({t.get_device() for t in tensors}) <= 1 and all(t.layout is torch.strided and t.is_cuda and t.dtype in _GRAD_TYPES for t in tensors) \
+        and len({t.data_ptr() for t in tensors if t.numel()}) == sum(1 for t in tensors if t.numel())
+
+
 def _refuse_grads(tensors, what):
     for t in tensors:
         if t.layout is not torch.strided or t.dtype not in _GRAD_TYPES:

@@ -15,7 +15,7 @@ import torch
 import torch.distributed as dist
 
 from .denoiser.denoiser import BilateralDenoiser
-from .optim import HipAdam, clip_grad_norm_
+from .optim import HipAdam, clip_grad_norm_, takes
 from .geometry.gshell_tets_geometry import GShellTetsGeometry
 from .render import light, mlptexture, render
 from .render import rast as dr
@@ -246,8 +246,10 @@ class Trainer:
             enc.grad /= 8.0                                            # train script :435
         if self.FLAGS.clip_max_norm > 0.0:                            # train script :440-444 (after the all-reduce: global gradient)
             # ONE joint norm over geometry + material parameters, as the reference's clip_grad_norm_(geometry.parameters() + params)
-            # (two HIP launches over the list: gshell_amd/optim.py)
-            clip_grad_norm_(list(self.geometry.parameters()) + list(self.mat_params), self.FLAGS.clip_max_norm)
+            # (two HIP launches over the list: gshell_amd/optim.py; a list with other gradients in it -- float64, sparse, off the GPU -- by torch)
+            params = list(self.geometry.parameters()) + list(self.mat_params)
+            clip = clip_grad_norm_ if takes([p.grad for p in params if p.grad is not None]) else torch.nn.utils.clip_grad_norm_
+            clip(params, self.FLAGS.clip_max_norm)
         self.opt_mat.step(); self.scheds[0].step()
         self.opt_mesh.step(); self.scheds[1].step()
         self.opt_light.step(); self.scheds[2].step()
