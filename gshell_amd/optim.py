@@ -175,7 +175,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)) -> norm, one fp32 value on the device.  Without `out`, in place.
 
     `out`: tensors of the gradients' shapes and types; one may be its gradient's own place, otherwise no output shares memory with a gradient or another output (such a
-    call is refused; of outputs that are not contiguous the same one twice).  A norm that is NaN makes every output NaN, one that is infinite makes finite elements zero."""
+    call is refused; of outputs that are not contiguous the same one twice, and expanded views).  A norm that is NaN makes every output NaN, one that is infinite makes finite elements zero."""
     code = _norm_code(norm_type, "clip_grads")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
@@ -201,6 +201,8 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         apart = [o.data_ptr() for o, c in zip(out, whole) if not c]
         if len(set(apart)) != len(apart):
             raise _lib.GShellHipError("clip_grads: the same output twice")
+        if any(n > 1 and step == 0 for o, c in zip(out, whole) if not c for n, step in zip(o.shape, o.stride())):
+            raise _lib.GShellHipError("clip_grads: elements of an output share a place (an expanded view)")
         dst = src if out is grads else [o if c else torch.empty_like(o, memory_format=torch.contiguous_format) for o, c in zip(out, whole)]
         norm = _launch_norm(src, dst, types, max_norm, code)
         for o, d in zip(out, dst):
