@@ -28,6 +28,17 @@ def _at(t):
     return 0 if t is None else t.data_ptr()
 
 
+def _within(t):
+    """What a tensor that outlived a transform of torch.func holds (it has no storage of its own), any other one as it is."""
+    for held in (lambda: t, lambda: t.view_as(t)):
+        try:
+            held().data_ptr()
+            return held()
+        except RuntimeError:
+            pass
+    return t
+
+
 def _rows(t):
     """`t` [rows, n] with contiguous rows, and the stride between them (a copy only where a row's elements are apart)."""
     ld, step = t.stride()
@@ -178,10 +189,16 @@ def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
         rows = xs[:-1].numel()
         x = x.reshape(rows, ws[1])
         residual = None if residual is None else residual.reshape(rows, ws[0])
-    if grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:          # (forward-mode differentiation is refused there)
-        y = (_LinearFn.apply if _transforms_active() else _linear_apply)(x, weight, bias, residual, act, beta)
-    else:
-        y = _linear_forward(x, weight, bias, residual, act, beta, False)[0]
+    try:
+        if grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:          # (forward-mode differentiation is refused there)
+            y = (_LinearFn.apply if _transforms_active() else _linear_apply)(x, weight, bias, residual, act, beta)
+        else:
+            y = _linear_forward(x, weight, bias, residual, act, beta, False)[0]
+    except RuntimeError:
+        inner = [t if t is None else _within(t) for t in (x, weight, bias, residual)]
+        if _transforms_active() or all(a is b for a, b in zip(inner, (x, weight, bias, residual))):
+            raise
+        y = linear(*inner, activation, beta)
     return y if flat else y.reshape(xs[:-1] + ws[:1])
 
 
@@ -277,10 +294,16 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
                 raise GShellHipError(f"embedding: {name} must live in HBM (got device {t.device}); the HIP path has no CPU fallback")
         raise GShellHipError(f"embedding: ids are on {ids.device}, the weight on {weight.device}")
     flat = ids if ids.is_contiguous() else ids.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:
-        y = (_EmbeddingFn.apply if _transforms_active() else _embedding_apply)(flat, weight, float(scale), int(padding_idx))
-    else:
-        y = _lookup(flat, weight, float(scale))
+    try:
+        if weight.requires_grad and torch.is_grad_enabled() or _forward_ad._current_level >= 0:
+            y = (_EmbeddingFn.apply if _transforms_active() else _embedding_apply)(flat, weight, float(scale), int(padding_idx))
+        else:
+            y = _lookup(flat, weight, float(scale))
+    except RuntimeError:
+        inner = _within(flat), _within(weight)
+        if _transforms_active() or inner[0] is flat and inner[1] is weight:
+            raise
+        y = embedding(*inner, scale, None if padding_idx < 0 else padding_idx)
     return y if ids.dim() == 1 else y.view(ids.shape + (D,))
 
 
