@@ -863,7 +863,8 @@ int gs_flexi_cut_bwd(const int64_t* pa, const int64_t* pb, int64_t n, const floa
  *   dact [M,N] (contiguous; null = not wanted) receives act'(z) for gs_linear_bwd: fp32, for bf16 layers 16 bits an element in a code of the two
  *   functions' own (11 bits from 2^-14 on, 8 down to 2^-126).
  *   gs_linear_bwd: gz = g act'(z) -> dx = gz W [M,K], dW = gz^T x [N,K], db = column sums of gz; any of the three may be null.
- *   dact null = no activation; where act'(z) is exactly zero nothing passes, whatever g is.  M, N, K < 2^31; N, K < 2^21 for 16-bit layers.  Sums are taken in a fixed order: the same bits every time.
+ *   dact null = no activation; where act'(z) is exactly zero nothing passes, whatever g is.  M, N, K < 2^31; N, K < 2^21 for 16-bit layers.  Sums are taken in a fixed order: the same bits every time
+ *   (db's order goes by which of dx and dW are wanted beside it).
  *   The workspaces are the caller's, start on 16 bytes and hold nothing between calls; their sizes go by the addresses and strides too (16-bit operands
  *   whose rows do not start on 16 bytes are repacked first).
  * ---------------------------------------------------------------------------------- */
