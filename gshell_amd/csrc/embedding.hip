@@ -217,19 +217,6 @@ template <typename T, int VEC, typename U> __device__ __forceinline__ void store
     }
 }
 
-// The same; `through`: beside the caches, where they are 16 bytes.
-template <typename T, int VEC, typename U> __device__ __forceinline__ void store_row(T* p, int64_t left, const U (&in)[VEC], bool through) {
-    if (through && left >= VEC && VEC * sizeof(T) == 16) {
-        typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t Words;
-        Pack<T, VEC> q;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) q.v[k] = (T)in[k];
-        if constexpr (VEC * sizeof(T) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words, q), (Words*)p);
-    } else {
-        store_row<T, VEC>(p, left, in);
-    }
-}
-
 // Forward: the output is one stretch of memory, written 16 aligned bytes a lane and piece; LOOKUPS pieces a lane are on their way together.  A piece inside a row is one load (at
 // whatever address the row has it), one that runs over a row's end is gathered.  The place of a lane's next piece comes without a division: step_rows, step_cols are
 // what a workgroup's pieces of one round cover.
@@ -308,7 +295,7 @@ constexpr int BVEC = 4;          // columns of a lane in the sums of narrow rows
 
 // Rows of the table that no token names: `rows` of them a wave from v0 on, 64 at most, 2^group_log lanes a row
 // (6 tokens of 3389 fp32 over 1801 rows: 15 us with one row a wave, 80 with 64)
-template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int64_t v0, int rows, int group_log, bool through, T* dw) {
+template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t* keys, int64_t tokens, int64_t V, int64_t D, int64_t v0, int rows, int group_log, T* dw) {
     constexpr int VEC = 16 / sizeof(T);
     const int lane = threadIdx.x & 63, group = 1 << group_log;
     const int64_t v = v0 + lane;
@@ -322,20 +309,20 @@ template <typename T> __device__ __forceinline__ void clear_rows(const uint32_t*
     const float zero[VEC] = {};
     for (int r = lane >> group_log; r < rows; r += 64 >> group_log)
         if (which >> r & 1)
-            for (int64_t c = (lane & (group - 1)) * VEC; c < D; c += group * VEC) store_row<T, VEC>(dw + (v0 + r) * D + c, D - c, zero, through);
+            for (int64_t c = (lane & (group - 1)) * VEC; c < D; c += group * VEC) store_row<T, VEC>(dw + (v0 + r) * D + c, D - c, zero);
 }
 // 64 rows a wave, fewer where the waves would be fewer than those of four workgroups a compute unit
 static int rows_a_wave(int64_t V) { return V >= 64 * 4096 ? 64 : V >= 16 * 4096 ? 16 : V >= 4 * 4096 ? 4 : 1; }
 
 // Rows of more than 256 bytes: a wave takes one (chunk, stretch of columns), and its lanes hold the chunk's rows and numbers, so that every choice is a scalar one and
 // eight rows are on their way at a time.  A run of up to CHUNK tokens is summed as a whole by the chunk where it begins; a longer one leaves a part in each of its chunks.
-// Bound by memory: 65536 tokens of 1024 bf16, their numbers spread like 1 / n over 50000 rows: 61 us for 134 MB of gradient, 102 MB of table and the long runs' parts
-// (3.9 TB/s).
+// Bound by memory: 65536 tokens of 1024 bf16, their numbers spread like 1 / n over 50000 rows: 75 us for 134 MB of gradient, 102 MB of table and the long runs' parts
+// (3.2 TB/s).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int64_t stretches,
-                                                  int64_t chunks, int64_t sum_blocks, int rows, int clear_log, bool through, float scale, T* dw, float* first, float* last) {
+                                                  int64_t chunks, int64_t sum_blocks, int rows, int clear_log, float scale, T* dw, float* first, float* last) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + wave) * rows, rows, clear_log, through, dw);
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + wave) * rows, rows, clear_log, dw);
     const int64_t unit = (int64_t)blockIdx.x * 4 + wave;
     if (unit >= chunks * stretches) return;
     const int64_t chunk = unit / stretches, c = (unit % stretches * 64 + lane) * VEC, e0 = chunk * CHUNK;
@@ -382,7 +369,7 @@ __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const ui
             } else {
 #pragma unroll
                 for (int q = 0; q < VEC; ++q) acc[q] *= scale;
-                store_row<T, VEC>(dw + (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j + k) * D + c, D - c, acc, through);
+                store_row<T, VEC>(dw + (int64_t)(uint32_t)__builtin_amdgcn_readlane(key, j + k) * D + c, D - c, acc);
             }
 #pragma unroll
             for (int q = 0; q < VEC; ++q) acc[q] = 0.f;
@@ -393,8 +380,8 @@ __global__ void __launch_bounds__(256) k_sum_wide(const uint32_t* keys, const ui
 // Narrower rows: several groups of lanes a wave, a chunk each, 25 us for 262144 tokens of 64 bf16 over 160 rows; every run that crosses chunks leaves its parts.  Blocks below `sum_blocks` sum chunks, the others write the rows that no token names.
 template <typename T>
 __global__ void __launch_bounds__(256) k_sum_chunks(const uint32_t* keys, const uint32_t* pos, const T* g, int64_t ldg, int64_t tokens, int64_t V, int64_t D, int group_log,
-                                                    int64_t stretches, int64_t chunks, int64_t sum_blocks, int rows, int clear_log, bool through, float scale, T* dw, float* first, float* last) {
-    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * rows, rows, clear_log, through, dw);
+                                                    int64_t stretches, int64_t chunks, int64_t sum_blocks, int rows, int clear_log, float scale, T* dw, float* first, float* last) {
+    if ((int64_t)blockIdx.x >= sum_blocks) return clear_rows<T>(keys, tokens, V, D, (((int64_t)blockIdx.x - sum_blocks) * 4 + (threadIdx.x >> 6)) * rows, rows, clear_log, dw);
     const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> group_log;
     if (unit >= chunks * stretches) return;
     const int64_t chunk = unit / stretches, c = ((unit % stretches) << group_log) * BVEC + (threadIdx.x & ((1 << group_log) - 1)) * BVEC;
@@ -671,9 +658,8 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
     if (tokens > 0)
         if (const int rc = sort_tokens<I>(ids, tokens, V, padding, p, base, keys, pos, stream)) return rc;
     float *first = (float*)(base + p.first), *last = (float*)(base + p.last);
-    // A large table's gradient goes past the caches, where it would take the place of the gradient that is read, and of most of itself: 65536 tokens of 1024 bf16 over 50000 rows
-    // (102 MB) 61 us for 75.  A small one stays for its next reader.
-    const bool through = V * D * (int64_t)sizeof(T) >= 64 << 20;
+    // The gradient stays in the caches for its next reader.  Written past them it is alone 2 .. 30 % faster (82 MB 92 us for 109, 164 MB 104 for 132), but 2 .. 6 % slower with the
+    // clipping behind it (149 for 146, 203 for 195), and with clipping and HipAdam (355 for 349, 513 for 504).
     const int rows = rows_a_wave(V), clear_log = group_log_of(gs::cdiv(D, 16 / sizeof(T)));
     const int64_t zero_blocks = gs::cdiv(V, 4 * rows);
     constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
@@ -690,12 +676,12 @@ int gradient(const void* ids, const void* g, int64_t ldg, int64_t tokens, int64_
         GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         const auto kernel = vec == V16 ? k_sum_wide<T, V16> : k_sum_wide<T, V8>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
-                           across, p.chunks, sum_blocks, rows, clear_log, through, scale, (T*)dw, first, last);
+                           across, p.chunks, sum_blocks, rows, clear_log, scale, (T*)dw, first, last);
     } else {
         const int64_t sum_blocks = gs::cdiv((p.chunks * stretches) << gl, 256);
         GS_REQUIRE(sum_blocks + zero_blocks < (1ll << 24), "gs_embedding_bwd: too large for one launch");
         hipLaunchKernelGGL(k_sum_chunks<T>, dim3((unsigned)(sum_blocks + zero_blocks)), dim3(256), 0, stream, (const uint32_t*)keys, (const uint32_t*)pos, (const T*)g, ldg, tokens, V, D,
-                           gl, stretches, p.chunks, sum_blocks, rows, clear_log, through, scale, (T*)dw, first, last);
+                           gl, stretches, p.chunks, sum_blocks, rows, clear_log, scale, (T*)dw, first, last);
     }
     if (p.chunks > 1) {
         // groups cover a whole row; a run may hold most of the tokens: a large workgroup where rows are used a thousand times and more
