@@ -869,7 +869,7 @@ __global__ void __launch_bounds__(BM * 4) k_product16_deep(Operand<T> A, Operand
 // CHUNK, and fragments come straight from memory: each matrix instruction takes 16 bytes a lane of 16 rows of W, so W is read once, with nothing staged, and the loads of the
 // next stretch are on their way while one is multiplied.  16-bit: one instruction a load; fp32: the fp32 matrix instruction four times (its rate does not matter here, and it
 // rounds like a chain of fused multiply-adds).  The waves' sums meet in LDS.
-// 1 x 4096 x 4096 bf16 9.7 us, 24 rows of 8192 -> 2048 fp16 with bias and silu 10.2: 33.6 MB, 6.5 us of a large copy's rate, and a launch; all of W is asked for at once.
+// 1 x 4096 x 4096 bf16 9.7 us, 24 rows of 2048 -> 8192 fp16 with bias and silu 10.2: 33.6 MB, 6.5 us of a large copy's rate, and a launch; all of W is asked for at once.
 constexpr int ROWS_THREADS = 512, ROWS_WAVES = ROWS_THREADS / 64;
 template <typename T, int MT, int NT>
 __global__ void __launch_bounds__(ROWS_THREADS) k_rows(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int64_t slice, Epilogue<T> E) {
@@ -993,8 +993,10 @@ template <typename T> __global__ void __launch_bounds__(256) k_join(const float*
     finish<T, V, 1>(E, i, 0, j, M, N, z, q);
 }
 
-// What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type, in rows that start on 16 bytes with zeros behind their ends, and its
-// column sums (of the unrounded values) by slabs of rows: 16384 x 4096 bf16 73 us, 402 MB at 5.5 TB/s; 28432 x 6528 260 us, 1.1 GB (one line of a lane at a time 300, four 354).  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
+// What the products read, made in one launch.  Workgroups 0 .. : gz = g act'(z), rounded to the layer's type (the matrix instructions take 16-bit operands, and a
+// second part of gz would double both products; the gradients' error is 1.4 times that of unrounded ones), in rows that start on 16 bytes with zeros behind their ends, and its
+// column sums (of the unrounded values) by slabs of rows: 16384 x 4096 bf16 77 us, 402 MB at 5.2 TB/s (the code of act' taken apart costs 3 us); 28432 x 6528 260 us, 1.1 GB (one line of a lane at a
+// time 300, four 354).  The others repack: operands' rows copied to rows that start on 16 bytes, zeros behind their ends.
 constexpr int GZ_LANES = 32, GZ_LINES = 8, GZ_ROUND = 2 * GZ_LINES;
 template <typename T> struct Gz {
     const T* g;
@@ -1096,7 +1098,8 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
     if (es == 4) {
         // 128: 2.8 us a step with two a unit, 2.2 with one, 64: 1.4 with four, 1.1 with two, 0.85 with one -- times 1.2 where one operand comes a column at a time (dx), 1.5 where both do
         // (dW).  131072 x 256 x 256: tiles of 128 / 64 107 / 122 us for y, 113 / 127 for dx, 107 / 147 for dW; 50000 x 256 x 295 with softplus: 82 / 73 for y; 52549 x 4927 x 671
-        // 2220 / 2580; 31273 x 418 x 40 45 / 32.
+        // 2220 / 2580; 31273 x 418 x 40 45 / 32.  The us are rougher than the differences between the two: over full rounds they favour 64 by up to 14 %, and where the last round
+        // tips the balance (110000 x 256 x 256) the choice may be the slower by 4 % (y 117 / 113, dx 125 / 120).
         const int64_t steps = gs::cdiv(K, BK);
         const double slow = columns == 0 ? 1.05 : columns == 1 ? 1.2 : 1.5;
         for (int r = 64; r <= TILE; r += 64) {
@@ -1115,6 +1118,9 @@ static Plan plan(int es, int columns /* operands that come by columns */, int64_
             }
         }
     } else if (tiles(256, 256) >= 192) {
+        // With tiles of 256 / 128, K 2048: 3584 x 3584 (196 tiles of 256) y 57 / 67 us, 4096 x 4096 (256) 61 / 77, 4096 x 4352 (272, a second round for 16 of them) 103 / 95; below
+        // them 4096 x 2048 over 4096 (128 tiles) 101 / 75.  A few columns leave most of such a tile outside of the output, which the rule does not
+        // look at: 131072 x 64 x 64 21 / 12, 83195 x 62 -> 103 27 / 16.
         p.rows = p.cols = 256, p.tiles = tiles(256, 256);
     } else if (tiles(TILE, TILE) > CUS) {
         p.tiles = tiles(TILE, TILE);
