@@ -337,8 +337,8 @@ template <typename T> __device__ __forceinline__ void join_columns(const Columns
 // fall on distinct banks.
 //   rows operand     a lane loads 8 neighbours of the contraction at a time; columns operand: 16 or 8 of one line, neighbouring lanes neighbouring lines
 // A may have a gate: the factor act'(z) that makes gz of g, so that gz is never stored; the products with dW also add up its columns, for db.
-// 131072 x 256 x 256: y 107 us (161 Tflop/s; the library's fp32 product 155), with softplus and act' kept 158; dx 114 (154), with a gate 156; dW 107 (319), with a gate and db 131.
-// 4096 x 4096 x 4096: 780, 660, 680 us (1040); 512 x 512 x 512 11, 12, 12 (20).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (45 us of dx, 65 of y with
+// 131072 x 256 x 256: y 107 us (161 Tflop/s; the library's fp32 product 155), with softplus and act' kept 164; dx 114 (154), with a gate 156; dW 107 (319), with a gate and db 131.
+// 4096 x 4096 x 4096: 780, 660, 680 us (1040); 512 x 512 x 512 11, 12, 12 (20).  At 131072 rows memory needs 52 .. 78 us and the matrix cores 60; both, the splitting and the epilogue (45 us of dx, 71 of y with
 // softplus, by leaving it out) share a compute unit and overlap in part.  Tried and left: the weight's parts made once by a launch of their own and loaded straight into LDS, 165
 // + 5 us of 184 for dx and 180 + 5 of 184 for y; workgroups that start a quarter of a tile apart, no change.
 constexpr int TILE = 128, BK = 32;
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(256, LINES == 64 ? 4 : 2) k_product32(Operand<
 //   columns operand  LDS holds [64][line]; fragments come out transposed by ds_read_b64_tr_b16 (4 contraction rows x 16 lines a 16-lane group); the 32-byte
 //                    piece q of row k sits at q ^ h(k), with h different for the 16 rows that one instruction reads
 // Lines and contraction beyond the operand are loaded as zero (an offset outside of the buffer's range).
-// 16384 x 4096 x 4096 bf16 with 256 x 256 tiles: y 511 us (1.08 Pflop/s; the library 448), with gelu, residual and act' kept 535; dx 500 (522), dW 442 .. 484 (577).  Four tiles a
+// 16384 x 4096 x 4096 bf16 with 256 x 256 tiles: y 511 us (1.08 Pflop/s; the library 448), with gelu, residual and act' kept 541; dx 500 (522), dW 442 .. 484 (577).  Four tiles a
 // compute unit: what is left is their starts and ends, 15 us each, in which the matrix cores wait; the clock falls with them busy, so less waiting gains less than it
 // takes away.  The next lines' residual loaded ahead in the epilogue: 588 us for 577.  4096 x 2048 x 2048 with 128 x 128 tiles: 39, 40, 41 us (36, 38, 50).
 typedef __attribute__((address_space(3))) void lds_void;
