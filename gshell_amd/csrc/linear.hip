@@ -31,15 +31,15 @@ enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SOFTPLUS = 2, ACT_SILU = 3, ACT_GELU = 4 };
 
 // act'(z) as the forward pass keeps it for the backward pass: fp32 for fp16 and fp32 layers (one more rounding to the layer's own type would cost the gradients as much as their
-// own), 16 bits for bf16 layers.  |act'| <= 1.13, so from 2^-14 on these are fp16's, 11 bits next to bf16's 8; fp16's codes of 2 and above, which no derivative needs, hold
-// the smaller ones as bf16 does, 8 bits down to 2^-126: in fp16 itself they would lose bits from 2^-14 on and be zero below 2^-25 (softplus at beta z = -17.3).
-//   |v| >= 2^-14, NaN: the fp16 of v        smaller: sign, 0x4000 | bf16 of |v| (at most 0x3880: no bit is in the other's place)
+// own), 16 bits for bf16 layers.  |act'| <= 1.13, so down to 2^-14 these are fp16's, 11 bits next to bf16's 8, and down to 2^-17 its subnormals, 8 bits and more; fp16's codes of 2
+// and above, which no derivative needs, hold the smaller ones as bf16 does, 8 bits down to 2^-126: in fp16 itself they would be zero below 2^-25 (softplus at beta z = -17.3).
+//   |v| >= 2^-17, NaN: the fp16 of v        smaller: sign, 0x4000 | bf16 of |v| (at most 0x3700: no bit is in the other's place)
 struct Slope16 {
     uint16_t bits;
     Slope16() = default;
     __device__ __forceinline__ explicit Slope16(float v) {
         const uint16_t small = __builtin_bit_cast(uint16_t, (bf16)v) | 0x4000, large = __builtin_bit_cast(uint16_t, (f16)v);
-        bits = fabsf(v) < 0x1p-14f ? small : large;
+        bits = fabsf(v) < 0x1p-17f ? small : large;
     }
     __device__ __forceinline__ explicit operator float() const {
         const uint32_t small = (uint32_t)(bits & 0xbfff) << 16;
