@@ -9,7 +9,7 @@
 // fp32 operands are split into three bf16 parts, x = x1 + x2 + x3 (each part the rounding of what the ones before left: 24 bits and more in all,
 // and bf16 has fp32's exponents), and six products are summed, x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1; the three left out are below
 // 2^-25 |x y| each.  That is 1 / 6 of the bf16 rate, where the fp32 matrix instruction has 1 / 16.  An infinity has no such split (inf * 0): a sum
-// that comes out non-finite is done again with the fp32 matrix instruction (nothing but NaN takes 4 .. 10 times an ordinary product: y of 131072 x 256 x 256 0.6 ms, of
+// that comes out non-finite is done again with the fp32 matrix instruction (nothing but NaN takes 4 .. 11 times an ordinary product: y of 131072 x 256 x 256 0.6 ms, of
 // 8192 x 4096 x 4096 8.3 ms; a sum a lane took 100 times).  The matrix cores take parts below 2^-126 as zero: operands
 // below 2^-112 keep fewer bits, 2^-17 at 2^-118.
 #include <hip/hip_runtime.h>

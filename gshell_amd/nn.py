@@ -168,7 +168,7 @@ def linear(x, weight, bias=None, residual=None, activation=None, beta=1.0):
     activation: None, "relu", "softplus" (log(1 + exp(beta z)) / beta), "silu" or "gelu" (erf form).  The residual is added behind the activation and has the
     output's shape (an expanded view may stand for it).  All operands have one type (float32, bfloat16, float16) and one device; x, weight and residual may be views whose rows are
     any stride apart.  fp32 operands of 2^-112 and above keep fp32's accuracy; fp32 outputs that meet infinities or NaN are summed a second time, which costs
-    up to ten times the product.  Where the gradient is taken of an activation, act'(z) is kept for the backward pass: 2 bytes an output
+    up to eleven times the product.  Where the gradient is taken of an activation, act'(z) is kept for the backward pass: 2 bytes an output
     for bf16, 4 for the others; where it is exactly zero (relu of z <= 0) nothing passes, an infinite gradient neither.  16-bit layers round
     the gradient times act' to their type before the products of dx and dW, as torch's do."""
     act = ACTIVATIONS.get(activation)

@@ -47,7 +47,7 @@ class HipAdam(torch.optim.Adam):
                 if st.get("_host_step") is None:          # fresh state or one loaded from a checkpoint: read the counter once
                     st["_host_step"] = float(st["step"])
                     # a checkpoint written by torch's default (non-fused) Adam keeps `step` on the CPU: the kernel writes the counter through
-                    # this pointer, so it has to be a float32 scalar on the parameter's device (ADVICE r3)
+                    # this pointer, so it has to be a float32 scalar on the parameter's device
                     if st["step"].device != p.device or st["step"].dtype != torch.float32:
                         st["step"] = st["step"].detach().to(device=p.device, dtype=torch.float32)
                     for name in ("exp_avg", "exp_avg_sq"):

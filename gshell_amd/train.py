@@ -1,7 +1,7 @@
 """One optimisation iteration of G-Shell reconstruction, as the reference's `optimize_mesh` body does it
 (train_gshelltet_deepfashion.py:278-497: zero_grad x3 -> lgt.update_pdf -> geometry.tick -> backward -> gradient
 rescaling -> 3 Adam steps + LambdaLR -> clamps), plus what the reference lacks: view-sharded data parallelism with ONE
-RCCL all-reduce of the flattened gradient per iteration (SURVEY.md 8e).
+RCCL all-reduce of the flattened gradient per iteration.
 
     flags   = default_flags(gshell_grid=..., n_samples=..., batch=..., train_res=[H, W])
     trainer = Trainer(flags, tet_grid=(verts, indices))
@@ -147,7 +147,7 @@ def flat_all_reduce_grads(params, shard, buf=None):
 
 def sharded_total_loss(per_view, global_terms, B_local, B_global, world, presharded=None):
     """Loss a rank back-propagates so that the SUM of all ranks' gradients equals the single-GPU gradient of
-    mean-over-global-batch(per-view terms) + view-independent terms (SURVEY.md 8e).  `presharded` terms are already
+    mean-over-global-batch(per-view terms) + view-independent terms.  `presharded` terms are already
     divided over the ranks by construction (each rank owns a disjoint part of a sum) and enter with weight 1."""
     total = per_view * (B_local / B_global) + global_terms / world
     return total if presharded is None else total + presharded
